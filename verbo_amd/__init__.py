@@ -8,6 +8,13 @@ addresses cross the C ABI.
     ctx = Context()
     ids = ctx.pick_batch(logits, Params(temp=.8, top_k=50), u_mode=U_COUNTER)  # logits: cuda [B,V]
     s = Sampler(temp=.7, seed=42); s.accept(3); tok = s.pick(numpy_row)        # verbo::Sampler
+
+The operators around the pick (include/vsmp_logits.h):
+
+    x = ctx.head_logits_q4(hidden, q, scales, group)                # 4-bit head: cuda [B, D] -> [B, V]
+    x = ctx.adjust_logits(x, Penalty(presence=.5), hist=h, hist_off=o, mask=m, out=x, left=left)
+    ids = ctx.pick_batch(x, Params(temp=.8, top_k=50))
+    logprob, rank, lse = ctx.logprobs(x, ids[:, None])
 """
 import ctypes
 import os
@@ -17,7 +24,7 @@ import numpy as np
 
 from .workloads import SAMPLING_DTYPE
 
-__all__ = ["Context", "Sampler", "Params", "RowInfo", "Debug", "VsmpError", "pick_batch_noalloc", "load_library", "U_SUPPLIED", "U_COUNTER",
+__all__ = ["Context", "Sampler", "Params", "Penalty", "PENALTY_DTYPE", "RowInfo", "Debug", "VsmpError", "pick_batch_noalloc", "load_library", "U_SUPPLIED", "U_COUNTER",
            "U_XORSHIFT", "ROW_INFO_DTYPE", "SAMPLING_DTYPE"]
 __version__ = "0.1.0"
 
@@ -48,6 +55,16 @@ class Params(ctypes.Structure):
 
     def __init__(self, temp=0.7, top_k=40, top_p=0.9, min_p=0.0, repeat=1.0, repeat_last=64, seed=0):
         super().__init__(temp, top_k, top_p, min_p, repeat, repeat_last, seed)
+
+
+class Penalty(ctypes.Structure):
+    """vsmp_penalty: what Context.adjust_logits takes from the logits of ids seen before (off by default)."""
+
+    _fields_ = [("repeat", ctypes.c_float), ("presence", ctypes.c_float), ("frequency", ctypes.c_float),
+                ("window", ctypes.c_int)]
+
+    def __init__(self, repeat=1.0, presence=0.0, frequency=0.0, window=0):
+        super().__init__(repeat, presence, frequency, window)
 
 
 class RowInfo(ctypes.Structure):
@@ -86,6 +103,8 @@ ROW_INFO_DTYPE = np.dtype([("id", "i4"), ("path", "i4"), ("k", "i4"), ("keep_min
                            ("sum", "f8"), ("tot", "f8"), ("u", "f8"), ("draw_margin", "f8")])
 assert ROW_INFO_DTYPE.itemsize == ctypes.sizeof(RowInfo) == 72
 assert SAMPLING_DTYPE.itemsize == ctypes.sizeof(Params) == 32
+PENALTY_DTYPE = np.dtype([("repeat", "f4"), ("presence", "f4"), ("frequency", "f4"), ("window", "i4")])
+assert PENALTY_DTYPE.itemsize == ctypes.sizeof(Penalty) == 16
 
 _lib = None
 _P = ctypes.c_void_p
@@ -144,6 +163,14 @@ def load_library():
         "vsmp_head_pick": (ctypes.c_int, [_P, _P, ctypes.c_longlong, _P, ctypes.c_longlong, ctypes.c_int, ctypes.c_int,
                                           ctypes.c_int, _P, ctypes.c_int, _P, _P, ctypes.c_int, _P, _P,
                                           ctypes.c_ulonglong, _P, _P, ctypes.c_longlong, ctypes.POINTER(Debug), _P]),
+        "vsmp_adjust_logits": (ctypes.c_int, [_P, _P, ctypes.c_int, ctypes.c_longlong, ctypes.c_int, ctypes.c_int, _P,
+                                              ctypes.c_int, _P, _P, _P, _P, _P, _P, _P, ctypes.c_longlong, ctypes.c_int,
+                                              _P, _P, ctypes.c_longlong, _P, _P]),
+        "vsmp_logprobs": (ctypes.c_int, [_P, _P, ctypes.c_int, ctypes.c_longlong, ctypes.c_int, ctypes.c_int, _P,
+                                         ctypes.c_longlong, ctypes.c_int, _P, _P, _P, _P]),
+        "vsmp_head_logits_q4": (ctypes.c_int, [_P, _P, ctypes.c_int, ctypes.c_longlong, _P, ctypes.c_longlong, _P,
+                                               ctypes.c_int, ctypes.c_longlong, _P, ctypes.c_longlong, ctypes.c_int,
+                                               ctypes.c_int, ctypes.c_int, ctypes.c_int, _P, ctypes.c_longlong, _P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -275,6 +302,105 @@ def _head_shapes(hidden, head):
     return hidden.shape[0], hidden.shape[1], head.shape[0]
 
 
+_DTYPES = None  # torch dtype -> vsmp_dtype, once torch is there
+
+
+def _dtype(t, name):
+    global _DTYPES
+    if _DTYPES is None:
+        import torch
+
+        _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise VsmpError(f"{name} must be float32, bfloat16 or float16")
+    return code
+
+
+def _rows_of(t, name, device):
+    """(dtype code, row stride) of a 2-D matrix with contiguous rows on `device` (of a single row: its length)."""
+    code = _dtype(t, name)
+    if t.dim() != 2 or not t.is_cuda or t.device != device:
+        raise VsmpError(f"{name} must be a 2-D tensor on {device}")
+    rows, cols = t.shape
+    sr, sc = t.stride()
+    if cols > 1 and sc != 1:
+        raise VsmpError(f"{name} must have contiguous rows")
+    return code, sr if rows > 1 else cols
+
+
+def _array_of(t, dtype, n, name, device):
+    """The address of a contiguous device array of `dtype` with at least n entries (None stays None)."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.device != device or not t.is_contiguous() or t.numel() < n:
+        raise VsmpError(f"{name} must be a contiguous {dtype} tensor on {device} of at least {n} entries")
+    return t.data_ptr()
+
+
+def to_device_penalties(rows, device="cuda"):
+    """Upload a PENALTY_DTYPE array, or a list of Penalty, as a device byte tensor for per-row penalties."""
+    import torch
+
+    if not isinstance(rows, np.ndarray):
+        rows = np.array([(p.repeat, p.presence, p.frequency, p.window) for p in rows], dtype=PENALTY_DTYPE)
+    a = np.ascontiguousarray(rows, dtype=PENALTY_DTYPE)
+    return torch.from_numpy(a.view(np.uint8).copy()).to(device)
+
+
+def _adjust_args(logits, penalty, hist, hist_off, prompt_len, bias_ids, bias, bias_off, mask, mask_row, out, left, stream,
+                 csr=True):
+    """The arguments of an adjust call as (in, dtype, ldi), (B, V), the penalties, histories, and the rest up to the
+    stream; `out`; and what the addresses need kept alive."""
+    import torch
+
+    dev = logits.device
+    code, ld = _rows_of(logits, "logits", dev)
+    B, V = logits.shape
+    if out is None:  # rows on 16 bytes, so that pick_batch can take them
+        out = torch.empty(B, (V + 3) // 4 * 4, dtype=torch.float32, device=dev)
+        ldo = out.stride(0)
+        out = out[:, :V]
+    else:
+        ocode, ldo = _rows_of(out, "out", dev)
+        if ocode != 0 or out.shape != logits.shape:
+            raise VsmpError("out must be float32 of the logits' shape")
+    i32 = torch.int32
+    if penalty is None or isinstance(penalty, Penalty):
+        pp, per_row = (ctypes.addressof(penalty) if penalty is not None else None), 0
+    else:
+        if penalty.dtype != torch.uint8 or penalty.numel() != 16 * B:
+            raise VsmpError("per-row penalties must hold B entries (to_device_penalties)")
+        pp, per_row = _array_of(penalty, torch.uint8, 16 * B, "per-row penalties", dev), 1
+    if csr:
+        if (hist is None) != (hist_off is None):
+            raise VsmpError("hist and hist_off go together")
+        if hist is not None and hist.numel() == 0:  # every history is empty
+            hist = hist_off = prompt_len = None
+        h, ho = _array_of(hist, i32, 0, "hist", dev), _array_of(hist_off, i32, B + 1, "hist_off", dev)
+    else:
+        h = ho = None
+    if (bias_ids is None) != (bias_off is None) or (bias is None) != (bias_off is None):
+        raise VsmpError("bias_ids, bias and bias_off go together")
+    if bias_ids is not None and bias_ids.numel() == 0:
+        bias_ids = bias = bias_off = None
+    ldm = n_masks = 0
+    mp = None
+    if mask is not None:
+        if mask.dtype != i32 or mask.dim() != 2 or mask.device != dev or mask.stride(1) != 1 or mask.shape[1] < (V + 31) // 32:
+            raise VsmpError("mask must be an int32 tensor [masks, >= ceil(V / 32)] with contiguous rows on the logits' device")
+        n_masks = mask.shape[0]
+        ldm = mask.stride(0) if n_masks > 1 else mask.shape[1]
+        mp = mask.data_ptr()
+    st = stream if stream is not None else torch.cuda.current_stream(dev)
+    rest = (_array_of(prompt_len, i32, B, "prompt_len", dev), _array_of(bias_ids, i32, 0, "bias_ids", dev),
+            _array_of(bias, torch.float32, bias_ids.numel() if bias_ids is not None else 0, "bias", dev),
+            _array_of(bias_off, i32, B + 1, "bias_off", dev), mp, ldm, n_masks,
+            _array_of(mask_row, i32, B, "mask_row", dev), out.data_ptr(), ldo, _array_of(left, i32, B, "left", dev),
+            st.cuda_stream)
+    return (logits.data_ptr(), code, ld), (B, V), (pp, per_row), (h, ho), rest, out
+
+
 class Context:
     """A vsmp_ctx on one device: scratch for batched picks, staging for host picks."""
 
@@ -357,6 +483,99 @@ class Context:
             raise _err()
         del params, dbg
         return out
+
+    def _check_device(self, t):
+        if not t.is_cuda or (self.device >= 0 and t.device.index != self.device):
+            raise VsmpError(f"expected tensors on the context's device ({self.device})")
+
+    def adjust_logits(self, logits, penalty=None, hist=None, hist_off=None, prompt_len=None, bias_ids=None, bias=None,
+                      bias_off=None, mask=None, mask_row=None, out=None, left=None, stream=None):
+        """vsmp_adjust_logits: penalties for repeated tokens, biases and grammar masks on device logits [B, V]
+        (float32, bfloat16 or float16; rows contiguous). `penalty`: a Penalty (shared by all rows) or a device
+        byte tensor from to_device_penalties; hist / hist_off / prompt_len (int32): CSR histories and the length of
+        each one's prompt; bias_ids (int32) / bias (float32) / bias_off (int32): CSR biases; mask (int32 [masks,
+        ceil(V / 32)], bits set for allowed tokens) and mask_row (int32 [B], negative: none). `out`: None, a float32
+        [B, V] tensor, or `logits` itself; `left`: None, or int32 [B] for the number of tokens left in each row.
+        Returns `out`, whose rows pick_batch can take."""
+        self._check_device(logits)
+        x, shape, pen, hists, rest, out = _adjust_args(logits, penalty, hist, hist_off, prompt_len, bias_ids, bias, bias_off,
+                                                       mask, mask_row, out, left, stream)
+        if _lib.vsmp_adjust_logits(self._h, *x, *shape, *pen, *hists, *rest) != 0:
+            raise _err()
+        return out
+
+    def logprobs(self, logits, ids=None, rank=True, stream=None):
+        """vsmp_logprobs: the log-probabilities of ids (int32 [B, n], n <= 64, rows contiguous) under the softmax of
+        device logits [B, V] (float32, bfloat16 or float16), their ranks in the sampler's order (rank=False: None)
+        and each row's log of the sum of exponentials. Ids outside [0, V) give -inf and rank -1. Returns (logprob
+        float32 [B, n], rank int32 [B, n], lse float32 [B]); without ids the first two are None."""
+        import torch
+
+        self._check_device(logits)
+        dev = logits.device
+        code, ld = _rows_of(logits, "logits", dev)
+        B, V = logits.shape
+        lse = torch.empty(B, dtype=torch.float32, device=dev)
+        lp = rk = None
+        n = ldj = 0
+        if ids is not None:
+            if ids.dtype != torch.int32 or ids.dim() != 2 or ids.shape[0] != B or ids.device != dev:
+                raise VsmpError("ids must be an int32 tensor [B, n] on the logits' device")
+            n = ids.shape[1]
+            if n > 1 and ids.stride(1) != 1:
+                raise VsmpError("ids must have contiguous rows")
+            ldj = ids.stride(0) if B > 1 else n
+            lp = torch.empty(B, n, dtype=torch.float32, device=dev)
+            rk = torch.empty(B, n, dtype=torch.int32, device=dev) if rank else None
+        st = stream if stream is not None else torch.cuda.current_stream(dev)
+        if _lib.vsmp_logprobs(self._h, logits.data_ptr(), code, ld, B, V, ids.data_ptr() if n else None, ldj, n,
+                              lp.data_ptr() if n else None, rk.data_ptr() if n and rk is not None else None,
+                              lse.data_ptr(), st.cuda_stream) != 0:
+            raise _err()
+        return lp, rk, lse
+
+    def head_logits_q4(self, hidden, q, scales, group, zeros=None, logits=None, stream=None):
+        """vsmp_head_logits_q4: the head's product with 4-bit weights, logits = hidden @ W.T with W[c, d] =
+        scales[c, d / group] * (q[c, d] - zeros[c, d / group]). hidden: bfloat16 or float16 [B, D]; q: uint8
+        [V, D / 2], two weights a byte, the even d in the low half; scales: float32, bfloat16 or float16 [V, D /
+        group]; zeros: uint8 [V, D / group], or None for 8. Returns logits (float32 [B, V] unless given)."""
+        import torch
+
+        self._check_device(hidden)
+        dev = hidden.device
+        code, ldh = _rows_of(hidden, "hidden", dev)
+        if code == 0:
+            raise VsmpError("hidden must be bfloat16 or float16")
+        B, D = hidden.shape
+        if q.dtype != torch.uint8 or q.dim() != 2 or q.device != dev or (q.shape[1] > 1 and q.stride(1) != 1):
+            raise VsmpError("q must be a 2-D uint8 tensor with contiguous rows on the hidden states' device")
+        V = q.shape[0]
+        if 2 * q.shape[1] != D:
+            raise VsmpError("q must hold D / 2 bytes per row")
+        scode, lds = _rows_of(scales, "scales", dev)
+        group = int(group)
+        if group < 1 or scales.shape != (V, D // group):
+            raise VsmpError("scales must be [V, D / group]")
+        ldz = 0
+        if zeros is not None:
+            if zeros.dtype != torch.uint8 or zeros.shape != scales.shape or zeros.device != dev or \
+                    (zeros.shape[1] > 1 and zeros.stride(1) != 1):
+                raise VsmpError("zeros must be uint8 of the scales' shape with contiguous rows")
+            ldz = zeros.stride(0) if V > 1 else zeros.shape[1]
+        if logits is None:  # rows padded to 16 bytes, so that pick_batch can take them
+            ldl = (V + 3) // 4 * 4
+            logits = torch.empty(B, ldl, dtype=torch.float32, device=dev)[:, :V]
+        else:
+            lcode, ldl = _rows_of(logits, "logits", dev)
+            if lcode != 0 or logits.shape != (B, V):
+                raise VsmpError("logits must be float32 [B, V]")
+        st = stream if stream is not None else torch.cuda.current_stream(dev)
+        if _lib.vsmp_head_logits_q4(self._h, hidden.data_ptr(), code, ldh, q.data_ptr(),
+                                    q.stride(0) if V > 1 else D // 2,
+                                    scales.data_ptr(), scode, lds, zeros.data_ptr() if zeros is not None else None, ldz,
+                                    group, B, V, D, logits.data_ptr(), ldl, st.cuda_stream) != 0:
+            raise _err()
+        return logits
 
     def read_probe(self, t, stream=None):
         """vsmp_read_probe: stream the bytes of device tensor `t` through a plain read kernel on

@@ -18,6 +18,7 @@
 #include "vsmp_common.hpp"
 #include "vsmp_error.hpp"
 #include "vsmp_internal.hpp"
+#include "vsmp_logits.hpp"
 
 using vsmp::hip_ok;
 
@@ -392,6 +393,43 @@ int vsmp_bsampler_accept_rows(vsmp_bsampler* s, const int* ids, const int* rows,
   vsmp::launch_hist_accept(s->hist, s->off, s->len, s->cap, s->params, vsmp_params{}, ids, 0, active, rows, n_rows,
                            s->full, static_cast<hipStream_t>(stream));
   return hip_ok(hipGetLastError(), "accept launch") ? 0 : -1;
+}
+
+int vsmp_bsampler_adjust_rows(vsmp_bsampler* s, const void* in, int dtype, long long ldi, int V, const int* rows,
+                              int n_rows, const vsmp_penalty* pen, int pen_per_row, const int* prompt_len,
+                              const int* bias_ids, const float* bias, const int* bias_off, const unsigned int* mask,
+                              long long ldm, int n_masks, const int* mask_row, float* out, long long ldo, int* left,
+                              void* stream) {
+  vsmp::clear_error();
+  if (!s) return vsmp::set_error("vsmp: null sampler");
+  if (n_rows < 0 || n_rows > s->n || (!rows && n_rows != s->n))
+    return vsmp::set_error("vsmp: need 0 <= n_rows <= the sampler's slots, and the slot list (or every slot)");
+  if (n_rows == 0) return 0;
+  vsmp::AdjustArgs a{};
+  a.in = in;
+  a.ldi = ldi;
+  a.B = n_rows;
+  a.V = V;
+  a.hist = s->hist;
+  a.hist_off = s->off;
+  a.hist_len = s->len;
+  a.slot = rows;
+  a.prompt_len = prompt_len;
+  a.bias_ids = bias_ids;
+  a.bias = bias;
+  a.bias_off = bias_off;
+  a.mask = mask;
+  a.ldm = ldm;
+  a.n_masks = n_masks;
+  a.mask_row = mask_row;
+  a.out = out;
+  a.ldo = ldo;
+  a.left = left;
+  const bool per_row = pen && pen_per_row != 0;
+  if (vsmp::check_adjust(a, dtype, per_row, pen) != 0) return -1;
+  vsmp::DeviceScope scope(s->device);
+  if (!scope.ok() || !vsmp::stream_on_device(s->ctx, static_cast<hipStream_t>(stream))) return -1;
+  return vsmp::adjust_logits(s->ctx, a, dtype, per_row, pen, static_cast<hipStream_t>(stream));
 }
 
 int vsmp_bsampler_full(vsmp_bsampler* s, void* stream) {

@@ -17,6 +17,7 @@
 #include "vsmp_common.hpp"
 #include "vsmp_error.hpp"
 #include "vsmp_internal.hpp"
+#include "vsmp_logits.hpp"
 
 namespace vsmp {
 
@@ -139,6 +140,9 @@ struct vsmp_ctx {
   size_t n_rcand = 0;
   int* h_rcnt = nullptr;
   size_t n_rcnt = 0;
+  // the operators around the pick (ops_scratch): one allocation of a fixed size, zero between calls
+  unsigned char* o_scr = nullptr;
+  size_t n_oscr = 0;
   // host-pointer path (vsmp_pick_host): one pinned host area, mapped into the device's address
   // space (hs_dev), holding the row, the history, its offsets and the draw, then the id and the row
   // diagnostics: the kernels read their inputs from it and write their results into it, with no
@@ -879,6 +883,22 @@ int pick_batch_noalloc(const float* logits, int B, int V, long long ld, const vs
 
 namespace vsmp {
 int ctx_device(const vsmp_ctx* c) { return c->device; }
+int ctx_cus(const vsmp_ctx* c) { return c->cus; }
+
+bool ops_scratch(vsmp_ctx* c, hipStream_t st, OpScratch* out) {
+  constexpr size_t kLeft = sizeof(unsigned long long) * kOpRows, kTick = sizeof(unsigned) * kOpSlots,
+                   kPart = 2 * sizeof(float) * kOpSlots, kCount = sizeof(int) * kOpSlots * kOpIds;
+  if (!c->o_scr && capturing(st)) {
+    set_error("vsmp: the context has no scratch for this operator yet: issue the call once before capturing it");
+    return false;
+  }
+  if (!grow(c->o_scr, c->n_oscr, kLeft + kTick + kPart + kCount, true, "scratch", st)) return false;
+  out->left = reinterpret_cast<unsigned long long*>(c->o_scr);
+  out->tick = reinterpret_cast<unsigned*>(c->o_scr + kLeft);
+  out->part = reinterpret_cast<float*>(c->o_scr + kLeft + kTick);
+  out->count = reinterpret_cast<int*>(c->o_scr + kLeft + kTick + kPart);
+  return true;
+}
 
 // A stream passed with a context must belong to the context's device (its scratch lives there).
 bool stream_on_device(const vsmp_ctx* c, hipStream_t st) {
@@ -937,7 +957,7 @@ void vsmp_ctx_free(vsmp_ctx* c) {
   (void)hipDeviceSynchronize();
   void* bufs[] = {c->x_flag, c->x_u,    c->x_buf,    c->s_cand, c->s_cnt,   c->s_npen,   c->s_max,
                   c->s_min,  c->s_bits, c->g_rows,   c->t_scr,  c->h_probe,  c->h_full,
-                  c->h_tk,   c->h_rmode, c->h_rcand, c->h_rcnt, c->p_scr};
+                  c->h_tk,   c->h_rmode, c->h_rcand, c->h_rcnt, c->p_scr, c->o_scr};
   for (void* p : bufs)
     if (p) (void)hipFree(p);
   for (unsigned char* h : c->hs_host)

@@ -5,15 +5,16 @@
 
 #include <cstdint>
 
-#include "vsmp.h"
+#include "vsmp_logits.h"
 
 namespace vsmp {
 
 // false, with the calling thread's error set to "vsmp: <what>: <HIP message>", unless e is success.
 bool hip_ok(hipError_t e, const char* what);
 
-// The device a context was created on.
+// The device a context was created on, and its compute units.
 int ctx_device(const vsmp_ctx* c);
+int ctx_cus(const vsmp_ctx* c);
 // true when `st` (null: the device's null stream) belongs to the context's device; else false, with
 // the error set.
 bool stream_on_device(const vsmp_ctx* c, hipStream_t st);
@@ -53,6 +54,19 @@ int pick_batch(vsmp_ctx* ctx, const float* logits, int B, int V, long long ld, c
                int params_per_row, const int* hist, const int* hist_off, int u_mode, const double* u,
                unsigned long long* rng_state, unsigned long long counter, int* out, const vsmp_debug* dbg,
                hipStream_t st, const int* hist_len = nullptr, const int* slot = nullptr);
+
+// The scratch of the operators around the pick (vsmp_logits.hpp): allocated and zeroed on `st` by the
+// context's first call that needs it, the same memory from then on. false (error set) when it could not
+// be, or when `st` is capturing and it is not there yet.
+struct OpScratch;
+bool ops_scratch(vsmp_ctx* c, hipStream_t st, OpScratch* out);
+
+// vsmp_adjust_logits's argument checks, and its work for arguments that pass them: rows with histories of
+// their own (hist_off with B + 1 entries) or, with hist_len, with sequences' regions (see pick_batch).
+// pen_per_row: pen is a device array of B. Both return 0 or -1 (error set).
+struct AdjustArgs;
+int check_adjust(const AdjustArgs& a, int dtype, bool pen_per_row, const vsmp_penalty* pen);
+int adjust_logits(vsmp_ctx* ctx, AdjustArgs a, int dtype, bool pen_per_row, const vsmp_penalty* pen, hipStream_t st);
 
 // verbo::Sampler's seeding (reference src/sampler.cpp:11-16,26-31): two successive SplitMix64
 // outputs of the seed; seed 0 stands for the steady clock in microseconds.

@@ -27,7 +27,7 @@ import ctypes
 
 import numpy as np
 
-from . import Params, VsmpError, _err, load_library
+from . import Params, Penalty, VsmpError, _adjust_args, _err, load_library, to_device_penalties
 
 __all__ = ["Opts", "Request", "BatchDecoder", "params_of"]
 
@@ -51,13 +51,16 @@ class Opts(ctypes.Structure):
 
 class Request:
     """One generation request of a serving loop: the prompt's ids, its options (Opts), the window
-    of its repetition penalty and the step at which it arrives."""
+    of its repetition penalty and the step at which it arrives. penalty: None, or a Penalty taken from its
+    logits before each pick, over the ids its slot keeps (the last repeat_last ones at least, the prompt's among
+    them)."""
 
-    def __init__(self, prompt, opts, repeat_last=64, arrival=0):
+    def __init__(self, prompt, opts, repeat_last=64, arrival=0, penalty=None):
         self.prompt = np.ascontiguousarray(prompt, dtype=np.int32)
         self.opts = opts
         self.repeat_last = int(repeat_last)
         self.arrival = int(arrival)
+        self.penalty = penalty
 
 
 def params_of(o, repeat_last=64):
@@ -83,6 +86,9 @@ def _lib():
             "vsmp_bsampler_admit": (ctypes.c_int, [P, ctypes.c_int, P, P, ctypes.c_int, P]),
             "vsmp_bsampler_pick_rows": (ctypes.c_int, [P, P, ctypes.c_int, ctypes.c_longlong, P, ctypes.c_int, P, P]),
             "vsmp_bsampler_accept_rows": (ctypes.c_int, [P, P, P, P, ctypes.c_int, P]),
+            "vsmp_bsampler_adjust_rows": (ctypes.c_int, [P, P, ctypes.c_int, ctypes.c_longlong, ctypes.c_int, P, ctypes.c_int,
+                                                         P, ctypes.c_int, P, P, P, P, P, ctypes.c_longlong, ctypes.c_int, P, P,
+                                                         ctypes.c_longlong, P, P]),
         }.items():
             fn = getattr(lib, name)
             fn.restype = res
@@ -186,6 +192,22 @@ class BatchDecoder:
                                             out.data_ptr(), ctypes.c_void_p(stream.cuda_stream)) != 0:
             raise _err()
 
+    def adjust_rows(self, logits, rows, penalty=None, prompt_len=None, bias_ids=None, bias=None, bias_off=None, mask=None,
+                    mask_row=None, out=None, left=None, stream=None):
+        """Context.adjust_logits for the live slots rows[i] (device int32, distinct), before pick_rows: row i is
+        penalised by slot rows[i]'s history. Per-row arrays go by row of the call; prompt_len counts from the first
+        id that the slot still keeps. Returns the adjusted logits (`out`)."""
+        dev = logits.device
+        if dev.type != "cuda" or dev.index != self.device or tuple(logits.shape) != (rows.numel(), self.vocab):
+            raise VsmpError("logits must be a [len(rows), V] tensor on the decoder's device")
+        if rows.dtype.itemsize != 4 or rows.is_floating_point() or rows.device != dev or not rows.is_contiguous():
+            raise VsmpError("rows must be a contiguous int32 tensor on the decoder's device")
+        x, (n, vocab), pen, _, rest, out = _adjust_args(logits, penalty, None, None, prompt_len, bias_ids, bias, bias_off,
+                                                        mask, mask_row, out, left, stream, csr=False)
+        if self.lib.vsmp_bsampler_adjust_rows(self._h, *x, vocab, rows.data_ptr(), n, *pen, *rest) != 0:
+            raise _err()
+        return out
+
     def accept_rows(self, ids, rows, active, stream):
         """Sampler::accept of ids[i] into slot rows[i] where active[i] != 0 (device int32 tensors)."""
         if self.lib.vsmp_bsampler_accept_rows(self._h, ids.data_ptr(), rows.data_ptr(), active.data_ptr(),
@@ -234,8 +256,11 @@ class BatchDecoder:
             slots = sorted(live)
             reqs = [live[s] for s in slots]
             rows = torch.tensor(slots, dtype=torch.int32, device=dev)
-            self.pick_rows(logits_fn(reqs, [steps[j] for j in reqs], [last[j] for j in reqs]), rows,
-                           out[:len(slots)], stream)
+            lg = logits_fn(reqs, [steps[j] for j in reqs], [last[j] for j in reqs])
+            pens = [requests[j].penalty for j in reqs]
+            if any(p is not None for p in pens):
+                lg = self.adjust_rows(lg, rows, to_device_penalties([p or Penalty() for p in pens], dev), stream=stream)
+            self.pick_rows(lg, rows, out[:len(slots)], stream)
             self.schedule.append(list(zip(reqs, slots)))
             ids = out[:len(slots)].cpu().numpy()  # the only per-step copy to the host: one id per live slot
             take = np.zeros(len(slots), np.int32)
