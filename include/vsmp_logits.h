@@ -58,7 +58,7 @@ typedef struct {
  *       is 16-byte aligned with ldo a multiple of 4.)
  *   left: NULL, or device int[B]: how many of the row's ids have y > -inf. A row with 0 has nothing to
  *       pick from (vsmp_pick_batch is not defined on it).
- * V <= 1048576 (2^20). With `left`, the context holds about 1 MB of scratch from the first such call on;
+ * V <= 1048576 (2^20). With `left`, the context holds about 2 MB of scratch from the first such call on;
  * a call that is captured into a graph needs one before it. Returns 0 or -1. */
 VSMP_API int vsmp_adjust_logits(vsmp_ctx* ctx, const void* in, int dtype, long long ldi, int B, int V,
                                 const vsmp_penalty* pen, int pen_per_row, const int* hist, const int* hist_off,
@@ -75,7 +75,7 @@ VSMP_API int vsmp_adjust_logits(vsmp_ctx* ctx, const void* in, int dtype, long l
  *   logits, dtype, ld: device logits, row r at element r * ld (ld >= V). V <= 1048576 (2^20).
  *   ids, ldj, n: device int ids, 0 <= n <= 64 (0: lse alone; ids, logprob and rank unused), ldj >= n.
  *   logprob, rank: device [B][n]; rank may be NULL. lse: device float[B], may be NULL (n > 0).
- * The context holds about 1 MB of scratch from the first call on; a call that is captured into a
+ * The context holds about 2 MB of scratch from the first call on; a call that is captured into a
  * graph needs one before it. Returns 0 or -1. */
 VSMP_API int vsmp_logprobs(vsmp_ctx* ctx, const void* logits, int dtype, long long ld, int B, int V, const int* ids,
                            long long ldj, int n, float* logprob, int* rank, float* lse, void* stream);

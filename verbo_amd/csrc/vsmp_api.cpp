@@ -886,8 +886,8 @@ int ctx_device(const vsmp_ctx* c) { return c->device; }
 int ctx_cus(const vsmp_ctx* c) { return c->cus; }
 
 bool ops_scratch(vsmp_ctx* c, hipStream_t st, OpScratch* out) {
-  constexpr size_t kLeft = sizeof(unsigned long long) * kOpRows, kTick = sizeof(unsigned) * kOpSlots,
-                   kPart = 2 * sizeof(float) * kOpSlots, kCount = sizeof(int) * kOpSlots * kOpIds;
+  constexpr size_t kLeft = sizeof(unsigned) * kOpPad * kOpRows, kTick = sizeof(unsigned) * kOpPad * (kOpSlots / 2),
+                   kPart = sizeof(unsigned long long) * kOpSlots, kCount = sizeof(int) * kOpIds * kOpSlots;
   if (!c->o_scr && capturing(st)) {
     set_error("vsmp: the context has no scratch for this operator yet: issue the call once before capturing it");
     return false;
@@ -895,7 +895,7 @@ bool ops_scratch(vsmp_ctx* c, hipStream_t st, OpScratch* out) {
   if (!grow(c->o_scr, c->n_oscr, kLeft + kTick + kPart + kCount, true, "scratch", st)) return false;
   out->left = reinterpret_cast<unsigned long long*>(c->o_scr);
   out->tick = reinterpret_cast<unsigned*>(c->o_scr + kLeft);
-  out->part = reinterpret_cast<float*>(c->o_scr + kLeft + kTick);
+  out->part = reinterpret_cast<unsigned long long*>(c->o_scr + kLeft + kTick);
   out->count = reinterpret_cast<int*>(c->o_scr + kLeft + kTick + kPart);
   return true;
 }

@@ -10,14 +10,8 @@ constexpr int kNt = 256;  // threads per workgroup
 // ---- loads -------------------------------------------------------------------------------------------
 
 // Rows start where their element type allows, so that a row of a bf16 matrix with an odd number of
-// columns may start at any even address: gfx950 takes global loads and stores of any size there.
-template <class T>
-__device__ __forceinline__ T load_any(const void* p) {
-  T v;
-  __builtin_memcpy(&v, p, sizeof v);
-  return v;
-}
-
+// columns may start at any even address: gfx950 takes global loads and stores of any size there. What is
+// read once is read with the non-temporal hint.
 struct F32 {
   static constexpr int kSize = 4;
   __device__ static float get(const void* p, long long i) { return static_cast<const float*>(p)[i]; }
@@ -25,24 +19,35 @@ struct F32 {
 struct Bf16 {
   static constexpr int kSize = 2;
   __device__ static float from(uint32_t h) { return __uint_as_float(h << 16); }
+  __device__ static uint32_t bits(float v) { return __float_as_uint(v) >> 16; }
   __device__ static float get(const void* p, long long i) { return from(static_cast<const uint16_t*>(p)[i]); }
 };
 struct F16 {
   static constexpr int kSize = 2;
   __device__ static float from(uint32_t h) { return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(h))); }
+  __device__ static uint32_t bits(float v) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(v)); }
   __device__ static float get(const void* p, long long i) { return from(static_cast<const uint16_t*>(p)[i]); }
 };
 
 // N consecutive logits from element i on, N * size = 8 or 16 bytes.
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 template <class E, int N>
 struct Raw {
   static constexpr int kWords = N * E::kSize / 4;
   uint32_t w[kWords];
+  typedef uint32_t vec __attribute__((ext_vector_type(kWords), aligned(E::kSize)));
   __device__ void load(const void* p, long long i) {
-    __builtin_memcpy(w, static_cast<const char*>(p) + i * E::kSize, sizeof w);
+    const vec v = __builtin_nontemporal_load(reinterpret_cast<const vec*>(static_cast<const char*>(p) + i * E::kSize));
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) w[k] = v[k];
+  }
+  __device__ void set(const float (&v)[N]) {  // of values that get() gave, or infinities
+    if constexpr (E::kSize == 4) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) w[k] = __float_as_uint(v[k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; k += 2) w[k / 2] = E::bits(v[k]) | E::bits(v[k + 1]) << 16;
+    }
   }
   __device__ float get(int k) const {
     if constexpr (E::kSize == 4)
@@ -187,11 +192,11 @@ __global__ __launch_bounds__(kNt) void k_adjust(AdjustArgs a) {
   __syncthreads();
   if (tid == 0) {
     // the ticket and the count in one word: the part that takes the last ticket has every part's count
-    const unsigned long long old = __hip_atomic_fetch_add(&a.acc[row], (1ull << 32) | static_cast<unsigned>(s_left),
+    const unsigned long long old = __hip_atomic_fetch_add(&a.acc[row * (kOpPad / 2)], (1ull << 32) | static_cast<unsigned>(s_left),
                                                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (static_cast<int>(old >> 32) == a.P - 1) {
       a.left[row] = static_cast<int>(old & 0xFFFFFFFFu) + s_left;
-      __hip_atomic_store(&a.acc[row], 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(&a.acc[row * (kOpPad / 2)], 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
   }
 }
@@ -203,66 +208,141 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // exp(x - m) for x <= m: 1 at x = m, 0 at x = -inf. m finite.
 __device__ __forceinline__ float exp_rel(float x, float m) { return __builtin_amdgcn_exp2f((x - m) * kLog2e); }
 
-// A running maximum and the sum of exp(x - maximum): log of the sum of exponentials in one pass. The
-// maximum of nothing is -inf, with a sum of 0.
+// A maximum and the sum of exp(x - maximum): the log of the sum of exponentials in one pass. The maximum of
+// nothing is -inf, with a sum of 0.
 struct Lse {
   float m, s;
-  __device__ void join(float om, float os) {
-    const float t = fmaxf(m, om);
-    if (t == -INFINITY) return;
-    s = s * exp_rel(m, t) + os * exp_rel(om, t);
-    m = t;
-  }
+  // The sum relative to a maximum t >= m.
+  __device__ float at(float t) const { return m == -INFINITY ? 0.0f : s * exp_rel(m, t); }
 };
+__device__ __forceinline__ unsigned long long pack_lse(const Lse& z) {
+  return static_cast<unsigned long long>(__float_as_uint(z.m)) << 32 | __float_as_uint(z.s);
+}
+__device__ __forceinline__ Lse unpack_lse(unsigned long long w) {
+  return {__uint_as_float(static_cast<uint32_t>(w >> 32)), __uint_as_float(static_cast<uint32_t>(w))};
+}
 
-// One part of a row: NV logits a step and thread in 16-byte groups. A wave keeps the asked ids' logits
-// one in a lane, and compares a step with one of them only where the step's largest value reaches it:
-// the ids that are asked for are mostly the likeliest, which few logits come before.
+__device__ __forceinline__ float lane_f32(float v, int l) {
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), l));
+}
+// Reductions over a wave with the same result in every lane, all lanes taking part: within rows of 16 lanes by
+// rotation, then over the four rows.
+template <int N>
+__device__ __forceinline__ uint32_t ror(uint32_t v) {
+  return __builtin_amdgcn_update_dpp(0u, v, 0x120 + N, 0xF, 0xF, false);
+}
+template <int N>
+__device__ __forceinline__ float ror(float v) {
+  return __uint_as_float(ror<N>(__float_as_uint(v)));
+}
+__device__ __forceinline__ float wave_max(float v) {
+  v = fmaxf(v, ror<8>(v));
+  v = fmaxf(v, ror<4>(v));
+  v = fmaxf(v, ror<2>(v));
+  v = fmaxf(v, ror<1>(v));
+  return fmaxf(fmaxf(lane_f32(v, 0), lane_f32(v, 16)), fmaxf(lane_f32(v, 32), lane_f32(v, 48)));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  v += ror<8>(v);
+  v += ror<4>(v);
+  v += ror<2>(v);
+  v += ror<1>(v);
+  return (lane_f32(v, 0) + lane_f32(v, 16)) + (lane_f32(v, 32) + lane_f32(v, 48));
+}
+__device__ __forceinline__ int wave_sum(int i) {
+  uint32_t v = static_cast<uint32_t>(i);
+  v += ror<8>(v);
+  v += ror<4>(v);
+  v += ror<2>(v);
+  v += ror<1>(v);
+  return static_cast<int>(__builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16) + __builtin_amdgcn_readlane(v, 32) +
+                          __builtin_amdgcn_readlane(v, 48));
+}
+__device__ __forceinline__ Lse wave_lse(const Lse& z) {
+  const float m = wave_max(z.m);
+  return {m, wave_sum(z.at(m))};
+}
+
+// The least float above v (finite or -inf; zeros of either sign have the same).
+__device__ __forceinline__ float next_up(float v) {
+  const uint32_t b = __float_as_uint(v + 0.0f);
+  return __uint_as_float((b << 1) == 0u ? 1u : (b >> 31 ? b - 1u : b + 1u));
+}
+
+// One part of a row, a step of four 16-byte groups per thread at a time, the next step's in flight while one
+// is summed.
+//
+// Ranks: a wave keeps the asked ids' logits one in a lane and counts, per step, the logits before each. Only ids
+// that the step's largest logit reaches can gain, and the ids that are asked for are mostly the likeliest, so
+// that few steps do more than find that out. The step's few largest logits (those that reach the least of the
+// four rows' maxima) are listed in LDS and compared one by one with all ids above that line at once; the ids
+// below it are taken one by one, each compared with all of the step's logits. The latter takes one comparison
+// and one addition per logit: where ties do not matter, v >= t before the id and v >= the next float above t
+// after it. They matter in the id's own group, whose equal logits before the id the id's lane counts first.
 template <class E>
 __global__ __launch_bounds__(kNt) void k_logprobs(LogprobArgs a) {
   constexpr int N = 16 / E::kSize, G = 4;  // elements per group, groups per step
-  __shared__ float s_m[kNt / 64], s_s[kNt / 64];
-  __shared__ int s_cnt[kOpIds];
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  constexpr int kStep = kNt * N * G, kW = kNt / 64;
+  constexpr int kList = 128, kLanes = 16;  // listed logits of a step and wave, and lanes they may come from
+  __shared__ float s_m[kW], s_s[kW];
+  __shared__ int s_cnt[kW][kOpIds];
+  __shared__ uint2 s_list[kW][kList];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row = static_cast<int>(blockIdx.x / static_cast<unsigned>(a.P));
   const int part = static_cast<int>(blockIdx.x % static_cast<unsigned>(a.P));
   const int lo = part * a.L, hi = min(a.V, lo + a.L);
   const char* x = static_cast<const char*>(a.x) + row * a.ld * E::kSize;
 
   int id = -1;
-  float t = INFINITY;
-  if (lane < a.n) {
-    id = a.ids[row * a.ldj + lane];
-    if (id < 0 || id >= a.V) id = -1;
-    if (id >= 0) t = E::get(x, id);
-  }
-  if (tid < kOpIds) s_cnt[tid] = 0;
-  __syncthreads();
+  if (lane < a.n) id = a.ids[row * a.ldj + lane];
+  Raw<E, N> r[G];
+  auto load_group = [&](Raw<E, N>& d, int e, int end) {
+    if (e + N <= end) {
+      d.load(x, e);
+    } else {  // the row's end: its last elements one by one, then -inf
+      float v[N];
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[k] = e + k < end ? E::get(x, e + k) : -INFINITY;
+      d.set(v);
+    }
+  };
+  auto load = [&](int e0) {
+#pragma unroll
+    for (int g = 0; g < G; ++g) load_group(r[g], e0 + N * (tid + g * kNt), hi);
+  };
+  load(lo);
+  if (id < 0 || id >= a.V) id = -1;
+  Raw<E, N> d;  // the id's own group
+  if (id >= 0) load_group(d, id & ~(N - 1), a.V);
+  float t = INFINITY, tup = INFINITY;
+  int cnt = 0;  // logits before the lane's id, as far as this wave has counted them
+  int own = 0;  // equal ones before it in its own group
+  auto take_ids = [&]() {
+    if (id < 0) return;
+    t = d.get(0);
+#pragma unroll
+    for (int k = 1; k < N; ++k) t = k == (id & (N - 1)) ? d.get(k) : t;
+#pragma unroll
+    for (int k = 0; k < N - 1; ++k) own += k < (id & (N - 1)) && d.get(k) == t ? 1 : 0;
+    tup = next_up(t);
+  };
 
   Lse z{-INFINITY, 0.0f};
-  int cnt = 0;  // of the lane's id
-  for (int e0 = lo; e0 < hi; e0 += kNt * N * G) {
-    Raw<E, N> r[G];
+  int low = 0, acc = 0;  // the id that was last taken by itself, and the lane's count of logits before it
+  for (int e0 = lo; e0 < hi; e0 += kStep) {
+    float v[G][N], gm[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[g][k] = r[g].get(k);
+    if (e0 + kStep < hi) load(e0 + kStep);
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      const int e = e0 + N * (tid + g * kNt);
-      if (e + N <= hi) r[g].load(x, e);
+      gm[g] = v[g][0];
+#pragma unroll
+      for (int k = 1; k < N; ++k) gm[g] = fmaxf(gm[g], v[g][k]);
     }
-    float v[G][N];
-    float mx = -INFINITY;
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const int e = e0 + N * (tid + g * kNt);
-      if (e + N <= hi) {
-#pragma unroll
-        for (int k = 0; k < N; ++k) v[g][k] = r[g].get(k);
-      } else {
-#pragma unroll
-        for (int k = 0; k < N; ++k) v[g][k] = e + k < hi ? E::get(x, e + k) : -INFINITY;
-      }
-#pragma unroll
-      for (int k = 0; k < N; ++k) mx = fmaxf(mx, v[g][k]);
-    }
+    const float mx = fmaxf(fmaxf(gm[0], gm[1]), fmaxf(gm[2], gm[3]));
     const float m = fmaxf(z.m, mx);
     if (m != -INFINITY) {
       float s = z.s * exp_rel(z.m, m);
@@ -272,79 +352,131 @@ __global__ __launch_bounds__(kNt) void k_logprobs(LogprobArgs a) {
         for (int k = 0; k < N; ++k) s += exp_rel(v[g][k], m);
       z = {m, s};
     }
-    if (a.rank) {
-      float wm = mx;
+    if (e0 == lo) take_ids();  // after the first step's sums: the ids' logits were loaded behind it
+    if (!a.rank) continue;
+    float rm = mx;  // the largest of each row of 16 lanes
+    rm = fmaxf(rm, ror<8>(rm));
+    rm = fmaxf(rm, ror<4>(rm));
+    rm = fmaxf(rm, ror<2>(rm));
+    rm = fmaxf(rm, ror<1>(rm));
+    const float r0 = lane_f32(rm, 0), r1 = lane_f32(rm, 16), r2 = lane_f32(rm, 32), r3 = lane_f32(rm, 48);
+    unsigned long long todo = __ballot(t <= fmaxf(fmaxf(r0, r1), fmaxf(r2, r3)));
+    if (!todo) continue;
+    const float few = fminf(fminf(r0, r1), fminf(r2, r3));
+    const unsigned long long high = __ballot(t >= few) & todo;
+    if (high && __popcll(__ballot(mx >= few)) <= kLanes) {
+      int n = 0;
 #pragma unroll
-      for (int d = 32; d; d >>= 1) wm = fmaxf(wm, __shfl_xor(wm, d));
-      for (unsigned long long todo = __ballot(id >= 0 && wm >= t); todo; todo &= todo - 1ull) {
-        const int j = __ffsll(static_cast<long long>(todo)) - 1;
-        const float tj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(t), j));
-        const int ij = __builtin_amdgcn_readlane(id, j);
-        int c = 0;
+      for (int g = 0; g < G; ++g) {
+        if (!__ballot(gm[g] >= few)) continue;
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-          const int e = e0 + N * (tid + g * kNt);
-#pragma unroll
-          for (int k = 0; k < N; ++k) c += (v[g][k] > tj || (v[g][k] == tj && e + k < ij && e + k < hi)) ? 1 : 0;
+        for (int k = 0; k < N; ++k) {
+          const unsigned long long at = __ballot(v[g][k] >= few);
+          if (!at) continue;
+          const int pos = n + static_cast<int>(__builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(at >> 32),
+                                                                         __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(at), 0u)));
+          if (v[g][k] >= few && pos < kList)
+            s_list[wv][pos] = make_uint2(__float_as_uint(v[g][k]), static_cast<uint32_t>(e0 + N * (tid + g * kNt) + k));
+          n += __popcll(at);
         }
-        c = sum64(c);
-        if (lane == j) cnt += c;
+      }
+      if (n <= kList) {
+        todo &= ~high;
+        const float th = t >= few ? t : INFINITY;
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+        for (int i = 0; i < n; i += 4) {
+          uint2 c[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) c[u] = s_list[wv][min(i + u, n - 1)];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const float w = i + u < n ? __uint_as_float(c[u].x) : -INFINITY;
+            // its own group's equal logits are in `own`
+            const int e = static_cast<int>(c[u].y);
+            cnt += w > th || (w == th && e < (id & ~(N - 1)) && i + u < n) ? 1 : 0;
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
       }
     }
-  }
+    for (; todo; todo &= todo - 1ull) {
+      const int j = __ffsll(static_cast<long long>(todo)) - 1;
+      if (j != low) {  // the sum over the lanes waits until another id's turn
+        const int sum = wave_sum(acc);
+        if (lane == low) cnt += sum;
+        low = j;
+        acc = 0;
+      }
+      const float tj = lane_f32(t, j), uj = lane_f32(tup, j);
+      const int ij = __builtin_amdgcn_readlane(id, j);
+      int c[G];
 #pragma unroll
-  for (int d = 32; d; d >>= 1) z.join(__shfl_xor(z.m, d), __shfl_xor(z.s, d));
+      for (int g = 0; g < G; ++g) {
+        const float b = e0 + N * (tid + g * kNt) + N <= ij ? tj : uj;
+        c[g] = 0;
+#pragma unroll
+        for (int k = 0; k < N; ++k) c[g] += v[g][k] >= b ? 1 : 0;
+      }
+      acc += (c[0] + c[1]) + (c[2] + c[3]);
+    }
+  }
+  if (a.rank) {
+    const int sum = wave_sum(acc);
+    if (lane == low) cnt += sum;
+  }
+  z = wave_lse(z);
   if (lane == 0) {
     s_m[wv] = z.m;
     s_s[wv] = z.s;
   }
-  if (lane < a.n && cnt) atomicAdd(&s_cnt[lane], cnt);
+  s_cnt[wv][lane] = cnt;
   __syncthreads();
   if (wv != 0) return;
-  z = {s_m[0], s_s[0]};
+  z = wave_lse(lane < kW ? Lse{s_m[lane], s_s[lane]} : Lse{-INFINITY, 0.0f});
+  cnt = 0;
 #pragma unroll
-  for (int w = 1; w < kNt / 64; ++w) z.join(s_m[w], s_s[w]);
-  cnt = s_cnt[lane];
+  for (int w = 0; w < kW; ++w) cnt += s_cnt[w][lane];
 
   if (a.P > 1) {
-    // hand over through the device's memory: agent-scope stores, completed before the ticket is taken;
-    // the part with the last ticket reads them with agent-scope loads after an acquire
+    // hand over through the device's memory: agent-scope stores, completed before the ticket is taken; the
+    // part with the last ticket reads them with agent-scope loads after an acquire, and clears the ticket
     const int slot = row * a.P + part;
-    if (lane == 0) {
-      __hip_atomic_store(&a.s.part[2 * slot], z.m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      __hip_atomic_store(&a.s.part[2 * slot + 1], z.s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    if (lane < a.n) __hip_atomic_store(&a.s.count[slot * kOpIds + lane], cnt, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (lane == 0)
+      __hip_atomic_store(&a.s.part[slot], pack_lse(z), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (a.rank && lane < a.n) __hip_atomic_store(&a.s.count[slot * a.n + lane], cnt, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
     unsigned n = 0u;
-    if (lane == 0) n = __hip_atomic_fetch_add(&a.s.tick[row], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (lane == 0) n = __hip_atomic_fetch_add(&a.s.tick[row * kOpPad], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (static_cast<int>(__builtin_amdgcn_readfirstlane(n)) != a.P - 1) return;
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-    if (lane == 0) __hip_atomic_store(&a.s.tick[row], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (lane == 0) __hip_atomic_store(&a.s.tick[row * kOpPad], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     z = {-INFINITY, 0.0f};
-    cnt = 0;
-    for (int p = lane; p < a.P; p += 64) {
-      const int o = row * a.P + p;
-      z.join(__hip_atomic_load(&a.s.part[2 * o], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
-             __hip_atomic_load(&a.s.part[2 * o + 1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-    }
+    if (lane < a.P)
+      z = unpack_lse(__hip_atomic_load(&a.s.part[row * a.P + lane], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    if (a.rank) {  // the parts' counts lie one after the other: every lane adds some of them up
+      s_cnt[0][lane] = 0;
+      const int total = a.P * a.n;
+      constexpr int kAhead = 8;
+      for (int i0 = lane; i0 < total; i0 += 64 * kAhead) {
+        int c[kAhead];
 #pragma unroll
-    for (int d = 32; d; d >>= 1) z.join(__shfl_xor(z.m, d), __shfl_xor(z.s, d));
-    if (a.rank && lane < a.n)
-      for (int p = 0; p < a.P; ++p)
-        cnt += __hip_atomic_load(&a.s.count[(row * a.P + p) * kOpIds + lane], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        for (int u = 0; u < kAhead; ++u)
+          c[u] = i0 + 64 * u < total ? __hip_atomic_load(&a.s.count[row * total + i0 + 64 * u], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+          if (c[u]) atomicAdd(&s_cnt[0][(i0 + 64 * u) % a.n], c[u]);
+      }
+      cnt = s_cnt[0][lane];
+    }
+    z = wave_lse(z);
   }
-  // the lanes joined the parts in different orders: one of them for all, so that equal logits have equal
-  // log-probabilities
-  z.m = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(z.m)));
-  z.s = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(z.s)));
   const float ls = logf(z.s);  // of a sum in [1, V]
   if (lane < a.n) {
     const long long o = static_cast<long long>(row) * a.n + lane;
     a.logprob[o] = id >= 0 && t != -INFINITY ? (t - z.m) - ls : -INFINITY;
-    if (a.rank) a.rank[o] = id >= 0 ? cnt : -1;
+    if (a.rank) a.rank[o] = id >= 0 ? cnt + own : -1;
   }
   if (lane == 0 && a.lse) a.lse[row] = z.m == -INFINITY ? -INFINITY : z.m + ls;
 }
@@ -368,13 +500,17 @@ void launch_adjust(const AdjustArgs& a, int dtype, hipStream_t st) {
     go(F16{});
 }
 
-// Enough workgroups for four per CU, each of at least one step (a whole number of steps, so that every
-// part but a row's last reads whole groups).
+// Workgroups of four a CU, each of at least one step (a whole number of steps, so that every part but a row's
+// last reads whole groups), at most 64 parts a row (a lane each reads their results). Measured for one and five
+// ids against one, two and eight a CU: 32 x 151,936 fp32 8.9 / 9.6 us, against 10.0 / 11.0, 9.1 / 10.3, 8.7 / 9.1;
+// 128 x 50,257 fp32 9.7 / 10.4 against 12.2 / 13.8, 9.8 / 10.7, 12.0 / 12.8; 1,024 x 49,152 bf16 20.6 / 22.4 against
+// 20.5 / 23.0, 20.4 / 21.2, 24.7 / 27.0. Workgroups of 512 threads measured the same, of 1,024 slower from 300 rows on.
 void logprob_parts(int B, int V, int dtype, int cus, int* P, int* L) {
   const int step = kNt * 4 * (dtype == VSMP_F32 ? 4 : 8);
   const int steps = (V + step - 1) / step;
   int p = (4 * cus + B - 1) / B;
   if (p > steps) p = steps;
+  if (p > 64) p = 64;  // a lane each reads their results
   if (p > kOpSlots / B) p = kOpSlots / B;
   if (p < 1) p = 1;
   *L = (steps + p - 1) / p * step;

@@ -13,17 +13,21 @@ namespace vsmp {
 
 constexpr int kOpVocab = 1 << 20;     // logits per row
 constexpr int kOpIds = 64;            // tokens a row of vsmp_logprobs may ask for: one lane each
-constexpr int kOpRows = 1 << 16;      // rows of one launch (the words that count `left`)
-constexpr int kOpSlots = 2048;        // parts of one launch of split rows
+constexpr int kOpRows = 1 << 13;      // rows of one launch of k_adjust that counts `left`
+constexpr int kOpSlots = 4096;        // parts of one launch of split rows, two a row at least
+// 32-bit words between two rows' tickets: 128 bytes, so that rows do not share a line. Every part of every row
+// adds to its row's, and a line takes them one after the other (32 rows of 151,936 logits in 38 parts: 16.1 us
+// with the tickets side by side).
+constexpr int kOpPad = 32;
 constexpr int kAdjustParts = 4096;    // logits per 256-thread workgroup of k_adjust, 16 per thread
 
 // Device scratch of these operators: allocated at its full size by a context's first call that needs
 // it, never replaced. The words are zero between calls, which the last part of a row sees to.
 struct OpScratch {
-  unsigned long long* left;  // [kOpRows]: tickets << 32 | logits counted
-  unsigned int* tick;        // [kOpSlots]
-  float* part;               // [kOpSlots][2]: a part's maximum and its sum relative to it
-  int* count;                // [kOpSlots][kOpIds]: ids before each asked id, in a part
+  unsigned long long* left;  // [kOpRows][kOpPad / 2], the first of each: tickets << 32 | logits counted
+  unsigned int* tick;        // [kOpSlots / 2][kOpPad], the first of each
+  unsigned long long* part;  // [kOpSlots]: a part's maximum << 32 | its sum relative to it (any value between calls)
+  int* count;                // [kOpSlots][kOpIds]: per part, ids before each asked id (any value between calls)
 };
 
 struct AdjustArgs {
