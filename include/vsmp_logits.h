@@ -92,6 +92,7 @@ VSMP_API int vsmp_logprobs(vsmp_ctx* ctx, const void* logits, int dtype, long lo
  *   scales, scale_dtype, lds: device [V][lds] of fp32, bf16 or f16, lds >= D / group.
  *   zeros, ldz: device bytes [V][ldz], one zero point per group (0 .. 255), ldz >= D / group; NULL: 8
  *       everywhere.
+ *   ldq and ldz below 2^26, lds below 2^24.
  *   group: 32, 64 or 128. D: a multiple of group in [32, 16384]. V <= 1048576 (2^20).
  *   logits, ldl: device fp32 [B][ldl], ldl >= V.
  * Returns 0 or -1. */

@@ -144,6 +144,9 @@ def test_logprobs_refuses(change, words):
     (dict(lds=3), "lds"),
     (dict(scales=OTHER + 1), "scales must be aligned"),
     (dict(zeros=OTHER, ldz=3), "ldz"),
+    (dict(ldq=1 << 26), "2^26"),
+    (dict(lds=1 << 24), "2^24"),
+    (dict(zeros=OTHER, ldz=1 << 26), "2^26"),
     (dict(ldl=99), "ldl"),
     (dict(out=OUT + 2), "ldl"),
 ])

@@ -16,6 +16,8 @@
 // (64) the quarters' dwords are transposed between lanes 16 and 32 apart (32 apart) with the lane
 // swaps, until an MFMA's four quarters lie in one group. x and the scales go through LDS, staged per
 // chunk in two buffers; x in the order in which the nibbles of a dword come out: 0 4 1 5 2 6 3 7.
+#include <algorithm>
+
 #include "vsmp_lds.hpp"
 #include "vsmp_logits.hpp"
 
@@ -32,24 +34,22 @@ constexpr int kQNt = 256;  // threads per workgroup
 constexpr int kQNs = 2;    // strips of 16 columns per wave
 constexpr int kQBn = kQNt / 64 * 16 * kQNs;
 
-// Eight weights of a dword as 16 + q, in the order 0 4 1 5 2 6 3 7.
+// Eight weights of a dword as 16 + q, in the order 0 4 1 5 2 6 3 7. The constants are held in registers, one scalar
+// and one vector: an and-or takes no literal, and with literals it would be two instructions.
 template <bool H>
-__device__ __forceinline__ u32x4 widen(uint32_t w) {
-  constexpr uint32_t one = H ? 0x4C004C00u : 0x41804180u, mask = H ? 0x03C003C0u : 0x00780078u;
-  u32x4 r;
-  if constexpr (H) {
-    r.x = ((w << 6) & mask) | one;
-    r.y = ((w << 2) & mask) | one;
-    r.z = ((w >> 2) & mask) | one;
-    r.w = ((w >> 6) & mask) | one;
-  } else {
-    r.x = ((w << 3) & mask) | one;
-    r.y = ((w >> 1) & mask) | one;
-    r.z = ((w >> 5) & mask) | one;
-    r.w = ((w >> 9) & mask) | one;
+struct Widen {
+  uint32_t mask = H ? 0x03C003C0u : 0x00780078u, one = H ? 0x4C004C00u : 0x41804180u;
+  __device__ Widen() {
+    asm("" : "+s"(mask));
+    asm("" : "+v"(one));
   }
-  return r;
-}
+  __device__ u32x4 operator()(uint32_t w) const {
+    if constexpr (H)
+      return u32x4{((w << 6) & mask) | one, ((w << 2) & mask) | one, ((w >> 2) & mask) | one, ((w >> 6) & mask) | one};
+    else
+      return u32x4{((w << 3) & mask) | one, ((w >> 1) & mask) | one, ((w >> 5) & mask) | one, ((w >> 9) & mask) | one};
+  }
+};
 
 template <bool H>
 __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
@@ -171,6 +171,7 @@ __global__ __launch_bounds__(kQNt) void k_head_q4(HeadQ4Args a, int rows_ld) {
     }
   };
 
+  const Widen<H> widen;
   f32x4 acc[kQNs][MB];
 #pragma unroll
   for (int s = 0; s < kQNs; ++s)
@@ -220,7 +221,7 @@ __global__ __launch_bounds__(kQNt) void k_head_q4(HeadQ4Args a, int rows_ld) {
         for (int i = 0; i < MB; ++i) A[i] = *reinterpret_cast<const u32x4*>(&sx(buf)[xa[i] + k]);
 #pragma unroll
         for (int s = 0; s < kQNs; ++s) {
-          const u32x4 wb = widen<H>(t[s][step]);
+          const u32x4 wb = widen(t[s][step]);
 #pragma unroll
           for (int i = 0; i < MB; ++i) {
             f32x4 c = u ? P[s][i] : X[i];
@@ -271,6 +272,272 @@ __global__ __launch_bounds__(kQNt) void k_head_q4(HeadQ4Args a, int rows_ld) {
   }
 }
 
+// ---- few rows: x stays in LDS ----------------------------------------------------------------------------
+
+constexpr int kQAhead = 2;  // pairs of blocks of 128 in flight per wave and strip
+// The most waves of a workgroup whose registers then suffice.
+constexpr int few_waves(int rt, int st) { return rt <= 16 ? (st == VSMP_F32 ? 12 : 16) : 8; }
+
+// One workgroup per CU, RT rows (4, 16, 32 or 64). x (rows_ld rows) and its group sums are staged once; each
+// wave then takes pairs of strips by itself, without a barrier, with kQAhead pairs of blocks of weights, scales
+// and zero points always in flight, across the end of a pair of strips too (the last blocks are loaded again
+// there and their products dropped). Two neighbouring blocks of a column are one line of 128 bytes and are
+// loaded together. The last block ends at D: it overlaps the one before where D is no multiple of 128, and x is
+// zero there. The scales and zero points of two blocks are loaded with them, a column's side by side in the lanes,
+// and reach the lanes that need them through LDS of the wave's own. (No load depends on a condition: the
+// compiler's waits then count only the loads that are behind.) With RT = 4 row r is the matrix cores' row 4 r, so that one accumulator register of four holds
+// results and the others are left alone.
+template <bool H, int G, int RT, bool ZP, int ST>
+__global__ __launch_bounds__(64 * few_waves(RT, ST)) void k_head_q4_few(HeadQ4Args a, int rows_ld, int pairs) {
+  constexpr int kGb = 128 / G, kSteps = G / 32;
+  constexpr int MB = RT <= 16 ? 1 : RT / 16, RR = RT == 4 ? 1 : 4;
+  constexpr int kSize = ST == VSMP_F32 ? 4 : 2, kSg = 2 * kGb;  // groups of two blocks
+  extern __shared__ __align__(16) unsigned char lds[];
+  const int D = a.D, nblk = (D + 127) / 128, str = nblk * 128 + 8;
+  uint16_t* sx = reinterpret_cast<uint16_t*>(lds);
+  float* sX = reinterpret_cast<float*>(lds + ((rows_ld * str * 2 + 15) & ~15));  // [nblk * kGb][RT]
+  const int tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, h = lane >> 4;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), nw = blockDim.x >> 6;
+  const int m0 = blockIdx.y * RT, rows = min(rows_ld, a.B - m0);
+
+  float* sS = sX + nblk * kGb * RT + wv * (kQNs * 16 * kSg * (ZP ? 2 : 1));  // the wave's [kQNs * 16][kSg]
+  float* sO = sS + kQNs * 16 * kSg;
+
+  const int first = blockIdx.x * nw + wv, pstep = gridDim.x * nw;
+  u32x4 w[kQAhead][2][kQNs];
+  int lp = first, lb = 0;  // the next two blocks to load
+  uint32_t ls[kQAhead][kGb], lz[kQAhead][ZP ? kGb : 1];
+  const char *qb, *sb, *zb = nullptr;     // the pair's first column
+  uint32_t qo[kQNs], so[kGb], zo[kGb];  // the lane's column and quarter from there, and the columns of its scales
+  auto at_pair = [&]() {
+    const int col = lp * (16 * kQNs);
+    qb = reinterpret_cast<const char*>(a.q) + col * a.ldq;
+    sb = static_cast<const char*>(a.sc) + col * a.lds * kSize;
+    if (ZP) zb = reinterpret_cast<const char*>(a.z) + col * a.ldz;
+#pragma unroll
+    for (int s = 0; s < kQNs; ++s)
+      qo[s] = static_cast<uint32_t>(min(16 * s + c16, a.V - 1 - col)) * static_cast<uint32_t>(a.ldq) + 16 * h;
+#pragma unroll
+    for (int i = 0; i < kGb; ++i) {
+      const uint32_t c = min(i * (64 / kSg) + lane / kSg, a.V - 1 - col);
+      so[i] = c * static_cast<uint32_t>(a.lds) * kSize;
+      if (ZP) zo[i] = c * static_cast<uint32_t>(a.ldz);
+    }
+  };
+  auto load = [&](int u) {
+    // the lane's group of the two blocks (of the last block twice, where one is left)
+    const uint32_t g = min(min(lb + (lane % kSg) / kGb, nblk - 1) * 128, D - 128) / G + lane % kGb;
+#pragma unroll
+    for (int i = 0; i < kGb; ++i) {
+      if constexpr (ST == VSMP_F32)
+        ls[u][i] = *reinterpret_cast<const uint32_t*>(sb + (so[i] + 4u * g));
+      else
+        ls[u][i] = *reinterpret_cast<const uint16_t*>(sb + (so[i] + 2u * g));
+      if (ZP) lz[u][i] = *reinterpret_cast<const uint8_t*>(zb + (zo[i] + g));
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int k = min((lb + b) * 128, D - 128);
+#pragma unroll
+      for (int s = 0; s < kQNs; ++s)
+        w[u][b][s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(qb + k / 2 + qo[s]));
+    }
+    if ((lb += 2) >= nblk) {
+      lb = 0;
+      lp = min(lp + pstep, pairs - 1);
+      at_pair();
+    }
+  };
+  const int mine = first < pairs ? (pairs - 1 - first) / pstep + 1 : 0;
+  if (mine) {
+    at_pair();
+#pragma unroll
+    for (int u = 0; u < kQAhead; ++u) load(u);
+  }
+
+  {
+    const uint16_t* x = a.x + m0 * a.ldx;
+    const int ppr = nblk * 16;  // 16-byte pieces per row
+    for (int p = tid; p < rows * ppr; p += blockDim.x) {
+      const int r = p / ppr, k8 = p - r * ppr;
+      const int k = (k8 >> 4) == nblk - 1 ? D - 128 + 8 * (k8 & 15) : 8 * k8;  // the last block ends at D
+      u32x4 v{0u, 0u, 0u, 0u};
+      if (k >= (k8 >> 4) * 128) v = *reinterpret_cast<const u32x4*>(x + r * a.ldx + k);
+      float s = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s += half_val<H>(v[j] & 0xFFFFu) + half_val<H>(v[j] >> 16);
+#pragma unroll
+      for (int d = 1; d < G / 8; d <<= 1) s += __shfl_xor(s, d);
+      u32x4 o;
+      o.x = (v.x & 0xFFFFu) | (v.z << 16);
+      o.y = (v.x >> 16) | (v.z & 0xFFFF0000u);
+      o.z = (v.y & 0xFFFFu) | (v.w << 16);
+      o.w = (v.y >> 16) | (v.w & 0xFFFF0000u);
+      *reinterpret_cast<u32x4*>(&sx[r * str + 8 * k8]) = o;
+      if (k8 % (G / 8) == 0) sX[k8 / (G / 8) * RT + r] = ZP ? s : -24.0f * s;
+    }
+  }
+  __syncthreads();
+  if (!mine) return;
+
+  const Widen<H> widen;
+  float acc[kQNs][MB][RR];
+#pragma unroll
+  for (int s = 0; s < kQNs; ++s)
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int r = 0; r < RR; ++r) acc[s][i][r] = 0.0f;
+  int xa[MB];
+  const int kl = G == 32 ? 8 * h : (G == 64 ? 32 * (h & 1) + 16 * (h >> 1) : 32 * h);
+#pragma unroll
+  for (int i = 0; i < MB; ++i) xa[i] = min(RT == 4 ? c16 >> 2 : 16 * i + c16, rows - 1) * str + kl;
+
+  int cp = first, cb = 0;  // the blocks that are multiplied
+  const int total = mine * ((nblk + 1) / 2);
+  for (int it = 0; it < total; it += kQAhead) {
+#pragma unroll
+    for (int u = 0; u < kQAhead; ++u) {
+#pragma unroll
+      for (int i = 0; i < kGb; ++i) {
+        sS[lane + 64 * i] = ST == VSMP_F32 ? __uint_as_float(ls[u][i]) : half_val<ST == VSMP_F16>(ls[u][i]);
+        if (ZP) sO[lane + 64 * i] = -16.0f - static_cast<float>(lz[u][i]);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        if (cb + b >= nblk) continue;
+        uint32_t t[kQNs][4];
+        float sc[kQNs][kGb], of[kQNs][kGb];
+#pragma unroll
+        for (int s = 0; s < kQNs; ++s) {
+          t[s][0] = w[u][b][s].x, t[s][1] = w[u][b][s].y, t[s][2] = w[u][b][s].z, t[s][3] = w[u][b][s].w;
+          if constexpr (G <= 64) {
+            swap32(t[s][0], t[s][2]);
+            swap32(t[s][1], t[s][3]);
+          }
+          if constexpr (G == 32) {
+            swap16(t[s][0], t[s][1]);
+            swap16(t[s][2], t[s][3]);
+          }
+#pragma unroll
+          for (int g = 0; g < kGb; ++g) {
+            const int at = (16 * s + c16) * kSg + b * kGb + g;
+            sc[s][g] = sS[at];
+            of[s][g] = ZP ? sO[at] : 0.0f;
+          }
+        }
+        const uint16_t* xb = sx + (cb + b) * 128;
+        const float* Xb = sX + (cb + b) * kGb * RT;
+#pragma unroll
+        for (int g = 0; g < kGb; ++g) {
+          f32x4 X[MB], P[kQNs][MB];
+#pragma unroll
+          for (int i = 0; i < MB; ++i) {
+            if constexpr (RT == 4)
+              X[i] = f32x4{Xb[g * RT + h], 0.0f, 0.0f, 0.0f};
+            else
+              X[i] = *reinterpret_cast<const f32x4*>(&Xb[g * RT + 16 * i + 4 * h]);
+          }
+#pragma unroll
+          for (int v = 0; v < kSteps; ++v) {
+            const int step = g * kSteps + v;
+            const int k = G == 32 ? 32 * step : (G == 64 ? 64 * g + 8 * v : 8 * step);
+            u32x4 A[MB];
+#pragma unroll
+            for (int i = 0; i < MB; ++i) A[i] = *reinterpret_cast<const u32x4*>(&xb[xa[i] + k]);
+#pragma unroll
+            for (int s = 0; s < kQNs; ++s) {
+              const u32x4 wb = widen(t[s][step]);
+#pragma unroll
+              for (int i = 0; i < MB; ++i) {
+                f32x4 c = v ? P[s][i] : X[i];
+                if (ZP && v == 0) {
+#pragma unroll
+                  for (int r = 0; r < RR; ++r) c[r] *= of[s][g];
+                }
+                P[s][i] = mfma<H>(A[i], wb, c);
+              }
+            }
+          }
+#pragma unroll
+          for (int s = 0; s < kQNs; ++s)
+#pragma unroll
+            for (int i = 0; i < MB; ++i)
+#pragma unroll
+              for (int r = 0; r < RR; ++r) acc[s][i][r] = __builtin_fmaf(sc[s][g], P[s][i][r], acc[s][i][r]);
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+      __builtin_amdgcn_sched_barrier(0);
+      load(u);
+      __builtin_amdgcn_sched_barrier(0);
+      if ((cb += 2) >= nblk) {
+        if (it + u < total) {
+#pragma unroll
+          for (int s = 0; s < kQNs; ++s) {
+            const int col = (cp * kQNs + s) * 16 + c16;
+#pragma unroll
+            for (int i = 0; i < MB; ++i)
+#pragma unroll
+              for (int r = 0; r < RR; ++r) {
+                const int row = 16 * i + RR * h + r;
+                if (col < a.V && row < rows) a.out[(m0 + row) * a.ldo + col] = acc[s][i][r];
+                acc[s][i][r] = 0.0f;
+              }
+          }
+        }
+        cb = 0;
+        cp += pstep;
+      }
+    }
+  }
+}
+
+// LDS of k_head_q4_few: x and its group sums, and a wave's scales.
+size_t few_lds(int rows, int rt, int D, int group) {
+  const size_t nblk = (D + 127) / 128;
+  return ((rows * (nblk * 128 + 8) * 2 + 15) & ~size_t{15}) + nblk * (128 / group) * rt * sizeof(float);
+}
+size_t wave_lds(int group, bool zp) { return 16 * kQNs * 2 * (128 / group) * sizeof(float) * (zp ? 2 : 1); }
+constexpr size_t kFewLds = 160 * 1024;
+constexpr int kFewWaves = 4;  // the fewest that the rest of the LDS must hold
+
+template <bool H, int G, int RT, bool ZP, int ST>
+void launch_few_as(const HeadQ4Args& a, int cus, hipStream_t st) {
+  const int rows_ld = a.B < RT ? a.B : RT, groups = (a.B + RT - 1) / RT;
+  const int pairs = (a.V + 16 * kQNs - 1) / (16 * kQNs);
+  // waves per workgroup: as many rounds of pairs as the most waves would need, and no more waves than those fill
+  const size_t x_lds = few_lds(rows_ld, RT, a.D, G);
+  const int most = std::min(few_waves(RT, ST), static_cast<int>((kFewLds - x_lds) / wave_lds(G, ZP)));
+  const int wgs = cus > 0 ? cus : 256, per = (pairs + wgs - 1) / wgs, rounds = (per + most - 1) / most;
+  const int nw = (per + rounds - 1) / rounds;
+  static DynLdsOnce configured;
+  allow_dyn_lds(configured, {reinterpret_cast<const void*>(k_head_q4_few<H, G, RT, ZP, ST>)}, static_cast<int>(kFewLds));
+  const dim3 grid((pairs + nw - 1) / nw < wgs ? (pairs + nw - 1) / nw : wgs, groups);
+  hipLaunchKernelGGL((k_head_q4_few<H, G, RT, ZP, ST>), grid, dim3(64 * nw), x_lds + nw * wave_lds(G, ZP), st, a, rows_ld, pairs);
+}
+template <bool H, int G, int RT, bool ZP>
+void launch_few_zp(const HeadQ4Args& a, int cus, hipStream_t st) {
+  if (a.sc_type == VSMP_F32)
+    launch_few_as<H, G, RT, ZP, VSMP_F32>(a, cus, st);
+  else if (a.sc_type == VSMP_BF16)
+    launch_few_as<H, G, RT, ZP, VSMP_BF16>(a, cus, st);
+  else
+    launch_few_as<H, G, RT, ZP, VSMP_F16>(a, cus, st);
+}
+template <bool H, int G, int RT>
+bool launch_few(const HeadQ4Args& a, int cus, hipStream_t st) {
+  if (a.D < 128 || few_lds(a.B < RT ? a.B : RT, RT, a.D, G) + kFewWaves * wave_lds(G, a.z != nullptr) > kFewLds) return false;
+  if (a.z)
+    launch_few_zp<H, G, RT, true>(a, cus, st);
+  else
+    launch_few_zp<H, G, RT, false>(a, cus, st);
+  return true;
+}
+
+// ---- launches ----------------------------------------------------------------------------------------------
+
 template <bool H, int G, int MB, bool ZP>
 void launch_tile(const HeadQ4Args& a, hipStream_t st) {
   constexpr int KC = MB == 1 ? 512 : 256;
@@ -283,21 +550,25 @@ void launch_tile(const HeadQ4Args& a, hipStream_t st) {
   hipLaunchKernelGGL((k_head_q4<H, G, MB, ZP, KC>), grid, dim3(kQNt), 2 * stage, st, a, rows_ld);
 }
 
-template <bool H, int G>
-void launch_group(const HeadQ4Args& a, hipStream_t st) {
-  auto go = [&](auto mb) {
-    constexpr int MB = decltype(mb)::value;
-    if (a.z)
-      launch_tile<H, G, MB, true>(a, st);
-    else
-      launch_tile<H, G, MB, false>(a, st);
-  };
-  if (a.B <= 16)
-    go(std::integral_constant<int, 1>{});
-  else if (a.B <= 32)
-    go(std::integral_constant<int, 2>{});
+template <bool H, int G, int MB>
+void launch_tiles(const HeadQ4Args& a, hipStream_t st) {
+  if (a.z)
+    launch_tile<H, G, MB, true>(a, st);
   else
-    go(std::integral_constant<int, 4>{});
+    launch_tile<H, G, MB, false>(a, st);
+}
+
+template <bool H, int G>
+void launch_group(const HeadQ4Args& a, int cus, hipStream_t st) {
+  if (a.B <= 4) {
+    if (!launch_few<H, G, 4>(a, cus, st)) launch_tiles<H, G, 1>(a, st);
+  } else if (a.B <= 16) {
+    if (!launch_few<H, G, 16>(a, cus, st)) launch_tiles<H, G, 1>(a, st);
+  } else if (a.B <= 32) {
+    if (!launch_few<H, G, 32>(a, cus, st)) launch_tiles<H, G, 2>(a, st);
+  } else {
+    if (!launch_few<H, G, 64>(a, cus, st)) launch_tiles<H, G, 4>(a, st);
+  }
 }
 
 }  // namespace
@@ -306,11 +577,11 @@ void launch_head_q4(const HeadQ4Args& a, int dtype, int group, int cus, hipStrea
   auto go = [&](auto h) {
     constexpr bool H = decltype(h)::value;
     if (group == 32)
-      launch_group<H, 32>(a, st);
+      launch_group<H, 32>(a, cus, st);
     else if (group == 64)
-      launch_group<H, 64>(a, st);
+      launch_group<H, 64>(a, cus, st);
     else
-      launch_group<H, 128>(a, st);
+      launch_group<H, 128>(a, cus, st);
   };
   if (dtype == VSMP_F16)
     go(std::true_type{});

@@ -186,6 +186,8 @@ int vsmp_head_logits_q4(vsmp_ctx* ctx, const void* hidden, int dtype, long long 
     return set_error("vsmp: q must be 16-byte aligned with ldq >= D / 2 a multiple of 16");
   if (lds < D / group || lds > (LLONG_MAX >> 4) / V || !aligned(scales, vsmp::elem_size(scale_dtype)))
     return set_error("vsmp: scales must be aligned to their elements with lds >= D / group");
+  if (ldq >= 1 << 26 || lds >= 1 << 24 || (zeros && ldz >= 1 << 26))  // a tile's columns are addressed with 32 bits
+    return set_error("vsmp: ldq and ldz must be below 2^26, lds below 2^24");
   if (zeros && (ldz < D / group || ldz > (LLONG_MAX >> 4) / V)) return set_error("vsmp: ldz must be >= D / group");
   if (ldl < V || ldl > (LLONG_MAX >> 4) / B || !aligned(logits, 4)) return set_error("vsmp: ldl must be >= V, logits aligned to 4 bytes");
   vsmp::DeviceScope scope(vsmp::ctx_device(ctx));
