@@ -494,16 +494,19 @@ def test_head_q4_sizes(ctx, G, zeros, scales, dtype):
     assert np.array_equal(out._base.cpu().numpy(), around.cpu().numpy())
 
 
-@pytest.mark.parametrize("n,D,G", [(5000, 4096, 128), (2049, 16384, 32), (151936, 896, 64)])
-def test_head_q4_large(ctx, n, D, G):
-    import torch
-
+@pytest.mark.parametrize("n,D,G,B,zeros", [(5000, 4096, 128, 3, True), (2049, 16384, 32, 3, True), (151936, 896, 64, 3, True),
+                                           (333, 4096, 64, 40, False), (100, 16384, 32, 17, True), (257, 2240, 32, 64, True),
+                                           (290, 2176, 128, 70, False), (65, 16256, 128, 16, True), (70, 8192, 64, 129, False)])
+def test_head_q4_large(ctx, n, D, G, B, zeros):
+    """Large vocabularies and hidden sizes; hidden states that do not fit on chip whole, in chunks that end early."""
     rng = np.random.default_rng(1)
-    q, s, z, w = q4_weights(n, n, D, G, "bf16", True)
-    hidden = dev(rng.normal(0, 1, (3, D)).astype(np.float32), "bf16")
-    log("head q4", n, D, G)
-    check_head(ctx.head_logits_q4(hidden, q, s, G, zeros=z), hidden, s, z, w, G)
-    torch.cuda.synchronize()
+    q, s, z, w = q4_weights(n, n, D, G, "bf16", zeros)
+    hidden = dev(rng.normal(0, 1, (B, D)).astype(np.float32), "bf16")
+    log("head q4", n, D, G, B)
+    got = ctx.head_logits_q4(hidden, q, s, G, zeros=z)
+    check_head(got, hidden, s, z, w, G)
+    one = ctx.head_logits_q4(hidden[B - 1:], q, s, G, zeros=z)
+    assert np.array_equal(one.cpu().numpy(), got[B - 1:].cpu().numpy())
 
 
 @pytest.mark.parametrize("G,zeros", [(32, True), (64, False), (128, False)])

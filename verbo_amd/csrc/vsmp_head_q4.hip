@@ -89,7 +89,7 @@ __device__ __forceinline__ void swap16(uint32_t& a, uint32_t& b) {
 // H: f16 hidden states (else bf16). G: group. MB: blocks of 16 rows. ZP: zero points given. KC: hidden
 // elements per chunk.
 template <bool H, int G, int MB, bool ZP, int KC>
-__global__ __launch_bounds__(kQNt) void k_head_q4(HeadQ4Args a, int rows_ld) {
+__global__ __launch_bounds__(kQNt) void k_head_q4_tile(HeadQ4Args a, int rows_ld) {
   constexpr int kStr = KC + 8;        // halfwords per x row in LDS: 16 rows' reads fall on distinct banks
   constexpr int kBlk = KC / 128;      // blocks of 128 per chunk
   constexpr int kGc = KC / G;         // groups per chunk
@@ -274,41 +274,52 @@ __global__ __launch_bounds__(kQNt) void k_head_q4(HeadQ4Args a, int rows_ld) {
 
 // ---- few rows: x stays in LDS ----------------------------------------------------------------------------
 
-constexpr int kQAhead = 2;  // pairs of blocks of 128 in flight per wave and strip
+constexpr int kQAhead = 2;    // units of 256 in flight per wave and strip
+constexpr int kQTurn = 2048;  // bytes of LDS in which a strip's unit is turned
 // The most waves of a workgroup whose registers then suffice.
-constexpr int few_waves(int rt, int st) { return rt <= 16 ? (st == VSMP_F32 ? 12 : 16) : 8; }
+constexpr int few_waves(int rt, int group, bool zp, int st) {
+  return rt > 16 ? 8 : (st == VSMP_F32 || (zp && group < 128) ? 12 : 16);
+}
 
-// One workgroup per CU, RT rows (4, 16, 32 or 64). x (rows_ld rows) and its group sums are staged once; each
-// wave then takes pairs of strips by itself, without a barrier, with kQAhead pairs of blocks of weights, scales
-// and zero points always in flight, across the end of a pair of strips too (the last blocks are loaded again
-// there and their products dropped). Two neighbouring blocks of a column are one line of 128 bytes and are
-// loaded together. The last block ends at D: it overlaps the one before where D is no multiple of 128, and x is
-// zero there. The scales and zero points of two blocks are loaded with them, a column's side by side in the lanes,
-// and reach the lanes that need them through LDS of the wave's own. (No load depends on a condition: the
-// compiler's waits then count only the loads that are behind.) With RT = 4 row r is the matrix cores' row 4 r, so that one accumulator register of four holds
-// results and the others are left alone.
-template <bool H, int G, int RT, bool ZP, int ST>
-__global__ __launch_bounds__(64 * few_waves(RT, ST)) void k_head_q4_few(HeadQ4Args a, int rows_ld, int pairs) {
+// One workgroup per CU, RT rows (4, 16, 32 or 64). x (rows_ld rows) and its group sums are staged once; each wave
+// then takes pairs of strips by itself, without a barrier, in units of 256 weights a column, kQAhead units always in
+// flight, across the end of a pair too (the last units are loaded again there and their products dropped). The
+// last unit ends at D: it overlaps the one before where D is no multiple of 256, and x is zero there.
+//
+// A unit of a column is one line of 128 bytes, which eight neighbouring lanes load, so that a load touches 8 lines;
+// loaded as the products need them, 16 bytes of a column in lanes 16 apart, every 16 lanes touch 16 lines, and the
+// weights' stream alone was 1.2 to 1.3 times as long (1 x 128,256 x 4,096 70.6 against 56.8 us, 4 x 151,936 x 2,048
+// 42.1 / 33.0, timing only). The lanes exchange them through LDS of the wave's own; piece p of column c lies at
+// p ^ c, so that neither side meets a bank twice. Scales and zero points of a unit are loaded with it, a column's
+// side by side, and go through LDS likewise. (No load depends on a condition: the compiler's waits then count only
+// the loads that are behind.) With RT = 4 row r is the matrix cores' row 4 r, so that one accumulator register of
+// four holds results and the others are left alone.
+//
+// CH: x does not fit. It is staged chu units at a time (an even number), between two barriers, and each wave takes
+// one pair.
+template <bool H, int G, int RT, bool ZP, int ST, bool CH>
+__global__ __launch_bounds__(64 * few_waves(RT, G, ZP, ST)) void k_head_q4(HeadQ4Args a, int rows_ld, int pairs, int chu) {
   constexpr int kGb = 128 / G, kSteps = G / 32;
   constexpr int MB = RT <= 16 ? 1 : RT / 16, RR = RT == 4 ? 1 : 4;
-  constexpr int kSize = ST == VSMP_F32 ? 4 : 2, kSg = 2 * kGb;  // groups of two blocks
+  constexpr int kSize = ST == VSMP_F32 ? 4 : 2, kSg = 2 * kGb;  // groups of a unit
   extern __shared__ __align__(16) unsigned char lds[];
-  const int D = a.D, nblk = (D + 127) / 128, str = nblk * 128 + 8;
+  const int D = a.D, nun = (D + 255) / 256, held = CH ? chu : nun, str = held * 256 + 8;
   uint16_t* sx = reinterpret_cast<uint16_t*>(lds);
-  float* sX = reinterpret_cast<float*>(lds + ((rows_ld * str * 2 + 15) & ~15));  // [nblk * kGb][RT]
+  float* sX = reinterpret_cast<float*>(lds + ((rows_ld * str * 2 + 15) & ~15));  // [held * kSg][RT]
   const int tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, h = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), nw = blockDim.x >> 6;
   const int m0 = blockIdx.y * RT, rows = min(rows_ld, a.B - m0);
 
-  float* sS = sX + nblk * kGb * RT + wv * (kQNs * 16 * kSg * (ZP ? 2 : 1));  // the wave's [kQNs * 16][kSg]
+  unsigned char* sT = reinterpret_cast<unsigned char*>(sX + held * kSg * RT) + wv * (kQTurn + kQNs * 16 * kSg * 4 * (ZP ? 2 : 1));
+  float* sS = reinterpret_cast<float*>(sT + kQTurn);  // the wave's [kQNs * 16][kSg]
   float* sO = sS + kQNs * 16 * kSg;
 
   const int first = blockIdx.x * nw + wv, pstep = gridDim.x * nw;
   u32x4 w[kQAhead][2][kQNs];
-  int lp = first, lb = 0;  // the next two blocks to load
+  int lp = first, lu = 0;  // the next unit to load
   uint32_t ls[kQAhead][kGb], lz[kQAhead][ZP ? kGb : 1];
   const char *qb, *sb, *zb = nullptr;     // the pair's first column
-  uint32_t qo[kQNs], so[kGb], zo[kGb];  // the lane's column and quarter from there, and the columns of its scales
+  uint32_t qo[kQNs][2], so[kGb], zo[kGb];  // the lane's columns and piece from there, and the columns of its scales
   auto at_pair = [&]() {
     const int col = lp * (16 * kQNs);
     qb = reinterpret_cast<const char*>(a.q) + col * a.ldq;
@@ -316,7 +327,10 @@ __global__ __launch_bounds__(64 * few_waves(RT, ST)) void k_head_q4_few(HeadQ4Ar
     if (ZP) zb = reinterpret_cast<const char*>(a.z) + col * a.ldz;
 #pragma unroll
     for (int s = 0; s < kQNs; ++s)
-      qo[s] = static_cast<uint32_t>(min(16 * s + c16, a.V - 1 - col)) * static_cast<uint32_t>(a.ldq) + 16 * h;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        qo[s][b] = static_cast<uint32_t>(min(16 * s + 8 * b + (lane >> 3), a.V - 1 - col)) * static_cast<uint32_t>(a.ldq) +
+                   16 * ((lane & 7) ^ (lane >> 3));
 #pragma unroll
     for (int i = 0; i < kGb; ++i) {
       const uint32_t c = min(i * (64 / kSg) + lane / kSg, a.V - 1 - col);
@@ -325,8 +339,8 @@ __global__ __launch_bounds__(64 * few_waves(RT, ST)) void k_head_q4_few(HeadQ4Ar
     }
   };
   auto load = [&](int u) {
-    // the lane's group of the two blocks (of the last block twice, where one is left)
-    const uint32_t g = min(min(lb + (lane % kSg) / kGb, nblk - 1) * 128, D - 128) / G + lane % kGb;
+    const int k = min(lu * 256, D - 256);
+    const uint32_t g = k / G + lane % kSg;
 #pragma unroll
     for (int i = 0; i < kGb; ++i) {
       if constexpr (ST == VSMP_F32)
@@ -336,14 +350,12 @@ __global__ __launch_bounds__(64 * few_waves(RT, ST)) void k_head_q4_few(HeadQ4Ar
       if (ZP) lz[u][i] = *reinterpret_cast<const uint8_t*>(zb + (zo[i] + g));
     }
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int k = min((lb + b) * 128, D - 128);
+    for (int s = 0; s < kQNs; ++s)
 #pragma unroll
-      for (int s = 0; s < kQNs; ++s)
-        w[u][b][s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(qb + k / 2 + qo[s]));
-    }
-    if ((lb += 2) >= nblk) {
-      lb = 0;
+      for (int b = 0; b < 2; ++b)
+        w[u][b][s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(qb + k / 2 + qo[s][b]));
+    if (++lu == nun) {
+      lu = 0;
       lp = min(lp + pstep, pairs - 1);
       at_pair();
     }
@@ -355,14 +367,14 @@ __global__ __launch_bounds__(64 * few_waves(RT, ST)) void k_head_q4_few(HeadQ4Ar
     for (int u = 0; u < kQAhead; ++u) load(u);
   }
 
-  {
+  auto stage = [&](int u0, int n) {  // units [u0, u0 + n) of x
     const uint16_t* x = a.x + m0 * a.ldx;
-    const int ppr = nblk * 16;  // 16-byte pieces per row
+    const int ppr = n * 32;  // 16-byte pieces per row
     for (int p = tid; p < rows * ppr; p += blockDim.x) {
-      const int r = p / ppr, k8 = p - r * ppr;
-      const int k = (k8 >> 4) == nblk - 1 ? D - 128 + 8 * (k8 & 15) : 8 * k8;  // the last block ends at D
+      const int r = p / ppr, k8 = p - r * ppr, u = u0 + (k8 >> 5);
+      const int k = u == nun - 1 ? D - 256 + 8 * (k8 & 31) : u * 256 + 8 * (k8 & 31);  // the last unit ends at D
       u32x4 v{0u, 0u, 0u, 0u};
-      if (k >= (k8 >> 4) * 128) v = *reinterpret_cast<const u32x4*>(x + r * a.ldx + k);
+      if (k >= u * 256) v = *reinterpret_cast<const u32x4*>(x + r * a.ldx + k);
       float s = 0.0f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) s += half_val<H>(v[j] & 0xFFFFu) + half_val<H>(v[j] >> 16);
@@ -376,9 +388,12 @@ __global__ __launch_bounds__(64 * few_waves(RT, ST)) void k_head_q4_few(HeadQ4Ar
       *reinterpret_cast<u32x4*>(&sx[r * str + 8 * k8]) = o;
       if (k8 % (G / 8) == 0) sX[k8 / (G / 8) * RT + r] = ZP ? s : -24.0f * s;
     }
+  };
+  if constexpr (!CH) {
+    stage(0, nun);
+    __syncthreads();
+    if (!mine) return;
   }
-  __syncthreads();
-  if (!mine) return;
 
   const Widen<H> widen;
   float acc[kQNs][MB][RR];
@@ -393,150 +408,203 @@ __global__ __launch_bounds__(64 * few_waves(RT, ST)) void k_head_q4_few(HeadQ4Ar
 #pragma unroll
   for (int i = 0; i < MB; ++i) xa[i] = min(RT == 4 ? c16 >> 2 : 16 * i + c16, rows - 1) * str + kl;
 
-  int cp = first, cb = 0;  // the blocks that are multiplied
-  const int total = mine * ((nblk + 1) / 2);
-  for (int it = 0; it < total; it += kQAhead) {
+  int cp = first, cu = 0;  // the unit that is multiplied
+  const bool half = D - (nun - 1) * 256 <= 128;  // the first block of the last unit lies before it
+  int c0 = 0;  // the first unit of x that is staged
+  auto unit = [&](int u) {  // unit cu, which lies in slot u
 #pragma unroll
-    for (int u = 0; u < kQAhead; ++u) {
+    for (int i = 0; i < kGb; ++i) {
+      sS[lane + 64 * i] = ST == VSMP_F32 ? __uint_as_float(ls[u][i]) : half_val<ST == VSMP_F16>(ls[u][i]);
+      if (ZP) sO[lane + 64 * i] = -16.0f - static_cast<float>(lz[u][i]);
+    }
+    u32x4 turned[2][kQNs];
 #pragma unroll
-      for (int i = 0; i < kGb; ++i) {
-        sS[lane + 64 * i] = ST == VSMP_F32 ? __uint_as_float(ls[u][i]) : half_val<ST == VSMP_F16>(ls[u][i]);
-        if (ZP) sO[lane + 64 * i] = -16.0f - static_cast<float>(lz[u][i]);
-      }
+    for (int s = 0; s < kQNs; ++s) {
+      *reinterpret_cast<u32x4*>(sT + 16 * lane) = w[u][0][s];
+      *reinterpret_cast<u32x4*>(sT + 1024 + 16 * lane) = w[u][1][s];
       __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        if (cb + b >= nblk) continue;
-        uint32_t t[kQNs][4];
-        float sc[kQNs][kGb], of[kQNs][kGb];
+      for (int b = 0; b < 2; ++b)
+        turned[b][s] = *reinterpret_cast<const u32x4*>(sT + 128 * c16 + 16 * ((4 * b + h) ^ (c16 & 7)));
+      __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    load(u);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int s = 0; s < kQNs; ++s) {
-          t[s][0] = w[u][b][s].x, t[s][1] = w[u][b][s].y, t[s][2] = w[u][b][s].z, t[s][3] = w[u][b][s].w;
-          if constexpr (G <= 64) {
-            swap32(t[s][0], t[s][2]);
-            swap32(t[s][1], t[s][3]);
-          }
-          if constexpr (G == 32) {
-            swap16(t[s][0], t[s][1]);
-            swap16(t[s][2], t[s][3]);
-          }
+    for (int b = 0; b < 2; ++b) {
+      if (b == 0 && half && cu == nun - 1) continue;
+      uint32_t t[kQNs][4];
+      float sc[kQNs][kGb], of[kQNs][kGb];
 #pragma unroll
-          for (int g = 0; g < kGb; ++g) {
-            const int at = (16 * s + c16) * kSg + b * kGb + g;
-            sc[s][g] = sS[at];
-            of[s][g] = ZP ? sO[at] : 0.0f;
-          }
+      for (int s = 0; s < kQNs; ++s) {
+        t[s][0] = turned[b][s].x, t[s][1] = turned[b][s].y, t[s][2] = turned[b][s].z, t[s][3] = turned[b][s].w;
+        if constexpr (G <= 64) {
+          swap32(t[s][0], t[s][2]);
+          swap32(t[s][1], t[s][3]);
         }
-        const uint16_t* xb = sx + (cb + b) * 128;
-        const float* Xb = sX + (cb + b) * kGb * RT;
+        if constexpr (G == 32) {
+          swap16(t[s][0], t[s][1]);
+          swap16(t[s][2], t[s][3]);
+        }
 #pragma unroll
         for (int g = 0; g < kGb; ++g) {
-          f32x4 X[MB], P[kQNs][MB];
-#pragma unroll
-          for (int i = 0; i < MB; ++i) {
-            if constexpr (RT == 4)
-              X[i] = f32x4{Xb[g * RT + h], 0.0f, 0.0f, 0.0f};
-            else
-              X[i] = *reinterpret_cast<const f32x4*>(&Xb[g * RT + 16 * i + 4 * h]);
-          }
-#pragma unroll
-          for (int v = 0; v < kSteps; ++v) {
-            const int step = g * kSteps + v;
-            const int k = G == 32 ? 32 * step : (G == 64 ? 64 * g + 8 * v : 8 * step);
-            u32x4 A[MB];
-#pragma unroll
-            for (int i = 0; i < MB; ++i) A[i] = *reinterpret_cast<const u32x4*>(&xb[xa[i] + k]);
-#pragma unroll
-            for (int s = 0; s < kQNs; ++s) {
-              const u32x4 wb = widen(t[s][step]);
-#pragma unroll
-              for (int i = 0; i < MB; ++i) {
-                f32x4 c = v ? P[s][i] : X[i];
-                if (ZP && v == 0) {
-#pragma unroll
-                  for (int r = 0; r < RR; ++r) c[r] *= of[s][g];
-                }
-                P[s][i] = mfma<H>(A[i], wb, c);
-              }
-            }
-          }
-#pragma unroll
-          for (int s = 0; s < kQNs; ++s)
-#pragma unroll
-            for (int i = 0; i < MB; ++i)
-#pragma unroll
-              for (int r = 0; r < RR; ++r) acc[s][i][r] = __builtin_fmaf(sc[s][g], P[s][i][r], acc[s][i][r]);
+          const int at = (16 * s + c16) * kSg + b * kGb + g;
+          sc[s][g] = sS[at];
+          of[s][g] = ZP ? sO[at] : 0.0f;
         }
       }
-      __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-      __builtin_amdgcn_sched_barrier(0);
-      load(u);
-      __builtin_amdgcn_sched_barrier(0);
-      if ((cb += 2) >= nblk) {
-        if (it + u < total) {
+      const uint16_t* xb = sx + (2 * (cu - c0) + b) * 128;
+      const float* Xb = sX + (2 * (cu - c0) + b) * kGb * RT;
+#pragma unroll
+      for (int g = 0; g < kGb; ++g) {
+        f32x4 X[MB], P[kQNs][MB];
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+          if constexpr (RT == 4)
+            X[i] = f32x4{Xb[g * RT + h], 0.0f, 0.0f, 0.0f};
+          else
+            X[i] = *reinterpret_cast<const f32x4*>(&Xb[g * RT + 16 * i + 4 * h]);
+        }
+#pragma unroll
+        for (int v = 0; v < kSteps; ++v) {
+          const int step = g * kSteps + v;
+          const int k = G == 32 ? 32 * step : (G == 64 ? 64 * g + 8 * v : 8 * step);
+          u32x4 A[MB];
+#pragma unroll
+          for (int i = 0; i < MB; ++i) A[i] = *reinterpret_cast<const u32x4*>(&xb[xa[i] + k]);
 #pragma unroll
           for (int s = 0; s < kQNs; ++s) {
-            const int col = (cp * kQNs + s) * 16 + c16;
+            const u32x4 wb = widen(t[s][step]);
 #pragma unroll
-            for (int i = 0; i < MB; ++i)
+            for (int i = 0; i < MB; ++i) {
+              f32x4 c = v ? P[s][i] : X[i];
+              if (ZP && v == 0) {
 #pragma unroll
-              for (int r = 0; r < RR; ++r) {
-                const int row = 16 * i + RR * h + r;
-                if (col < a.V && row < rows) a.out[(m0 + row) * a.ldo + col] = acc[s][i][r];
-                acc[s][i][r] = 0.0f;
+                for (int r = 0; r < RR; ++r) c[r] *= of[s][g];
               }
+              P[s][i] = mfma<H>(A[i], wb, c);
+            }
           }
         }
-        cb = 0;
-        cp += pstep;
+#pragma unroll
+        for (int s = 0; s < kQNs; ++s)
+#pragma unroll
+          for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int r = 0; r < RR; ++r) acc[s][i][r] = __builtin_fmaf(sc[s][g], P[s][i][r], acc[s][i][r]);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+  };
+  auto finish = [&](int pair) {
+#pragma unroll
+    for (int s = 0; s < kQNs; ++s) {
+      const int col = (pair * kQNs + s) * 16 + c16;
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int r = 0; r < RR; ++r) {
+          const int row = 16 * i + RR * h + r;
+          if (col < a.V && row < rows) a.out[(m0 + row) * a.ldo + col] = acc[s][i][r];
+          acc[s][i][r] = 0.0f;
+        }
+    }
+  };
+  if constexpr (CH) {
+    for (; c0 < nun; c0 += chu) {
+      if (c0) __syncthreads();
+      const int end = min(c0 + chu, nun);
+      stage(c0, end - c0);
+      __syncthreads();
+      if (!mine) continue;
+      for (cu = c0; cu < end;) {
+#pragma unroll
+        for (int u = 0; u < kQAhead; ++u) {  // chu is even: a chunk begins in slot 0
+          if (cu < end) unit(u);
+          ++cu;
+        }
+      }
+    }
+    if (mine) finish(first);
+  } else {
+    const int total = mine * nun;
+    for (int it = 0; it < total; it += kQAhead) {
+#pragma unroll
+      for (int u = 0; u < kQAhead; ++u) {
+        unit(u);
+        if (++cu == nun) {
+          if (it + u < total) finish(cp);
+          cu = 0;
+          cp += pstep;
+        }
       }
     }
   }
 }
 
-// LDS of k_head_q4_few: x and its group sums, and a wave's scales.
-size_t few_lds(int rows, int rt, int D, int group) {
-  const size_t nblk = (D + 127) / 128;
-  return ((rows * (nblk * 128 + 8) * 2 + 15) & ~size_t{15}) + nblk * (128 / group) * rt * sizeof(float);
+// LDS: `units` units of x with their group sums, and what a wave has of its own.
+size_t x_lds(int rows, int rt, int units, int group) {
+  return ((static_cast<size_t>(rows) * (units * 256 + 8) * 2 + 15) & ~size_t{15}) +
+         static_cast<size_t>(units) * (256 / group) * rt * sizeof(float);
 }
-size_t wave_lds(int group, bool zp) { return 16 * kQNs * 2 * (128 / group) * sizeof(float) * (zp ? 2 : 1); }
-constexpr size_t kFewLds = 160 * 1024;
-constexpr int kFewWaves = 4;  // the fewest that the rest of the LDS must hold
+size_t wave_lds(int group, bool zp) { return kQTurn + 16 * kQNs * 2 * (128 / group) * sizeof(float) * (zp ? 2 : 1); }
+constexpr size_t kMostLds = 160 * 1024;
+
+struct Shape {
+  bool chunks;
+  int units, waves;  // units of x in LDS; waves of a workgroup at most
+};
+// What fits: x whole with at least kFewWaves waves, or as many units of it as do with the most waves.
+Shape shape_of(int rows, int rt, int D, int group, bool zp, int most) {
+  constexpr int kFewWaves = 4;
+  const int nun = (D + 255) / 256;
+  const size_t whole = x_lds(rows, rt, nun, group), own = wave_lds(group, zp);
+  if (whole + kFewWaves * own <= kMostLds) return {false, nun, std::min(most, static_cast<int>((kMostLds - whole) / own))};
+  int u = 2;
+  while (u + 2 < nun && x_lds(rows, rt, u + 2, group) + most * own <= kMostLds) u += 2;
+  return {true, u, most};
+}
+
+template <bool H, int G, int RT, bool ZP, int ST, bool CH>
+void launch_kernel(const HeadQ4Args& a, dim3 grid, int nw, size_t lds, int rows_ld, int pairs, int units, hipStream_t st) {
+  static DynLdsOnce configured;
+  allow_dyn_lds(configured, {reinterpret_cast<const void*>(k_head_q4<H, G, RT, ZP, ST, CH>)}, static_cast<int>(kMostLds));
+  hipLaunchKernelGGL((k_head_q4<H, G, RT, ZP, ST, CH>), grid, dim3(64 * nw), lds, st, a, rows_ld, pairs, units);
+}
 
 template <bool H, int G, int RT, bool ZP, int ST>
-void launch_few_as(const HeadQ4Args& a, int cus, hipStream_t st) {
-  const int rows_ld = a.B < RT ? a.B : RT, groups = (a.B + RT - 1) / RT;
+void launch_as(const HeadQ4Args& a, int cus, hipStream_t st) {
+  const int rows_ld = std::min(a.B, RT), groups = (a.B + RT - 1) / RT;
   const int pairs = (a.V + 16 * kQNs - 1) / (16 * kQNs);
-  // waves per workgroup: as many rounds of pairs as the most waves would need, and no more waves than those fill
-  const size_t x_lds = few_lds(rows_ld, RT, a.D, G);
-  const int most = std::min(few_waves(RT, ST), static_cast<int>((kFewLds - x_lds) / wave_lds(G, ZP)));
-  const int wgs = cus > 0 ? cus : 256, per = (pairs + wgs - 1) / wgs, rounds = (per + most - 1) / most;
-  const int nw = (per + rounds - 1) / rounds;
-  static DynLdsOnce configured;
-  allow_dyn_lds(configured, {reinterpret_cast<const void*>(k_head_q4_few<H, G, RT, ZP, ST>)}, static_cast<int>(kFewLds));
-  const dim3 grid((pairs + nw - 1) / nw < wgs ? (pairs + nw - 1) / nw : wgs, groups);
-  hipLaunchKernelGGL((k_head_q4_few<H, G, RT, ZP, ST>), grid, dim3(64 * nw), x_lds + nw * wave_lds(G, ZP), st, a, rows_ld, pairs);
-}
-template <bool H, int G, int RT, bool ZP>
-void launch_few_zp(const HeadQ4Args& a, int cus, hipStream_t st) {
-  if (a.sc_type == VSMP_F32)
-    launch_few_as<H, G, RT, ZP, VSMP_F32>(a, cus, st);
-  else if (a.sc_type == VSMP_BF16)
-    launch_few_as<H, G, RT, ZP, VSMP_BF16>(a, cus, st);
-  else
-    launch_few_as<H, G, RT, ZP, VSMP_F16>(a, cus, st);
+  const Shape sh = shape_of(rows_ld, RT, a.D, G, ZP, few_waves(RT, G, ZP, ST));
+  int nw = sh.waves;
+  // as many rounds of pairs as the most waves would need, and no more waves than those fill
+  const int wgs = cus > 0 ? cus : 256, per = (pairs + wgs - 1) / wgs, rounds = (per + nw - 1) / nw;
+  nw = (per + rounds - 1) / rounds;
+  const int need = (pairs + nw - 1) / nw;
+  const size_t lds = x_lds(rows_ld, RT, sh.units, G) + nw * wave_lds(G, ZP);
+  if (!sh.chunks)
+    launch_kernel<H, G, RT, ZP, ST, false>(a, dim3(std::min(need, wgs), groups), nw, lds, rows_ld, pairs, sh.units, st);
+  else if constexpr (RT == 16 || RT == 32)  // four rows always fit, and 64 are taken where they do
+    launch_kernel<H, G, RT, ZP, ST, true>(a, dim3(need, groups), nw, lds, rows_ld, pairs, sh.units, st);
 }
 template <bool H, int G, int RT>
-bool launch_few(const HeadQ4Args& a, int cus, hipStream_t st) {
-  if (a.D < 128 || few_lds(a.B < RT ? a.B : RT, RT, a.D, G) + kFewWaves * wave_lds(G, a.z != nullptr) > kFewLds) return false;
+void launch_rows(const HeadQ4Args& a, int cus, hipStream_t st) {
+  auto go = [&](auto zp) {
+    constexpr bool ZP = decltype(zp)::value;
+    if (a.sc_type == VSMP_F32)
+      launch_as<H, G, RT, ZP, VSMP_F32>(a, cus, st);
+    else if (a.sc_type == VSMP_BF16)
+      launch_as<H, G, RT, ZP, VSMP_BF16>(a, cus, st);
+    else
+      launch_as<H, G, RT, ZP, VSMP_F16>(a, cus, st);
+  };
   if (a.z)
-    launch_few_zp<H, G, RT, true>(a, cus, st);
+    go(std::true_type{});
   else
-    launch_few_zp<H, G, RT, false>(a, cus, st);
-  return true;
+    go(std::false_type{});
 }
-
-// ---- launches ----------------------------------------------------------------------------------------------
 
 template <bool H, int G, int MB, bool ZP>
 void launch_tile(const HeadQ4Args& a, hipStream_t st) {
@@ -546,28 +614,29 @@ void launch_tile(const HeadQ4Args& a, hipStream_t st) {
   const dim3 grid((a.V + kQBn - 1) / kQBn, (a.B + MB * 16 - 1) / (MB * 16));
   constexpr int kMost = 2 * (MB * 16 * (KC + 8) * 2 + KC / G * MB * 16 * 4 + kQBn * (KC / G) * 4 * (ZP ? 2 : 1));
   static DynLdsOnce configured;
-  allow_dyn_lds(configured, {reinterpret_cast<const void*>(k_head_q4<H, G, MB, ZP, KC>)}, kMost);
-  hipLaunchKernelGGL((k_head_q4<H, G, MB, ZP, KC>), grid, dim3(kQNt), 2 * stage, st, a, rows_ld);
+  allow_dyn_lds(configured, {reinterpret_cast<const void*>(k_head_q4_tile<H, G, MB, ZP, KC>)}, kMost);
+  hipLaunchKernelGGL((k_head_q4_tile<H, G, MB, ZP, KC>), grid, dim3(kQNt), 2 * stage, st, a, rows_ld);
 }
 
-template <bool H, int G, int MB>
-void launch_tiles(const HeadQ4Args& a, hipStream_t st) {
-  if (a.z)
-    launch_tile<H, G, MB, true>(a, st);
-  else
-    launch_tile<H, G, MB, false>(a, st);
-}
-
+// The rows of a workgroup: the fewest of 4, 16 and 32 that hold the batch, 64 for larger batches where their x fits
+// whole, else groups of 32 (64 x 151,936 x 2,048 100 us in two groups of 32 against 115 in chunks of 64; 64 x
+// 128,256 x 4,096 about 180 / 214; 24 rows of 4,096 in chunks of 32 90 against 120 in two groups of 16; 128 x 151,936 x
+// 1,024 80 us in two groups of 64).
 template <bool H, int G>
 void launch_group(const HeadQ4Args& a, int cus, hipStream_t st) {
-  if (a.B <= 4) {
-    if (!launch_few<H, G, 4>(a, cus, st)) launch_tiles<H, G, 1>(a, st);
+  if (a.D < 256) {
+    if (a.z)
+      launch_tile<H, G, 1, true>(a, st);
+    else
+      launch_tile<H, G, 1, false>(a, st);
+  } else if (a.B <= 4) {
+    launch_rows<H, G, 4>(a, cus, st);
   } else if (a.B <= 16) {
-    if (!launch_few<H, G, 16>(a, cus, st)) launch_tiles<H, G, 1>(a, st);
-  } else if (a.B <= 32) {
-    if (!launch_few<H, G, 32>(a, cus, st)) launch_tiles<H, G, 2>(a, st);
+    launch_rows<H, G, 16>(a, cus, st);
+  } else if (a.B <= 32 || shape_of(std::min(a.B, 64), 64, a.D, G, a.z != nullptr, 8).chunks) {
+    launch_rows<H, G, 32>(a, cus, st);
   } else {
-    if (!launch_few<H, G, 64>(a, cus, st)) launch_tiles<H, G, 4>(a, st);
+    launch_rows<H, G, 64>(a, cus, st);
   }
 }
 
