@@ -302,24 +302,46 @@ def _head_shapes(hidden, head):
     return hidden.shape[0], hidden.shape[1], head.shape[0]
 
 
-_DTYPES = None  # torch dtype -> vsmp_dtype, once torch is there
+class _Torch:
+    """What the calls below need of torch, looked up once: they are short enough for an import statement and a
+    Stream object per call to show."""
 
-
-def _dtype(t, name):
-    global _DTYPES
-    if _DTYPES is None:
+    def __init__(self):
         import torch
 
-        _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-    code = _DTYPES.get(t.dtype)
-    if code is None:
-        raise VsmpError(f"{name} must be float32, bfloat16 or float16")
-    return code
+        self.empty, self.int32, self.float32, self.uint8 = torch.empty, torch.int32, torch.float32, torch.uint8
+        self.codes = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # vsmp_dtype
+        self._raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        self._current = torch.cuda.current_stream
+
+    def stream(self, stream, device):
+        """The address of `stream`, or of torch's current one on `device`."""
+        if stream is not None:
+            return stream.cuda_stream
+        return self._raw(device.index) if self._raw is not None else self._current(device).cuda_stream
+
+    def rows16(self, B, V, device):
+        """A new float32 [B, V] whose rows are padded to 16 bytes, and their stride."""
+        ld = (V + 3) // 4 * 4
+        t = self.empty((B, ld), dtype=self.float32, device=device)
+        return (t if ld == V else t[:, :V]), ld
+
+
+_torch = None
+
+
+def _t():
+    global _torch
+    if _torch is None:
+        _torch = _Torch()
+    return _torch
 
 
 def _rows_of(t, name, device):
     """(dtype code, row stride) of a 2-D matrix with contiguous rows on `device` (of a single row: its length)."""
-    code = _dtype(t, name)
+    code = _t().codes.get(t.dtype)
+    if code is None:
+        raise VsmpError(f"{name} must be float32, bfloat16 or float16")
     if t.dim() != 2 or not t.is_cuda or t.device != device:
         raise VsmpError(f"{name} must be a 2-D tensor on {device}")
     rows, cols = t.shape
@@ -352,26 +374,23 @@ def _adjust_args(logits, penalty, hist, hist_off, prompt_len, bias_ids, bias, bi
                  csr=True):
     """The arguments of an adjust call as (in, dtype, ldi), (B, V), the penalties, histories, and the rest up to the
     stream; `out`; and what the addresses need kept alive."""
-    import torch
-
+    T = _t()
     dev = logits.device
     code, ld = _rows_of(logits, "logits", dev)
     B, V = logits.shape
     if out is None:  # rows on 16 bytes, so that pick_batch can take them
-        out = torch.empty(B, (V + 3) // 4 * 4, dtype=torch.float32, device=dev)
-        ldo = out.stride(0)
-        out = out[:, :V]
+        out, ldo = T.rows16(B, V, dev)
     else:
         ocode, ldo = _rows_of(out, "out", dev)
         if ocode != 0 or out.shape != logits.shape:
             raise VsmpError("out must be float32 of the logits' shape")
-    i32 = torch.int32
+    i32 = T.int32
     if penalty is None or isinstance(penalty, Penalty):
         pp, per_row = (ctypes.addressof(penalty) if penalty is not None else None), 0
     else:
-        if penalty.dtype != torch.uint8 or penalty.numel() != 16 * B:
+        if penalty.dtype != T.uint8 or penalty.numel() != 16 * B:
             raise VsmpError("per-row penalties must hold B entries (to_device_penalties)")
-        pp, per_row = _array_of(penalty, torch.uint8, 16 * B, "per-row penalties", dev), 1
+        pp, per_row = _array_of(penalty, T.uint8, 16 * B, "per-row penalties", dev), 1
     if csr:
         if (hist is None) != (hist_off is None):
             raise VsmpError("hist and hist_off go together")
@@ -392,12 +411,11 @@ def _adjust_args(logits, penalty, hist, hist_off, prompt_len, bias_ids, bias, bi
         n_masks = mask.shape[0]
         ldm = mask.stride(0) if n_masks > 1 else mask.shape[1]
         mp = mask.data_ptr()
-    st = stream if stream is not None else torch.cuda.current_stream(dev)
     rest = (_array_of(prompt_len, i32, B, "prompt_len", dev), _array_of(bias_ids, i32, 0, "bias_ids", dev),
-            _array_of(bias, torch.float32, bias_ids.numel() if bias_ids is not None else 0, "bias", dev),
+            _array_of(bias, T.float32, bias_ids.numel() if bias_ids is not None else 0, "bias", dev),
             _array_of(bias_off, i32, B + 1, "bias_off", dev), mp, ldm, n_masks,
             _array_of(mask_row, i32, B, "mask_row", dev), out.data_ptr(), ldo, _array_of(left, i32, B, "left", dev),
-            st.cuda_stream)
+            T.stream(stream, dev))
     return (logits.data_ptr(), code, ld), (B, V), (pp, per_row), (h, ho), rest, out
 
 
@@ -509,28 +527,26 @@ class Context:
         device logits [B, V] (float32, bfloat16 or float16), their ranks in the sampler's order (rank=False: None)
         and each row's log of the sum of exponentials. Ids outside [0, V) give -inf and rank -1. Returns (logprob
         float32 [B, n], rank int32 [B, n], lse float32 [B]); without ids the first two are None."""
-        import torch
-
+        T = _t()
         self._check_device(logits)
         dev = logits.device
         code, ld = _rows_of(logits, "logits", dev)
         B, V = logits.shape
-        lse = torch.empty(B, dtype=torch.float32, device=dev)
+        lse = T.empty((B,), dtype=T.float32, device=dev)
         lp = rk = None
         n = ldj = 0
         if ids is not None:
-            if ids.dtype != torch.int32 or ids.dim() != 2 or ids.shape[0] != B or ids.device != dev:
+            if ids.dtype != T.int32 or ids.dim() != 2 or ids.shape[0] != B or ids.device != dev:
                 raise VsmpError("ids must be an int32 tensor [B, n] on the logits' device")
             n = ids.shape[1]
             if n > 1 and ids.stride(1) != 1:
                 raise VsmpError("ids must have contiguous rows")
             ldj = ids.stride(0) if B > 1 else n
-            lp = torch.empty(B, n, dtype=torch.float32, device=dev)
-            rk = torch.empty(B, n, dtype=torch.int32, device=dev) if rank else None
-        st = stream if stream is not None else torch.cuda.current_stream(dev)
+            lp = T.empty((B, n), dtype=T.float32, device=dev)
+            rk = T.empty((B, n), dtype=T.int32, device=dev) if rank else None
         if _lib.vsmp_logprobs(self._h, logits.data_ptr(), code, ld, B, V, ids.data_ptr() if n else None, ldj, n,
                               lp.data_ptr() if n else None, rk.data_ptr() if n and rk is not None else None,
-                              lse.data_ptr(), st.cuda_stream) != 0:
+                              lse.data_ptr(), T.stream(stream, dev)) != 0:
             raise _err()
         return lp, rk, lse
 
@@ -539,15 +555,14 @@ class Context:
         scales[c, d / group] * (q[c, d] - zeros[c, d / group]). hidden: bfloat16 or float16 [B, D]; q: uint8
         [V, D / 2], two weights a byte, the even d in the low half; scales: float32, bfloat16 or float16 [V, D /
         group]; zeros: uint8 [V, D / group], or None for 8. Returns logits (float32 [B, V] unless given)."""
-        import torch
-
+        T = _t()
         self._check_device(hidden)
         dev = hidden.device
         code, ldh = _rows_of(hidden, "hidden", dev)
         if code == 0:
             raise VsmpError("hidden must be bfloat16 or float16")
         B, D = hidden.shape
-        if q.dtype != torch.uint8 or q.dim() != 2 or q.device != dev or (q.shape[1] > 1 and q.stride(1) != 1):
+        if q.dtype != T.uint8 or q.dim() != 2 or q.device != dev or (q.shape[1] > 1 and q.stride(1) != 1):
             raise VsmpError("q must be a 2-D uint8 tensor with contiguous rows on the hidden states' device")
         V = q.shape[0]
         if 2 * q.shape[1] != D:
@@ -558,22 +573,20 @@ class Context:
             raise VsmpError("scales must be [V, D / group]")
         ldz = 0
         if zeros is not None:
-            if zeros.dtype != torch.uint8 or zeros.shape != scales.shape or zeros.device != dev or \
+            if zeros.dtype != T.uint8 or zeros.shape != scales.shape or zeros.device != dev or \
                     (zeros.shape[1] > 1 and zeros.stride(1) != 1):
                 raise VsmpError("zeros must be uint8 of the scales' shape with contiguous rows")
             ldz = zeros.stride(0) if V > 1 else zeros.shape[1]
         if logits is None:  # rows padded to 16 bytes, so that pick_batch can take them
-            ldl = (V + 3) // 4 * 4
-            logits = torch.empty(B, ldl, dtype=torch.float32, device=dev)[:, :V]
+            logits, ldl = T.rows16(B, V, dev)
         else:
             lcode, ldl = _rows_of(logits, "logits", dev)
             if lcode != 0 or logits.shape != (B, V):
                 raise VsmpError("logits must be float32 [B, V]")
-        st = stream if stream is not None else torch.cuda.current_stream(dev)
         if _lib.vsmp_head_logits_q4(self._h, hidden.data_ptr(), code, ldh, q.data_ptr(),
                                     q.stride(0) if V > 1 else D // 2,
                                     scales.data_ptr(), scode, lds, zeros.data_ptr() if zeros is not None else None, ldz,
-                                    group, B, V, D, logits.data_ptr(), ldl, st.cuda_stream) != 0:
+                                    group, B, V, D, logits.data_ptr(), ldl, T.stream(stream, dev)) != 0:
             raise _err()
         return logits
 

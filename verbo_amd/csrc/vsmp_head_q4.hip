@@ -586,7 +586,7 @@ void launch_as(const HeadQ4Args& a, int cus, hipStream_t st) {
   const size_t lds = x_lds(rows_ld, RT, sh.units, G) + nw * wave_lds(G, ZP);
   if (!sh.chunks)
     launch_kernel<H, G, RT, ZP, ST, false>(a, dim3(std::min(need, wgs), groups), nw, lds, rows_ld, pairs, sh.units, st);
-  else if constexpr (RT == 16 || RT == 32)  // four rows always fit, and 64 are taken where they do
+  else if constexpr (RT > 4)  // four rows always fit
     launch_kernel<H, G, RT, ZP, ST, true>(a, dim3(need, groups), nw, lds, rows_ld, pairs, sh.units, st);
 }
 template <bool H, int G, int RT>
@@ -618,10 +618,10 @@ void launch_tile(const HeadQ4Args& a, hipStream_t st) {
   hipLaunchKernelGGL((k_head_q4_tile<H, G, MB, ZP, KC>), grid, dim3(kQNt), 2 * stage, st, a, rows_ld);
 }
 
-// The rows of a workgroup: the fewest of 4, 16 and 32 that hold the batch, 64 for larger batches where their x fits
-// whole, else groups of 32 (64 x 151,936 x 2,048 100 us in two groups of 32 against 115 in chunks of 64; 64 x
-// 128,256 x 4,096 about 180 / 214; 24 rows of 4,096 in chunks of 32 90 against 120 in two groups of 16; 128 x 151,936 x
-// 1,024 80 us in two groups of 64).
+// The rows of a workgroup: the fewest of 4, 16 and 32 that hold the batch; for larger ones 64, or 32 where the x of
+// 32 rows fits whole and that of 64 does not (64 x 151,936 x 2,048 100 us in two groups of 32 against 115 in chunks of
+// 64; where neither fits, 40 x 128,256 x 4,096 164 / 121 and 64 rows 261 / 214; 24 rows of 4,096 in chunks of 32 90 us
+// against 120 in two groups of 16).
 template <bool H, int G>
 void launch_group(const HeadQ4Args& a, int cus, hipStream_t st) {
   if (a.D < 256) {
@@ -633,10 +633,13 @@ void launch_group(const HeadQ4Args& a, int cus, hipStream_t st) {
     launch_rows<H, G, 4>(a, cus, st);
   } else if (a.B <= 16) {
     launch_rows<H, G, 16>(a, cus, st);
-  } else if (a.B <= 32 || shape_of(std::min(a.B, 64), 64, a.D, G, a.z != nullptr, 8).chunks) {
-    launch_rows<H, G, 32>(a, cus, st);
   } else {
-    launch_rows<H, G, 64>(a, cus, st);
+    const bool zp = a.z != nullptr;
+    const bool whole32 = !shape_of(32, 32, a.D, G, zp, 8).chunks, whole64 = !shape_of(std::min(a.B, 64), 64, a.D, G, zp, 8).chunks;
+    if (a.B <= 32 || (whole32 && !whole64))
+      launch_rows<H, G, 32>(a, cus, st);
+    else
+      launch_rows<H, G, 64>(a, cus, st);
   }
 }
 

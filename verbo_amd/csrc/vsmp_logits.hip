@@ -70,7 +70,8 @@ constexpr uint32_t kSeen = 0x80000000u;  // a slot's mark of a prompt id; the bi
 // One part of kAdjustParts logits, 16 per thread as four groups of four. The part's histories are
 // counted in LDS, a word per logit (integer atomics, so that the order does not matter); the last
 // entry that biases a logit is the largest index + 1 in a second array. Each thread's logits are in
-// flight while the lists are read. An element without a mark costs its LDS read alone.
+// flight while the lists are read. An element without a mark costs its LDS read alone. Logits of four
+// that the mask forbids are not read.
 template <class E, bool BIAS>
 __global__ __launch_bounds__(kNt) void k_adjust(AdjustArgs a) {
   __shared__ __align__(16) uint32_t s_cnt[kAdjustParts];
@@ -83,12 +84,6 @@ __global__ __launch_bounds__(kNt) void k_adjust(AdjustArgs a) {
   const char* in = static_cast<const char*>(a.in) + (row * a.ldi + lo) * E::kSize;
   float* out = a.out + row * a.ldo + lo;
 
-  Raw<E, 4> x[4];
-#pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const int e = 4 * (tid + g * kNt);
-    if (e + 4 <= len) x[g].load(in, e);
-  }
   uint32_t allow[4] = {0xFu, 0xFu, 0xFu, 0xFu};
   if (a.mask) {
     const int m = a.mask_row ? a.mask_row[row] : row;
@@ -100,6 +95,13 @@ __global__ __launch_bounds__(kNt) void k_adjust(AdjustArgs a) {
         allow[g] = m < a.n_masks && e < len ? (words[e >> 5] >> (e & 31)) & 0xFu : 0u;
       }
     }
+  }
+  Raw<E, 4> x[4];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int e = 4 * (tid + g * kNt);
+    x[g] = {};
+    if (e + 4 <= len && allow[g]) x[g].load(in, e);
   }
 
   const vsmp_penalty pen = a.pen ? a.pen[row] : a.shared;
@@ -124,14 +126,32 @@ __global__ __launch_bounds__(kNt) void k_adjust(AdjustArgs a) {
       if (BIAS) *reinterpret_cast<uint4*>(&s_bias[4 * (tid + g * kNt)]) = make_uint4(0u, 0u, 0u, 0u);
     }
     __syncthreads();
-    for (int i = h0 + tid; i < h1; i += kNt) {
-      const unsigned d = static_cast<unsigned>(a.hist[i]) - static_cast<unsigned>(lo);
-      if (d < static_cast<unsigned>(len)) {
+    auto count = [&](uint32_t id, int i) {
+      const uint32_t d = id - static_cast<uint32_t>(lo);
+      if (d < static_cast<uint32_t>(len)) {
         if (i < hp)
           atomicOr(&s_cnt[d], kSeen);
         else
           atomicAdd(&s_cnt[d], 1u);
       }
+    };
+    // eight ids a thread in flight; the last few one by one
+    int i = h0;
+    for (; h1 - i >= 8 * kNt; i += 8 * kNt) {
+      typedef uint32_t ids4 __attribute__((ext_vector_type(4), aligned(4)));
+      const int i0 = i + 4 * tid, i1 = i0 + 4 * kNt;
+      const ids4 u = *reinterpret_cast<const ids4*>(a.hist + i0), w = *reinterpret_cast<const ids4*>(a.hist + i1);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) count(u[k], i0 + k);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) count(w[k], i1 + k);
+    }
+    if (i < h1) {
+      uint32_t u[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) u[k] = i + tid + k * kNt < h1 ? static_cast<uint32_t>(a.hist[i + tid + k * kNt]) : 0xFFFFFFFFu;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) count(u[k], i + tid + k * kNt);
     }
     if (BIAS) {
       for (int i = b0 + tid; i < b1; i += kNt) {
@@ -155,6 +175,7 @@ __global__ __launch_bounds__(kNt) void k_adjust(AdjustArgs a) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) y[k] = e + k < len ? E::get(in, e + k) : -INFINITY;
     }
+    if (!allow[g]) y[0] = y[1] = y[2] = y[3] = -INFINITY;
     uint4 c = make_uint4(0u, 0u, 0u, 0u), b = c;
     if (counted) c = *reinterpret_cast<const uint4*>(&s_cnt[e]);
     if (biased) b = *reinterpret_cast<const uint4*>(&s_bias[e]);
