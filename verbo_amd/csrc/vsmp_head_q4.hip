@@ -582,6 +582,8 @@ void launch_as(const HeadQ4Args& a, int cus, hipStream_t st) {
   // as many rounds of pairs as the most waves would need, and no more waves than those fill
   const int wgs = cus > 0 ? cus : 256, per = (pairs + wgs - 1) / wgs, rounds = (per + nw - 1) / nw;
   nw = (per + rounds - 1) / rounds;
+  // With many rows the products bound it, and the SIMDs share them evenly (64 x 151,936 x 2,048: 8 waves 91 us, 7 101)
+  if (RT >= 32) nw = std::min(sh.waves, (nw + 3) / 4 * 4);
   const int need = (pairs + nw - 1) / nw;
   const size_t lds = x_lds(rows_ld, RT, sh.units, G) + nw * wave_lds(G, ZP);
   if (!sh.chunks)
