@@ -38,6 +38,24 @@ def test_header_compiles_as_c_and_the_struct_has_its_layout(tmp_path):
     assert (p.repeat, p.presence, p.frequency, p.window) == (1.0, 0.0, 0.0, 0)
 
 
+@pytest.mark.skipif(shutil.which("g++") is None, reason="g++ absent")
+def test_the_documented_step_compiles(tmp_path):
+    """The C++ block that INTEGRATION.md shows for these calls, with the variables that it names."""
+    block = [b for b in re.findall(r"```cpp\n(.*?)```", (ROOT / "INTEGRATION.md").read_text(), re.S) if "vsmp_logits.h" in b]
+    assert len(block) == 1
+    body = "\n".join(line for line in block[0].splitlines() if not line.startswith("#include"))
+    src = tmp_path / "step.cpp"
+    src.write_text("""#include "vsmp_logits.h"
+void step(vsmp_ctx* ctx, const void* d_hidden, long long ldh, const void* d_q, long long ldq, const void* d_scales, int B, int V,
+          int D, float* d_logits, long long ld, void* stream, const int* d_hist, const int* d_hist_off, const int* d_prompt_len,
+          const int* d_bias_ids, const float* d_bias, const int* d_bias_off, const unsigned* d_mask, long long ldm, int n_masks,
+          const int* d_mask_row, int* d_left, vsmp_params params, unsigned long long step, int* d_ids, float* d_logprob,
+          int* d_rank, float* d_lse) {
+""" + body + "\n}\n")
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-Wextra", "-Werror", "-I", str(ROOT / "include"), "-c", str(src), "-o",
+                    str(tmp_path / "step.o")], check=True)
+
+
 # Addresses that only the argument checks see: a call that they refuse reads nothing behind them.
 CTX, X, OUT, OTHER = 1 << 20, 1 << 32, 1 << 36, 1 << 40
 INF = float("inf")

@@ -1,21 +1,27 @@
-// The LM head's product with 4-bit weights (k_head_q4): logits = x . (s (q - z))^T.
+// The LM head's product with 4-bit weights: logits = x . (s (q - z))^T.
 //
 // A weight enters the matrix cores unrounded. A nibble q moved to the top of a 16-bit float's mantissa
-// under the exponent of 16 is the number 16 + q (bf16: bits 3-6, f16: bits 6-9), two shifts and masks
+// under the exponent of 16 is the number 16 + q (bf16: bits 3-6, f16: bits 6-9), a shift and an and-or
 // for two weights. With o = 16 + z,
 //   sum_{d in g} x_d (q_d - z) = sum_{d in g} x_d (16 + q_d) - o X_g,   X_g = sum_{d in g} x_d,
 // so the group's MFMAs start from -o X_g and the group's result is scaled and added in fp32:
 //   acc += s_g P_g.
 // The intermediate sums are at most some 31 / 8 of those of the centred weights, which costs one to two
-// bits of the fp32 accumulation.
+// bits of the fp32 accumulation (measured against 64 bits: 1.1e-7 to 3.7e-7 of the result, where the fp32
+// product of the unpacked weights has 2.1e-7 to 9.7e-7).
 //
-// Tiles: a workgroup of four waves takes MB x 16 rows and 128 columns, each wave two strips of 16
-// columns on v_mfma_f32_16x16x32. Weights go from HBM to registers, 16 bytes a lane: lane (column c,
-// quarter h) holds the 32 weights [32 h, 32 h + 32) of a block of 128 of its column, each chunk of KC
-// loaded while the one before is multiplied. An MFMA sums over the four quarters, so for groups of 32
-// (64) the quarters' dwords are transposed between lanes 16 and 32 apart (32 apart) with the lane
-// swaps, until an MFMA's four quarters lie in one group. x and the scales go through LDS, staged per
-// chunk in two buffers; x in the order in which the nibbles of a dword come out: 0 4 1 5 2 6 3 7.
+// Strips of 16 columns on v_mfma_f32_16x16x32. An operand's lane (column c, quarter h) holds the 32 weights
+// [32 h, 32 h + 32) of a block of 128 of its column as four dwords. An MFMA sums over the four quarters, so for
+// groups of 32 (64) the quarters' dwords are transposed between lanes 16 and 32 apart (32 apart) with the lane
+// swaps, until an MFMA's four quarters lie in one group. x lies in LDS in the order in which the nibbles of a
+// dword come out: 0 4 1 5 2 6 3 7.
+//
+// What bounds it: few rows read their weights and scales once from HBM (1 x 128,256 x 4,096 in groups of 32: 57 us,
+// 5.2 TB/s; 4 x 151,936 x 2,048: 33 us, 5.0 TB/s); small hidden sizes the launch, the staging of x and the few units a
+// wave has (1 x 151,936 x 896: 24 us, 3.3 TB/s); many rows the conversions, the scaling and the LDS reads beside
+// the MFMAs (64 x 151,936 x 2,048: 91 us, 440 TFLOP/s).
+//
+// k_head_q4 takes hidden sizes from 256 on, k_head_q4_tile the smaller ones.
 #include <algorithm>
 
 #include "vsmp_lds.hpp"
@@ -28,7 +34,6 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kQNt = 256;  // threads per workgroup
 constexpr int kQNs = 2;    // strips of 16 columns per wave
@@ -86,10 +91,14 @@ __device__ __forceinline__ void swap16(uint32_t& a, uint32_t& b) {
   b = r[1];
 }
 
-// H: f16 hidden states (else bf16). G: group. MB: blocks of 16 rows. ZP: zero points given. KC: hidden
+// The small hidden sizes: a workgroup of four waves takes 16 rows and 128 columns, x and the scales staged in
+// LDS by chunks of KC in two buffers, the next chunk's weights loaded while one is multiplied.
+//
+// H: f16 hidden states (else bf16). G: group. ZP: zero points given. KC: hidden
 // elements per chunk.
-template <bool H, int G, int MB, bool ZP, int KC>
+template <bool H, int G, bool ZP, int KC>
 __global__ __launch_bounds__(kQNt) void k_head_q4_tile(HeadQ4Args a, int rows_ld) {
+  constexpr int MB = 1;               // blocks of 16 rows
   constexpr int kStr = KC + 8;        // halfwords per x row in LDS: 16 rows' reads fall on distinct banks
   constexpr int kBlk = KC / 128;      // blocks of 128 per chunk
   constexpr int kGc = KC / G;         // groups per chunk
@@ -272,7 +281,7 @@ __global__ __launch_bounds__(kQNt) void k_head_q4_tile(HeadQ4Args a, int rows_ld
   }
 }
 
-// ---- few rows: x stays in LDS ----------------------------------------------------------------------------
+// ---- hidden sizes from 256 on: x stays in LDS ------------------------------------------------------------
 
 constexpr int kQAhead = 2;    // units of 256 in flight per wave and strip
 constexpr int kQTurn = 2048;  // bytes of LDS in which a strip's unit is turned
@@ -608,16 +617,16 @@ void launch_rows(const HeadQ4Args& a, int cus, hipStream_t st) {
     go(std::false_type{});
 }
 
-template <bool H, int G, int MB, bool ZP>
+template <bool H, int G, bool ZP>
 void launch_tile(const HeadQ4Args& a, hipStream_t st) {
-  constexpr int KC = MB == 1 ? 512 : 256;
-  const int rows_ld = a.B < MB * 16 ? a.B : MB * 16;
-  const int stage = rows_ld * (KC + 8) * 2 + KC / G * MB * 16 * 4 + kQBn * (KC / G) * 4 * (ZP ? 2 : 1);
-  const dim3 grid((a.V + kQBn - 1) / kQBn, (a.B + MB * 16 - 1) / (MB * 16));
-  constexpr int kMost = 2 * (MB * 16 * (KC + 8) * 2 + KC / G * MB * 16 * 4 + kQBn * (KC / G) * 4 * (ZP ? 2 : 1));
+  constexpr int KC = 256;
+  const int rows_ld = a.B < 16 ? a.B : 16;
+  const int stage = rows_ld * (KC + 8) * 2 + KC / G * 16 * 4 + kQBn * (KC / G) * 4 * (ZP ? 2 : 1);
+  const dim3 grid((a.V + kQBn - 1) / kQBn, (a.B + 15) / 16);
+  constexpr int kMost = 2 * (16 * (KC + 8) * 2 + KC / G * 16 * 4 + kQBn * (KC / G) * 4 * (ZP ? 2 : 1));
   static DynLdsOnce configured;
-  allow_dyn_lds(configured, {reinterpret_cast<const void*>(k_head_q4_tile<H, G, MB, ZP, KC>)}, kMost);
-  hipLaunchKernelGGL((k_head_q4_tile<H, G, MB, ZP, KC>), grid, dim3(kQNt), 2 * stage, st, a, rows_ld);
+  allow_dyn_lds(configured, {reinterpret_cast<const void*>(k_head_q4_tile<H, G, ZP, KC>)}, kMost);
+  hipLaunchKernelGGL((k_head_q4_tile<H, G, ZP, KC>), grid, dim3(kQNt), 2 * stage, st, a, rows_ld);
 }
 
 // The rows of a workgroup: the fewest of 4, 16 and 32 that hold the batch; for larger ones 64, or 32 where the x of
@@ -628,9 +637,9 @@ template <bool H, int G>
 void launch_group(const HeadQ4Args& a, int cus, hipStream_t st) {
   if (a.D < 256) {
     if (a.z)
-      launch_tile<H, G, 1, true>(a, st);
+      launch_tile<H, G, true>(a, st);
     else
-      launch_tile<H, G, 1, false>(a, st);
+      launch_tile<H, G, false>(a, st);
   } else if (a.B <= 4) {
     launch_rows<H, G, 4>(a, cus, st);
   } else if (a.B <= 16) {
