@@ -289,6 +289,18 @@ def test_adjust_long_histories(ctx):
     check_adjusted(got, left, *plain_adjust(x, [pen], hists, prompts))
 
 
+def test_adjust_prompt_lengths_beyond_the_history(ctx):
+    """A prompt length below 0 is none, one above the history's length is all of it, also at the type's ends."""
+    n = 500
+    x = np.zeros((4, n), np.float32)
+    h = np.tile(np.arange(10, dtype=np.int32), 4)
+    prompts = np.array([-(1 << 31), -1, (1 << 31) - 1, 11], np.int32)
+    got = ctx.adjust_logits(dev(x), V.Penalty(presence=1.0), dev(h), dev(np.arange(0, 41, 10, dtype=np.int32)), dev(prompts)).cpu().numpy()
+    want = np.zeros((4, n), np.float32)
+    want[:2, :10] = -1.0
+    assert np.array_equal(got, want)
+
+
 def test_adjust_repeat_is_the_picks_penalty(ctx):
     """The multiplicative penalty applied here and the one inside the pick give the same picks, penalised logits
     included: 40 rows, greedy and sampled."""

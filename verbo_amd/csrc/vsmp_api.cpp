@@ -140,7 +140,7 @@ struct vsmp_ctx {
   size_t n_rcand = 0;
   int* h_rcnt = nullptr;
   size_t n_rcnt = 0;
-  // the operators around the pick (ops_scratch): one allocation of a fixed size, zero between calls
+  // the operators around the pick (ops_scratch): one allocation of a fixed size, its tickets zero between calls
   unsigned char* o_scr = nullptr;
   size_t n_oscr = 0;
   // host-pointer path (vsmp_pick_host): one pinned host area, mapped into the device's address

@@ -110,7 +110,7 @@ __global__ __launch_bounds__(kNt) void k_adjust(AdjustArgs a) {
     const int seq = a.slot ? a.slot[row] : row;
     h0 = a.hist_off[seq];
     h1 = a.hist_len ? h0 + a.hist_len[seq] : a.hist_off[seq + 1];
-    hp = h0 + (a.prompt_len ? a.prompt_len[row] : 0);
+    hp = a.prompt_len ? h0 + min(max(a.prompt_len[row], 0), max(h1 - h0, 0)) : h0;
     if (pen.window > 0 && h1 - h0 > pen.window) h0 = h1 - pen.window;
   }
   int b0 = 0, b1 = 0;
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(kNt) void k_adjust(AdjustArgs a) {
     if (i < h1) {
       uint32_t u[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) u[k] = i + tid + k * kNt < h1 ? static_cast<uint32_t>(a.hist[i + tid + k * kNt]) : 0xFFFFFFFFu;
+      for (int k = 0; k < 8; ++k) u[k] = tid + k * kNt < h1 - i ? static_cast<uint32_t>(a.hist[i + tid + k * kNt]) : 0xFFFFFFFFu;
 #pragma unroll
       for (int k = 0; k < 8; ++k) count(u[k], i + tid + k * kNt);
     }

@@ -68,7 +68,7 @@ int adjust_logits(vsmp_ctx* ctx, AdjustArgs a, int dtype, bool pen_per_row, cons
     if (!ops_scratch(ctx, st, &s)) return -1;
     a.acc = s.left;
   }
-  const int rows = std::min(a.left ? kOpRows : 1 << 20, INT_MAX / a.P);
+  const int rows = std::min(a.left ? kOpRows : 1 << 20, (1 << 23) / a.P);  // a launch takes fewer than 2^32 threads
   for (int r = 0; r < a.B; r += rows) {  // the counting words of one launch serve the next one too
     AdjustArgs p = a;
     p.B = std::min(rows, a.B - r);
