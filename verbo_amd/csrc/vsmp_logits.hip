@@ -72,6 +72,11 @@ constexpr uint32_t kSeen = 0x80000000u;  // a slot's mark of a prompt id; the bi
 // entry that biases a logit is the largest index + 1 in a second array. Each thread's logits are in
 // flight while the lists are read. An element without a mark costs its LDS read alone. Logits of four
 // that the mask forbids are not read.
+//
+// Bound by the logits' read and the output's write: 512 x 128,256 f16 without histories 73 us (5.4 TB/s), 256 x
+// 151,936 fp32 54 us (5.8 TB/s), with 512 ids of history a row 56 us. Histories are read by every part of their row:
+// 512 x 128,256 with 5,000 ids a row 79 us. 64 x 151,936 with 40 tokens allowed a row 16.0 us, 20.2 where forbidden
+// logits are read too.
 template <class E, bool BIAS>
 __global__ __launch_bounds__(kNt) void k_adjust(AdjustArgs a) {
   __shared__ __align__(16) uint32_t s_cnt[kAdjustParts];
@@ -291,7 +296,8 @@ __device__ __forceinline__ float next_up(float v) {
 }
 
 // One part of a row, a step of four 16-byte groups per thread at a time, the next step's in flight while one
-// is summed.
+// is summed. Bound by the logits' read where there are many: 2,048 x 128,256 bf16 83 us without ids (6.3 TB/s), 86 us
+// with one id a row; few rows by latencies and the parts' hand-off: one row of 151,936 fp32 4.1 us, with 20 ids 6.6.
 //
 // Ranks: a wave keeps the asked ids' logits one in a lane and counts, per step, the logits before each. Only ids
 // that the step's largest logit reaches can gain, and the ids that are asked for are mostly the likeliest, so
