@@ -426,6 +426,24 @@ def test_logprobs_extreme_rows(ctx):
     assert lp[2, 1] == 0.0 and rank[2].tolist() == [1, 0, 4321, n - 1]
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lanes", [1, 2, 4, 5, 16])
+def test_logprobs_crowded_tops(ctx, dtype, lanes):
+    """Large logits, with and without ties, that a few lanes of every lane row hold in all their groups: from a list
+    that takes them to more than it holds and more lanes than it takes. Ids among them, between them and far below."""
+    n, N = 20000, 4 if dtype == "f32" else 8
+    rng = np.random.default_rng(lanes)
+    x = rng.normal(0, 1, (4, n)).astype(np.float32)
+    at = np.array([N * (16 * r + l + 256 * g) + k for r in range(4) for l in range(lanes) for g in range(4) for k in range(N)])
+    x[0, at] = 10.0
+    x[1, at] = 10.0 + rng.integers(0, 3, at.size)
+    x[2, at] = np.linspace(8.0, 16.0, at.size)
+    x[3, at] = 10.0 + rng.random(at.size)
+    x[:, at + 1] = np.where(rng.random((4, at.size)) < 0.3, 9.0, x[:, at + 1])
+    ids = np.concatenate([rng.choice(at, (4, 40)), rng.choice(at, (4, 10)) + 1, rng.integers(0, n, (4, 13)), np.full((4, 1), at[0])], 1)
+    check_logprobs(ctx, dev(x, dtype), ids.astype(np.int32))
+
+
 def test_logprobs_of_the_candidates(ctx):
     """The ids that pick_batch reports in order are at ranks 0, 1, 2, ... and the picked one at its info's rank."""
     import torch
