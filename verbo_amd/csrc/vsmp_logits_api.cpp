@@ -69,9 +69,10 @@ int adjust_logits(vsmp_ctx* ctx, AdjustArgs a, int dtype, bool pen_per_row, cons
     a.acc = s.left;
   }
   const int rows = std::min(a.left ? kOpRows : 1 << 20, (1 << 23) / a.P);  // a launch takes fewer than 2^32 threads
-  for (int r = 0; r < a.B; r += rows) {  // the counting words of one launch serve the next one too
+  for (int r = 0, n; r < a.B; r += n) {  // the counting words of one launch serve the next one too
+    n = std::min(rows, a.B - r);
     AdjustArgs p = a;
-    p.B = std::min(rows, a.B - r);
+    p.B = n;
     p.in = static_cast<const char*>(a.in) + static_cast<size_t>(r) * a.ldi * elem_size(dtype);
     p.out = a.out + static_cast<size_t>(r) * a.ldo;
     if (a.pen) p.pen = a.pen + r;
@@ -150,9 +151,10 @@ int vsmp_logprobs(vsmp_ctx* ctx, const void* logits, int dtype, long long ld, in
   a.ldj = ldj;
   a.n = n;
   const int rows = 1 << 20;  // of one launch
-  for (int r = 0; r < B; r += rows) {
+  for (int r = 0, m; r < B; r += m) {
+    m = std::min(rows, B - r);
     vsmp::LogprobArgs p = a;
-    p.B = std::min(rows, B - r);
+    p.B = m;
     p.x = static_cast<const char*>(logits) + static_cast<size_t>(r) * ld * vsmp::elem_size(dtype);
     p.ids = n ? ids + static_cast<size_t>(r) * ldj : nullptr;
     p.logprob = n ? logprob + static_cast<size_t>(r) * n : nullptr;
@@ -207,7 +209,7 @@ int vsmp_head_logits_q4(vsmp_ctx* ctx, const void* hidden, int dtype, long long 
   a.D = D;
   a.ldo = ldl;
   const int rows = 1 << 16;  // of one launch
-  for (int r = 0; r < B; r += rows) {
+  for (int r = 0; r < B; r += a.B) {
     a.B = std::min(rows, B - r);
     a.x = static_cast<const uint16_t*>(hidden) + static_cast<size_t>(r) * ldh;
     a.out = logits + static_cast<size_t>(r) * ldl;
