@@ -341,7 +341,7 @@ __global__ __launch_bounds__(kNt) void k_logprobs(LogprobArgs a) {
   if (id < 0 || id >= a.V) id = -1;
   Raw<E, N> d;  // the id's own group
   if (id >= 0) load_group(d, id & ~(N - 1), a.V);
-  float t = INFINITY, tup = INFINITY;
+  float t = NAN, tup = NAN;  // the id's logit and the next float above it; NaN where the lane has no id
   int cnt = 0;  // logits before the lane's id, as far as this wave has counted them
   int own = 0;  // equal ones before it in its own group
   auto take_ids = [&]() {
@@ -409,7 +409,7 @@ __global__ __launch_bounds__(kNt) void k_logprobs(LogprobArgs a) {
       }
       if (n <= kList) {
         todo &= ~high;
-        const float th = t >= few ? t : INFINITY;
+        const float th = t >= few ? t : NAN;  // the other ids gain nothing here, not from a +inf either
         __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
         for (int i = 0; i < n; i += 4) {
           uint2 c[4];
