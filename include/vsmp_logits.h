@@ -71,7 +71,9 @@ VSMP_API int vsmp_adjust_logits(vsmp_ctx* ctx, const void* in, int dtype, long l
  *   logprob[r * n + j] = x_i - lse[r]  and  rank[r * n + j] = how many ids come before i,
  * for i = ids[r * ldj + j], j < n. An id outside [0, V) (a position that is not scored) gets -inf and
  * rank -1. Sums are taken relative to the row's largest logit in fp32. A logit of -inf has probability
- * 0; a row of nothing else has lse -inf and log-probabilities -inf.
+ * 0; a row of nothing else has lse -inf and log-probabilities -inf. A row with a NaN or a +inf has no
+ * probabilities: its lse and the log-probabilities of ids in [0, V) are NaN. Ranks count +inf as the largest
+ * value; a NaN comes before no id, and an id whose logit is NaN has rank 0.
  *   logits, dtype, ld: device logits, row r at element r * ld (ld >= V). V <= 1048576 (2^20).
  *   ids, ldj, n: device int ids, 0 <= n <= 64 (0: lse alone; ids, logprob and rank unused), ldj >= n.
  *   logprob, rank: device [B][n]; rank may be NULL. lse: device float[B], may be NULL (n > 0).

@@ -4,11 +4,12 @@ import pytest
 
 import verbo_amd as V
 from helpers import log, mode_ctx
-from test_logits_ops import dev
+from test_logits_ops import dev, plain_logprobs
 
 pytestmark = pytest.mark.gpu
 
 INF = float("inf")
+NAN = float("nan")
 
 
 @pytest.fixture(scope="module")
@@ -49,3 +50,49 @@ def test_ranks_next_to_infinity(ctx, B, n, dtype):
     log("ranks", B, n, dtype)
     _, rank, _ = ctx.logprobs(xd, dev(ids))
     assert np.array_equal(rank.cpu().numpy(), plain_ranks(xs, ids))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n", [1, 7, 4096, 4099, 60001])
+def test_logprobs_of_rows_with_nan_or_infinity(ctx, n, dtype):
+    """A row with a NaN or a +inf has no probabilities: its lse and its ids' log-probabilities are NaN, wherever the
+    NaN lies and whatever surrounds it (a mask's -inf, nothing but NaN); ids outside the vocabulary are -inf as
+    ever, the other rows of the batch are what they are without it, and NaN comes before no id."""
+    rng = np.random.default_rng(n)
+    at = sorted({0, n // 3, n - 1})
+    rows, bad = [], []
+    for fill in ("finite", "masked", "all"):
+        for i in at:
+            r = rng.normal(0, 3, n).astype(np.float32) if fill == "finite" else np.full(n, -INF if fill == "masked" else NAN, np.float32)
+            r[i] = NAN
+            rows.append(r)
+            bad.append(True)
+            rows.append(rng.normal(0, 3, n).astype(np.float32))
+            bad.append(False)
+    for i in at:
+        r = rng.normal(0, 3, n).astype(np.float32)
+        r[i] = INF
+        rows.append(r)
+        bad.append(True)
+    r = np.full(n, -INF, np.float32)  # what a mask may leave: one allowed token and one NaN
+    r[0], r[n - 1] = 1.0, NAN
+    rows += [r, np.full(n, -INF, np.float32)]
+    bad = np.array(bad + [True, False])
+    xd = dev(np.array(rows), dtype)
+    xs = xd.float().cpu().numpy()
+    ids = np.tile(np.array(at + [n // 2, -1, n], np.int32), (len(rows), 1))
+    inside = (ids >= 0) & (ids < n)
+    log("nan", n, dtype)
+    lp, rank, lse = (t.cpu().numpy() for t in ctx.logprobs(xd, dev(ids)))
+    assert np.isnan(lse[bad]).all() and not np.isnan(lse[~bad]).any()
+    assert np.isnan(lp[bad[:, None] & inside]).all()
+    assert (lp[~inside] == -INF).all() and not np.isnan(lp[~bad]).any()
+    assert np.array_equal(rank, plain_ranks(xs, ids))
+    xs[bad] = 0.0  # the other rows beside ordinary ones
+    again = ctx.logprobs(dev(xs, dtype), dev(ids))
+    for a, b in zip((lp, rank, lse), again):
+        assert np.array_equal(a[~bad], b.cpu().numpy()[~bad])
+    wl, _, wz, tol = plain_logprobs(xs[~bad], ids[~bad])
+    fin = np.isfinite(wz)
+    z = lse[~bad]
+    assert np.array_equal(z[~fin], wz[~fin]) and (np.abs(z[fin] - wz[fin]) <= (tol[fin] + 2.0 ** -24 * np.abs(wz[fin]))).all()

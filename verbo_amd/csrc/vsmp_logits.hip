@@ -235,11 +235,12 @@ constexpr float kLog2e = 1.44269504088896340736f;
 __device__ __forceinline__ float exp_rel(float x, float m) { return __builtin_amdgcn_exp2f((x - m) * kLog2e); }
 
 // A maximum and the sum of exp(x - maximum): the log of the sum of exponentials in one pass. The maximum of
-// nothing is -inf, with a sum of 0.
+// nothing is -inf, with a sum of 0. NaN among the x is left out of the maximum and makes the sum NaN, also where
+// the maximum is -inf; so does a maximum of +inf.
 struct Lse {
   float m, s;
-  // The sum relative to a maximum t >= m.
-  __device__ float at(float t) const { return m == -INFINITY ? 0.0f : s * exp_rel(m, t); }
+  // The sum relative to a maximum t >= m (a sum at m = -inf is 0 or NaN, whatever it is relative to).
+  __device__ float at(float t) const { return m == -INFINITY ? s : s * exp_rel(m, t); }
 };
 __device__ __forceinline__ unsigned long long pack_lse(const Lse& z) {
   return static_cast<unsigned long long>(__float_as_uint(z.m)) << 32 | __float_as_uint(z.s);
@@ -370,15 +371,13 @@ __global__ __launch_bounds__(kNt) void k_logprobs(LogprobArgs a) {
       for (int k = 1; k < N; ++k) gm[g] = fmaxf(gm[g], v[g][k]);
     }
     const float mx = fmaxf(fmaxf(gm[0], gm[1]), fmaxf(gm[2], gm[3]));
-    const float m = fmaxf(z.m, mx);
-    if (m != -INFINITY) {
-      float s = z.s * exp_rel(z.m, m);
+    const float m = fmaxf(z.m, mx), rel = m == -INFINITY ? 0.0f : m;  // of -inf alone: exp(-inf - 0) = 0, and NaN stays
+    float s = z.s * exp_rel(z.m, rel);
 #pragma unroll
-      for (int g = 0; g < G; ++g)
+    for (int g = 0; g < G; ++g)
 #pragma unroll
-        for (int k = 0; k < N; ++k) s += exp_rel(v[g][k], m);
-      z = {m, s};
-    }
+      for (int k = 0; k < N; ++k) s += exp_rel(v[g][k], rel);
+    z = {m, s};
     if (e0 == lo) take_ids();  // after the first step's sums: the ids' logits were loaded behind it
     if (!a.rank) continue;
     float rm = mx;  // the largest of each row of 16 lanes
@@ -499,13 +498,13 @@ __global__ __launch_bounds__(kNt) void k_logprobs(LogprobArgs a) {
     }
     z = wave_lse(z);
   }
-  const float ls = logf(z.s);  // of a sum in [1, V]
+  const float ls = logf(z.s);  // of a sum in [1, V]; -inf for a row of -inf alone; NaN
   if (lane < a.n) {
     const long long o = static_cast<long long>(row) * a.n + lane;
-    a.logprob[o] = id >= 0 && t != -INFINITY ? (t - z.m) - ls : -INFINITY;
+    a.logprob[o] = id < 0 ? -INFINITY : (z.m == -INFINITY ? ls : (t - z.m) - ls);
     if (a.rank) a.rank[o] = id >= 0 ? cnt + own : -1;
   }
-  if (lane == 0 && a.lse) a.lse[row] = z.m == -INFINITY ? -INFINITY : z.m + ls;
+  if (lane == 0 && a.lse) a.lse[row] = z.m + ls;
 }
 
 }  // namespace
