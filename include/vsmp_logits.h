@@ -107,8 +107,10 @@ VSMP_API int vsmp_head_logits_q4(vsmp_ctx* ctx, const void* hidden, int dtype, l
  * vsmp_bsampler_pick_rows: row i of the call belongs to slot rows[i] (device array of n_rows distinct
  * slots; NULL: row i is slot i, n_rows = the sampler's slots) and is penalised by that slot's history
  * on the device. The rest is vsmp_adjust_logits's with B = n_rows, per-row arrays by row of the call.
- * n_rows = 0 does nothing. A slot keeps at least its last repeat_last ids (all of them with
- * repeat_last <= 0), so pen.window should be at most that. Returns 0 or -1. */
+ * Where the slot's repeat_last is above 0 its window is at most that: a pen.window of 0 or less, or of
+ * more, counts repeat_last ids, whatever the slot happens to keep beyond them. prompt_len counts from the
+ * first id that the sequence accepted (its prompt's, with vsmp_bsampler_admit), also after the slot has
+ * dropped it. n_rows = 0 does nothing. Returns 0 or -1. */
 VSMP_API int vsmp_bsampler_adjust_rows(vsmp_bsampler* s, const void* in, int dtype, long long ldi, int V,
                                        const int* rows, int n_rows, const vsmp_penalty* pen, int pen_per_row,
                                        const int* prompt_len, const int* bias_ids, const float* bias,

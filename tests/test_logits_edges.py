@@ -4,7 +4,8 @@ import pytest
 
 import verbo_amd as V
 from helpers import log, mode_ctx
-from test_logits_ops import dev, plain_logprobs
+from test_logits_ops import check_adjusted, dev, plain_adjust, plain_logprobs
+from verbo_amd import decode
 
 pytestmark = pytest.mark.gpu
 
@@ -96,3 +97,102 @@ def test_logprobs_of_rows_with_nan_or_infinity(ctx, n, dtype):
     fin = np.isfinite(wz)
     z = lse[~bad]
     assert np.array_equal(z[~fin], wz[~fin]) and (np.abs(z[fin] - wz[fin]) <= (tol[fin] + 2.0 ** -24 * np.abs(wz[fin]))).all()
+
+
+# ---- slots whose histories were trimmed ------------------------------------------------------------------
+
+
+class Slots:
+    """A decoder of slots beside its sequences' whole histories on the host."""
+
+    def __init__(self, windows, n, cap=4096):
+        self.n, self.said, self.windows = n, {}, dict(enumerate(windows))
+        self.d = decode.BatchDecoder.with_slots(len(windows), n, cap=cap)
+
+    def admit(self, slot, window, prompt):
+        import torch
+
+        self.windows[slot] = window
+        self.said[slot] = [int(i) for i in prompt]
+        self.d.admit(slot, V.Params(temp=0.0, repeat=1.0, repeat_last=window), prompt, torch.cuda.current_stream())
+
+    def accept(self, live, ids):
+        import torch
+
+        self.d.accept_rows(dev(np.array(ids, np.int32)), dev(np.array(live, np.int32)), torch.ones(len(live), dtype=torch.int32, device="cuda"),
+                           torch.cuda.current_stream())
+        for s, t in zip(live, ids):
+            self.said[s].append(int(t))
+
+    def check(self, live, pens, prompts, rng):
+        """Rows of the live slots against the whole histories' last window ids: the penalty's own window, at most the
+        slot's repeat_last where that is above 0."""
+        import torch
+
+        x = rng.normal(0, 2, (len(live), self.n)).astype(np.float32)
+        left = torch.empty(len(live), dtype=torch.int32, device="cuda")
+        y = self.d.adjust_rows(dev(x), dev(np.array(live, np.int32)), V.to_device_penalties(pens),
+                               prompt_len=dev(np.array(prompts, np.int32)) if prompts is not None else None, left=left)
+        counted = []
+        for s, p in zip(live, pens):
+            w = self.windows[s]
+            w = p.window if w <= 0 else w if p.window <= 0 else min(w, p.window)
+            counted.append(V.Penalty(p.repeat, p.presence, p.frequency, w))
+        want, tol = plain_adjust(x, counted, [self.said[s] for s in live], prompts)
+        check_adjusted(y, left, want, tol)
+
+
+def test_slots_windows_and_prompts_outlive_the_trims():
+    """Histories that are cut from four windows to one again and again: what is penalised is always the last window
+    ids, presence and frequency leave out the prompt however many of its ids are gone, and a slot's next sequence
+    begins anew. Prompts shorter and longer than what a slot keeps; ids accepted on the device and from the host."""
+    n = 40
+    rng = np.random.default_rng(1)
+    windows = [3, 5, 0, 2, 7]
+    st = Slots(windows, n)
+    lens = [4, 47, 30, 9, 0]
+    for s, (w, k) in enumerate(zip(windows, lens)):
+        st.admit(s, w, rng.integers(0, n, k).astype(np.int32))
+    prompts = lens
+    for step in range(70):
+        live = [int(s) for s in rng.permutation(len(windows))[:rng.integers(1, len(windows) + 1)]]
+        if step == 40:  # a new sequence in a slot that was trimmed before
+            st.admit(0, 4, rng.integers(0, n, 6).astype(np.int32))
+            prompts = [6] + lens[1:]
+        if step == 50:  # ids from the host, past a trim
+            ids = rng.integers(0, n, 23).astype(np.int32)
+            st.d.accept_prompt(3, ids)
+            st.said[3] += [int(i) for i in ids]
+        pens = [V.Penalty(1.0 + 0.1 * s, 0.5, 0.25, int(rng.choice([0, -3, 1, 2, 4, 1000]))) for s in live]
+        log("slots", step, live)
+        st.check(live, pens, [prompts[s] for s in live], rng)
+        st.check(live, pens, None, rng)
+        st.accept(live, rng.integers(0, n, len(live)))
+
+
+def test_slots_windows_in_a_replayed_graph():
+    """A captured adjustment reads the slots as they are at each replay: after trims, and after a new sequence."""
+    import torch
+
+    n = 30
+    rng = np.random.default_rng(2)
+    st = Slots([2, 3], n)
+    st.admit(0, 2, np.array([1, 2, 3], np.int32))
+    st.admit(1, 3, np.array([4], np.int32))
+    x = rng.normal(0, 2, (2, n)).astype(np.float32)
+    xd, rows, prompt = dev(x), dev(np.array([1, 0], np.int32)), dev(np.array([1, 3], np.int32))
+    pens = [V.Penalty(1.5, 1.0, 0.5, 0), V.Penalty(1.0, 2.0, 0.25, 0)]
+    pd, out = V.to_device_penalties(pens), torch.empty(2, n, device="cuda")
+    left = torch.empty(2, dtype=torch.int32, device="cuda")
+    st.d.adjust_rows(xd, rows, pd, prompt_len=prompt, out=out, left=left)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=torch.cuda.Stream()):
+        st.d.adjust_rows(xd, rows, pd, prompt_len=prompt, out=out, left=left)
+    for step in range(30):
+        if step == 17:
+            st.admit(1, 3, np.array([7], np.int32))
+        g.replay()
+        counted = [V.Penalty(1.5, 1.0, 0.5, 3), V.Penalty(1.0, 2.0, 0.25, 2)]
+        check_adjusted(out, left, *plain_adjust(x, counted, [st.said[1], st.said[0]], [1, 3]))
+        st.accept([0, 1], rng.integers(0, n, 2))

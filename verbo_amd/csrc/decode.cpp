@@ -179,7 +179,7 @@ int vsmp_dsampler_accept(vsmp_dsampler* s, const int* ids, int n, void* stream) 
   for (int i = 0; i < n; ++i) {
     if (rl <= 0 && !ds_reserve(s, s->h + 1, st)) return -1;
     vsmp::launch_hist_accept(s->hist, s->meta, s->meta + 1, s->cap, nullptr, s->cfg, nullptr, ids[i], nullptr, nullptr, 1,
-                             nullptr, st);
+                             nullptr, nullptr, st);
     if (!hip_ok(hipGetLastError(), "accept launch")) return -1;
     s->h = accepted_length(s->h, 1, rl);
   }
@@ -220,6 +220,7 @@ struct vsmp_bsampler {
   int* hist = nullptr;               // device [n][cap]
   int* off = nullptr;                // device [n]: r * cap
   int* len = nullptr;                // device [n]
+  int* gone = nullptr;               // device [n]: ids that trims dropped from a sequence's history so far
   int* full = nullptr;               // device flag
   int* host = nullptr;               // pinned staging: the flag read back
 };
@@ -266,7 +267,8 @@ vsmp_bsampler* vsmp_bsampler_new(int device, int n, const vsmp_params* params, i
   void* host = nullptr;
   bool ok = dev_alloc(s->params, static_cast<size_t>(n), "parameters") && dev_alloc(s->rng, 2 * static_cast<size_t>(n), "draw streams") &&
             dev_alloc(s->hist, static_cast<size_t>(n) * cap, "history windows") && dev_alloc(s->off, static_cast<size_t>(n), "offsets") &&
-            dev_alloc(s->len, static_cast<size_t>(n), "lengths") && dev_alloc(s->full, 1, "flag") &&
+            dev_alloc(s->len, static_cast<size_t>(n), "lengths") && dev_alloc(s->gone, static_cast<size_t>(n), "trimmed ids") &&
+            dev_alloc(s->full, 1, "flag") &&
             hip_ok(hipHostMalloc(&host, sizeof(int), hipHostMallocDefault), "pinned staging");
   s->host = static_cast<int*>(host);
   ok = ok &&
@@ -274,6 +276,7 @@ vsmp_bsampler* vsmp_bsampler_new(int device, int n, const vsmp_params* params, i
        hip_ok(hipMemcpy(s->rng, st.data(), sizeof(std::uint64_t) * st.size(), hipMemcpyHostToDevice), "copy draw streams") &&
        hip_ok(hipMemcpy(s->off, off.data(), sizeof(int) * off.size(), hipMemcpyHostToDevice), "copy offsets") &&
        hip_ok(hipMemset(s->len, 0, sizeof(int) * static_cast<size_t>(n)), "clear lengths") &&
+       hip_ok(hipMemset(s->gone, 0, sizeof(int) * static_cast<size_t>(n)), "clear trimmed ids") &&
        hip_ok(hipMemset(s->full, 0, sizeof(int)), "clear flag") && hip_ok(hipDeviceSynchronize(), "synchronise");
   if (!ok) {
     vsmp_bsampler_free(s);
@@ -287,7 +290,7 @@ void vsmp_bsampler_free(vsmp_bsampler* s) {
   if (s->ctx) vsmp_ctx_free(s->ctx);
   vsmp::DeviceScope scope(s->device);
   for (void* p : {static_cast<void*>(s->params), static_cast<void*>(s->rng), static_cast<void*>(s->hist),
-                  static_cast<void*>(s->off), static_cast<void*>(s->len), static_cast<void*>(s->full)})
+                  static_cast<void*>(s->off), static_cast<void*>(s->len), static_cast<void*>(s->gone), static_cast<void*>(s->full)})
     if (p) (void)hipFree(p);
   if (s->host) (void)hipHostFree(s->host);
   delete s;
@@ -301,9 +304,10 @@ int vsmp_bsampler_accept_host(vsmp_bsampler* s, int row, const int* ids, int m) 
   if (!scope.ok() || !hip_ok(hipDeviceSynchronize(), "synchronise")) return -1;
   // the row's parameters and current length, from the device (prompts are accepted before decoding)
   vsmp_params p{};
-  int h = 0;
+  int h = 0, gone = 0;
   if (!hip_ok(hipMemcpy(&p, s->params + row, sizeof p, hipMemcpyDeviceToHost), "read parameters") ||
-      !hip_ok(hipMemcpy(&h, s->len + row, sizeof h, hipMemcpyDeviceToHost), "read length"))
+      !hip_ok(hipMemcpy(&h, s->len + row, sizeof h, hipMemcpyDeviceToHost), "read length") ||
+      !hip_ok(hipMemcpy(&gone, s->gone + row, sizeof gone, hipMemcpyDeviceToHost), "read trimmed ids"))
     return -1;
   const int len = accepted_length(h, m, p.repeat_last);
   int* region = s->hist + static_cast<size_t>(row) * s->cap;
@@ -320,7 +324,11 @@ int vsmp_bsampler_accept_host(vsmp_bsampler* s, int row, const int* ids, int m) 
     std::copy(ids, ids + m, w.begin() + (len - m));
     if (!hip_ok(hipMemcpy(region, w.data(), sizeof(int) * w.size(), hipMemcpyHostToDevice), "copy window")) return -1;
   }
-  return hip_ok(hipMemcpy(s->len + row, &len, sizeof len, hipMemcpyHostToDevice), "copy length") ? 0 : -1;
+  gone += h + m - len;
+  return hip_ok(hipMemcpy(s->gone + row, &gone, sizeof gone, hipMemcpyHostToDevice), "copy trimmed ids") &&
+                 hip_ok(hipMemcpy(s->len + row, &len, sizeof len, hipMemcpyHostToDevice), "copy length")
+             ? 0
+             : -1;
 }
 
 int vsmp_bsampler_pick(vsmp_bsampler* s, const float* logits, int V, long long ld, int* out, void* stream) {
@@ -338,7 +346,7 @@ int vsmp_bsampler_accept(vsmp_bsampler* s, const int* ids, const int* active, vo
   vsmp::DeviceScope scope(s->device);
   if (!scope.ok()) return -1;
   vsmp::launch_hist_accept(s->hist, s->off, s->len, s->cap, s->params, vsmp_params{}, ids, 0, active, nullptr, s->n,
-                           s->full, static_cast<hipStream_t>(stream));
+                           s->full, s->gone, static_cast<hipStream_t>(stream));
   return hip_ok(hipGetLastError(), "accept launch") ? 0 : -1;
 }
 
@@ -365,7 +373,7 @@ int vsmp_bsampler_admit(vsmp_bsampler* s, int slot, const vsmp_params* params, c
                                         sizeof(int) * static_cast<size_t>(len), hipMemcpyHostToDevice, st),
                          "copy prompt ids"))
     return -1;
-  vsmp::launch_slot_admit(s->params, s->rng, s->len, slot, p, rs[0], rs[1], len, st);
+  vsmp::launch_slot_admit(s->params, s->rng, s->len, s->gone, slot, p, rs[0], rs[1], len, m - len, st);
   return hip_ok(hipGetLastError(), "admit launch") ? 0 : -1;
 }
 
@@ -391,7 +399,7 @@ int vsmp_bsampler_accept_rows(vsmp_bsampler* s, const int* ids, const int* rows,
   vsmp::DeviceScope scope(s->device);
   if (!scope.ok()) return -1;
   vsmp::launch_hist_accept(s->hist, s->off, s->len, s->cap, s->params, vsmp_params{}, ids, 0, active, rows, n_rows,
-                           s->full, static_cast<hipStream_t>(stream));
+                           s->full, s->gone, static_cast<hipStream_t>(stream));
   return hip_ok(hipGetLastError(), "accept launch") ? 0 : -1;
 }
 
@@ -413,6 +421,8 @@ int vsmp_bsampler_adjust_rows(vsmp_bsampler* s, const void* in, int dtype, long 
   a.hist = s->hist;
   a.hist_off = s->off;
   a.hist_len = s->len;
+  a.gone = s->gone;
+  a.seq_params = s->params;
   a.slot = rows;
   a.prompt_len = prompt_len;
   a.bias_ids = bias_ids;

@@ -186,13 +186,14 @@ void launch_head_finish(const KArgs& a, const HeadArgs& h, hipStream_t st);
 // (active[i]; active null: every entry), the id ids[i] (ids null: `tok`) is appended to row
 // slots[i] (slots null: row i); with repeat_last > 0 a history that would exceed 4 * repeat_last
 // keeps its last repeat_last ids, as the reference trims. A row whose region is full
-// (repeat_last <= 0) appends nothing and sets *full (when not null).
+// (repeat_last <= 0) appends nothing and sets *full (when not null). gone (when not null): gone[r] grows by the
+// ids that a trim drops from the front of row r's history.
 void launch_hist_accept(int* hist, const int* off, int* len, int cap, const vsmp_params* params,
                         const vsmp_params& shared, const int* ids, int tok, const int* active, const int* slots, int n,
-                        int* full, hipStream_t st);
-// A batched decoder's slot given to a new sequence: params[slot] = p, its xorshift state {s0, s1}
-// and history length h, on `st`.
-void launch_slot_admit(vsmp_params* params, unsigned long long* rng, int* len, int slot, const vsmp_params& p,
-                       unsigned long long s0, unsigned long long s1, int h, hipStream_t st);
+                        int* full, int* gone, hipStream_t st);
+// A batched decoder's slot given to a new sequence: params[slot] = p, its xorshift state {s0, s1},
+// history length h and ids already gone from its history's front, on `st`.
+void launch_slot_admit(vsmp_params* params, unsigned long long* rng, int* len, int* gone, int slot, const vsmp_params& p,
+                       unsigned long long s0, unsigned long long s1, int h, int dropped, hipStream_t st);
 
 }  // namespace vsmp

@@ -4908,7 +4908,7 @@ __global__ __launch_bounds__(256) void k_read_probe(const uint4* __restrict__ p,
 __global__ __launch_bounds__(256) void k_hist_accept(int* __restrict__ hist, const int* __restrict__ off,
                                                      int* __restrict__ len, int cap, const vsmp_params* params,
                                                      vsmp_params shared, const int* ids, int tok,
-                                                     const int* active, const int* slots, int n, int* full) {
+                                                     const int* active, const int* slots, int n, int* full, int* gone) {
   const int i = static_cast<int>(blockIdx.x) * 256 + static_cast<int>(threadIdx.x);
   if (i >= n || (active && !active[i])) return;
   const int r = slots ? slots[i] : i;  // the sequence entry i appends to
@@ -4921,6 +4921,7 @@ __global__ __launch_bounds__(256) void k_hist_accept(int* __restrict__ hist, con
     for (int i = 0; i < keep - 1; ++i) h[i] = h[s + 1 - keep + i];
     h[keep - 1] = t;
     len[r] = keep;
+    if (gone) gone[r] += s + 1 - keep;
   } else if (s < cap) {
     h[s] = t;
     len[r] = s + 1;
@@ -5317,27 +5318,29 @@ void launch_exp_probe(const double* x, double* y, long long n, hipStream_t st) {
 
 void launch_hist_accept(int* hist, const int* off, int* len, int cap, const vsmp_params* params,
                         const vsmp_params& shared, const int* ids, int tok, const int* active, const int* slots, int n,
-                        int* full, hipStream_t st) {
+                        int* full, int* gone, hipStream_t st) {
   hipLaunchKernelGGL(k_hist_accept, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, st, hist, off, len, cap,
-                     params, shared, ids, tok, active, slots, n, full);
+                     params, shared, ids, tok, active, slots, n, full, gone);
 }
 
 // A batched decoder's slot taken by a new sequence (stream-ordered with its picks and accepts): the
-// sequence's parameters, its draw stream's state (seeded on the host) and its history length (the
-// ids themselves are copied before this kernel, on the same stream).
+// sequence's parameters, its draw stream's state (seeded on the host), its history length (the
+// ids themselves are copied before this kernel, on the same stream) and how many ids the history
+// has lost at its front.
 __global__ void k_slot_admit(vsmp_params* __restrict__ params, unsigned long long* __restrict__ rng,
-                             int* __restrict__ len, int slot, vsmp_params p, unsigned long long s0,
-                             unsigned long long s1, int h) {
+                             int* __restrict__ len, int* __restrict__ gone, int slot, vsmp_params p,
+                             unsigned long long s0, unsigned long long s1, int h, int dropped) {
   if (threadIdx.x != 0) return;
   params[slot] = p;
   rng[2 * static_cast<size_t>(slot)] = s0;
   rng[2 * static_cast<size_t>(slot) + 1] = s1;
   len[slot] = h;
+  gone[slot] = dropped;
 }
 
-void launch_slot_admit(vsmp_params* params, unsigned long long* rng, int* len, int slot, const vsmp_params& p,
-                       unsigned long long s0, unsigned long long s1, int h, hipStream_t st) {
-  hipLaunchKernelGGL(k_slot_admit, dim3(1), dim3(64), 0, st, params, rng, len, slot, p, s0, s1, h);
+void launch_slot_admit(vsmp_params* params, unsigned long long* rng, int* len, int* gone, int slot, const vsmp_params& p,
+                       unsigned long long s0, unsigned long long s1, int h, int dropped, hipStream_t st) {
+  hipLaunchKernelGGL(k_slot_admit, dim3(1), dim3(64), 0, st, params, rng, len, gone, slot, p, s0, s1, h, dropped);
 }
 
 void launch_zero_u32(uint32_t* p, long long n, hipStream_t st) {

@@ -115,8 +115,14 @@ __global__ __launch_bounds__(kNt) void k_adjust(AdjustArgs a) {
     const int seq = a.slot ? a.slot[row] : row;
     h0 = a.hist_off[seq];
     h1 = a.hist_len ? h0 + a.hist_len[seq] : a.hist_off[seq + 1];
-    hp = a.prompt_len ? h0 + min(max(a.prompt_len[row], 0), max(h1 - h0, 0)) : h0;
-    if (pen.window > 0 && h1 - h0 > pen.window) h0 = h1 - pen.window;
+    int window = pen.window;
+    if (a.hist_len) {  // what a sequence's region holds beyond its repeat_last depends on when it was cut last
+      const int most = a.seq_params[seq].repeat_last;
+      if (most > 0 && (window <= 0 || window > most)) window = most;
+    }
+    hp = h0;
+    if (a.prompt_len) hp += min(max(max(a.prompt_len[row], 0) - (a.hist_len ? a.gone[seq] : 0), 0), max(h1 - h0, 0));
+    if (window > 0 && h1 - h0 > window) h0 = h1 - window;
   }
   int b0 = 0, b1 = 0;
   if (BIAS) {

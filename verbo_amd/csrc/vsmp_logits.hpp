@@ -39,6 +39,8 @@ struct AdjustArgs {
   const int* hist;           // null: no history
   const int* hist_off;
   const int* hist_len;       // null: row r's history ends at hist_off[r + 1]; else after hist_len[r] ids
+  const int* gone;           // with hist_len: ids that a sequence's history has lost at its front
+  const vsmp_params* seq_params;  // with hist_len: a sequence's parameters (repeat_last above 0 bounds its window)
   const int* slot;           // null, or the sequence whose history row r has
   const int* prompt_len;
   const int* bias_ids;

@@ -79,7 +79,11 @@ int adjust_logits(vsmp_ctx* ctx, AdjustArgs a, int dtype, bool pen_per_row, cons
     if (a.slot) p.slot = a.slot + r;
     else if (a.hist_off) {
       p.hist_off = a.hist_off + r;
-      if (a.hist_len) p.hist_len = a.hist_len + r;
+      if (a.hist_len) {
+        p.hist_len = a.hist_len + r;
+        p.gone = a.gone + r;
+        p.seq_params = a.seq_params + r;
+      }
     }
     if (a.prompt_len) p.prompt_len = a.prompt_len + r;
     if (a.bias_off) p.bias_off = a.bias_off + r;

@@ -195,8 +195,9 @@ class BatchDecoder:
     def adjust_rows(self, logits, rows, penalty=None, prompt_len=None, bias_ids=None, bias=None, bias_off=None, mask=None,
                     mask_row=None, out=None, left=None, stream=None):
         """Context.adjust_logits for the live slots rows[i] (device int32, distinct), before pick_rows: row i is
-        penalised by slot rows[i]'s history. Per-row arrays go by row of the call; prompt_len counts from the first
-        id that the slot still keeps. Returns the adjusted logits (`out`)."""
+        penalised by slot rows[i]'s history. Per-row arrays go by row of the call. A window is at most the slot's
+        repeat_last where that is above 0 (and that for a window of 0); prompt_len counts from the sequence's first
+        id, also after the slot has dropped it. Returns the adjusted logits (`out`)."""
         dev = logits.device
         if dev.type != "cuda" or dev.index != self.device or tuple(logits.shape) != (rows.numel(), self.vocab):
             raise VsmpError("logits must be a [len(rows), V] tensor on the decoder's device")
