@@ -196,3 +196,32 @@ def test_slots_windows_in_a_replayed_graph():
         counted = [V.Penalty(1.5, 1.0, 0.5, 3), V.Penalty(1.0, 2.0, 0.25, 2)]
         check_adjusted(out, left, *plain_adjust(x, counted, [st.said[1], st.said[0]], [1, 3]))
         st.accept([0, 1], rng.integers(0, n, 2))
+
+
+def test_serve_leaves_the_prompt_out():
+    """Requests whose presence and frequency penalties leave their prompts out, and ones whose penalties count them,
+    over windows that are cut several times: greedy picks over constant logits, by the rules alone."""
+    import torch
+
+    n = 24
+    base = np.linspace(6.0, 0.0, n).astype(np.float32)
+    cases = [  # prompt, window, penalty, prompt_len, ids to generate, arrival
+        ([0, 1, 2, 3, 0, 1], 3, V.Penalty(presence=1.0, frequency=0.75), 6, 40, 0),
+        ([0, 1, 2, 3, 0, 1], 3, V.Penalty(presence=1.0, frequency=0.75), 0, 40, 0),
+        ([5, 0, 0], 4, V.Penalty(frequency=0.5), 3, 30, 2),
+        ([5, 0, 0, 7], 4, V.Penalty(repeat=1.5, frequency=0.5, window=2), 2, 30, 3),
+        (list(range(20)), 2, V.Penalty(presence=3.0), 20, 25, 4),
+        ([0, 1, 2], 0, V.Penalty(presence=2.0), 3, 20, 5),
+    ]
+    reqs = [decode.Request(p, decode.Opts(max_tokens=m, temp=0.0), repeat_last=w, arrival=at, penalty=pen, prompt_len=k)
+            for p, w, pen, k, m, at in cases]
+    d = decode.BatchDecoder.with_slots(3, n)
+    res = d.serve(reqs, lambda js, steps, last: torch.from_numpy(np.tile(base, (len(js), 1))).cuda())
+    for (prompt, w, pen, k, m, _), (toks, _) in zip(cases, res):
+        said = list(prompt)
+        win = pen.window if w <= 0 else w if pen.window <= 0 else min(w, pen.window)
+        for _ in range(m):
+            y, _ = plain_adjust(base[None], [V.Penalty(pen.repeat, pen.presence, pen.frequency, win)], [said], [k])
+            said.append(int(y[0].argmax()))
+        assert toks == said[len(prompt):], (prompt, w, k)
+    assert res[0][0] != res[1][0]

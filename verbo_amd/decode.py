@@ -52,15 +52,19 @@ class Opts(ctypes.Structure):
 class Request:
     """One generation request of a serving loop: the prompt's ids, its options (Opts), the window
     of its repetition penalty and the step at which it arrives. penalty: None, or a Penalty taken from its
-    logits before each pick, over the ids its slot keeps (the last repeat_last ones at least, the prompt's among
-    them)."""
+    logits before each pick, over the last ids of the prompt and the answer: penalty.window of them, at most
+    repeat_last (each: all, where it is 0 or less). prompt_len: how many ids at the prompt's start count for the
+    penalty's `repeat` alone, not for presence and frequency (len(prompt) leaves the prompt out of those)."""
 
-    def __init__(self, prompt, opts, repeat_last=64, arrival=0, penalty=None):
+    def __init__(self, prompt, opts, repeat_last=64, arrival=0, penalty=None, prompt_len=0):
         self.prompt = np.ascontiguousarray(prompt, dtype=np.int32)
         self.opts = opts
         self.repeat_last = int(repeat_last)
         self.arrival = int(arrival)
         self.penalty = penalty
+        self.prompt_len = int(prompt_len)
+        if not 0 <= self.prompt_len <= self.prompt.size:
+            raise VsmpError("need 0 <= prompt_len <= the prompt's ids")
 
 
 def params_of(o, repeat_last=64):
@@ -260,7 +264,9 @@ class BatchDecoder:
             lg = logits_fn(reqs, [steps[j] for j in reqs], [last[j] for j in reqs])
             pens = [requests[j].penalty for j in reqs]
             if any(p is not None for p in pens):
-                lg = self.adjust_rows(lg, rows, to_device_penalties([p or Penalty() for p in pens], dev), stream=stream)
+                own = torch.tensor([requests[j].prompt_len for j in reqs], dtype=torch.int32, device=dev)
+                lg = self.adjust_rows(lg, rows, to_device_penalties([p or Penalty() for p in pens], dev), prompt_len=own,
+                                      stream=stream)
             self.pick_rows(lg, rows, out[:len(slots)], stream)
             self.schedule.append(list(zip(reqs, slots)))
             ids = out[:len(slots)].cpu().numpy()  # the only per-step copy to the host: one id per live slot
