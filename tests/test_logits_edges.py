@@ -225,3 +225,20 @@ def test_serve_leaves_the_prompt_out():
             said.append(int(y[0].argmax()))
         assert toks == said[len(prompt):], (prompt, w, k)
     assert res[0][0] != res[1][0]
+
+
+def test_serve_uploads_penalties_when_the_live_requests_change(monkeypatch):
+    """Penalties go to the device once for as long as the same requests are live in the same slots."""
+    import torch
+
+    n, calls = 12, []
+    upload = decode.to_device_penalties
+    monkeypatch.setattr(decode, "to_device_penalties", lambda p, dev: calls.append(len(p)) or upload(p, dev))
+    reqs = [decode.Request([0], decode.Opts(max_tokens=m, temp=0.0), repeat_last=0, arrival=at, penalty=V.Penalty(presence=9.0))
+            for m, at in ((9, 0), (4, 2), (6, 3))]
+    d = decode.BatchDecoder.with_slots(2, n)
+    base = torch.linspace(3.0, 0.0, n, device="cuda")
+    res = d.serve(reqs, lambda js, steps, last: base.expand(len(js), n).contiguous())
+    assert [t for t, _ in res] == [list(range(1, m + 1)) for m in (9, 4, 6)]
+    # request 0 alone, with 1 until its slot is free, with 2, 2 alone
+    assert calls == [1, 2, 2, 1]

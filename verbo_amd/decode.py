@@ -244,6 +244,7 @@ class BatchDecoder:
         stopped = [False] * len(requests)
         steps = [0] * len(requests)
         last = [-1] * len(requests)
+        held, pens, own = None, None, None  # the requests whose penalties and prompt lengths are on the device
         self.schedule = []
         step = 0
         while queue or live:
@@ -262,11 +263,12 @@ class BatchDecoder:
             reqs = [live[s] for s in slots]
             rows = torch.tensor(slots, dtype=torch.int32, device=dev)
             lg = logits_fn(reqs, [steps[j] for j in reqs], [last[j] for j in reqs])
-            pens = [requests[j].penalty for j in reqs]
-            if any(p is not None for p in pens):
-                own = torch.tensor([requests[j].prompt_len for j in reqs], dtype=torch.int32, device=dev)
-                lg = self.adjust_rows(lg, rows, to_device_penalties([p or Penalty() for p in pens], dev), prompt_len=own,
-                                      stream=stream)
+            if any(requests[j].penalty is not None for j in reqs):
+                if reqs != held:
+                    pens = to_device_penalties([requests[j].penalty or Penalty() for j in reqs], dev)
+                    own = torch.tensor([requests[j].prompt_len for j in reqs], dtype=torch.int32, device=dev)
+                    held = reqs
+                lg = self.adjust_rows(lg, rows, pens, prompt_len=own, stream=stream)
             self.pick_rows(lg, rows, out[:len(slots)], stream)
             self.schedule.append(list(zip(reqs, slots)))
             ids = out[:len(slots)].cpu().numpy()  # the only per-step copy to the host: one id per live slot
