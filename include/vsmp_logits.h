@@ -77,8 +77,8 @@ VSMP_API int vsmp_adjust_logits(vsmp_ctx* ctx, const void* in, int dtype, long l
  *   logits, dtype, ld: device logits, row r at element r * ld (ld >= V). V <= 1048576 (2^20).
  *   ids, ldj, n: device int ids, 0 <= n <= 64 (0: lse alone; ids, logprob and rank unused), ldj >= n.
  *   logprob, rank: device [B][n]; rank may be NULL. lse: device float[B], may be NULL (n > 0).
- * The context holds about 2 MB of scratch from the first call on; a call that is captured into a
- * graph needs one before it. Returns 0 or -1. */
+ * The context holds about 2 MB of scratch from the first call on, of whatever shape; a call that is
+ * captured into a graph needs one before it. Returns 0 or -1. */
 VSMP_API int vsmp_logprobs(vsmp_ctx* ctx, const void* logits, int dtype, long long ld, int B, int V, const int* ids,
                            long long ldj, int n, float* logprob, int* rank, float* lse, void* stream);
 

@@ -56,6 +56,7 @@ bool ops_scratch(vsmp_ctx*, hipStream_t, OpScratch* out) {
   *out = OpScratch{};
   return true;
 }
+bool ops_warm(vsmp_ctx*, hipStream_t) { return true; }
 
 void launch_adjust(const AdjustArgs& a, int, hipStream_t) {
   at(static_cast<const char*>(a.in), kIn, 2);

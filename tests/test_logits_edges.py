@@ -242,3 +242,26 @@ def test_serve_uploads_penalties_when_the_live_requests_change(monkeypatch):
     assert [t for t, _ in res] == [list(range(1, m + 1)) for m in (9, 4, 6)]
     # request 0 alone, with 1 until its slot is free, with 2, 2 alone
     assert calls == [1, 2, 2, 1]
+
+
+# ---- scratch, arguments, streams -----------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("warm", [(2, 500), (2000, 20000)])
+def test_any_first_call_holds_the_scratch(warm):
+    """After one call of vsmp_logprobs, whether it cut its rows into parts or not, calls of every shape are captured."""
+    import torch
+
+    fresh = V.Context(0)
+    fresh.logprobs(torch.randn(*warm, device="cuda"), torch.zeros(warm[0], 1, dtype=torch.int32, device="cuda"))
+    x, ids = torch.randn(2, 50000, device="cuda"), torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=torch.cuda.Stream()):
+        got = fresh.logprobs(x, ids)
+    for _ in range(3):
+        x.normal_()
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, fresh.logprobs(x, ids)):
+            assert torch.equal(a, b)

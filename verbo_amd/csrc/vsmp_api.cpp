@@ -900,6 +900,11 @@ bool ops_scratch(vsmp_ctx* c, hipStream_t st, OpScratch* out) {
   return true;
 }
 
+bool ops_warm(vsmp_ctx* c, hipStream_t st) {
+  OpScratch s{};
+  return c->o_scr || capturing(st) || ops_scratch(c, st, &s);
+}
+
 // A stream passed with a context must belong to the context's device (its scratch lives there).
 bool stream_on_device(const vsmp_ctx* c, hipStream_t st) {
   if (!c || !st) return true;  // a null context is rejected by the call; the null stream is the device's own

@@ -60,6 +60,9 @@ int pick_batch(vsmp_ctx* ctx, const float* logits, int B, int V, long long ld, c
 // be, or when `st` is capturing and it is not there yet.
 struct OpScratch;
 bool ops_scratch(vsmp_ctx* c, hipStream_t st, OpScratch* out);
+// true when the context has that scratch, or got it here; a capturing `st` leaves things as they are. For calls that
+// need none themselves but are promised to bring it. false (error set) when it could not be allocated.
+bool ops_warm(vsmp_ctx* c, hipStream_t st);
 
 // vsmp_adjust_logits's argument checks, and its work for arguments that pass them: rows with histories of
 // their own (hist_off with B + 1 entries) or, with hist_len, with sequences' regions (see pick_batch).

@@ -165,7 +165,7 @@ int vsmp_logprobs(vsmp_ctx* ctx, const void* logits, int dtype, long long ld, in
     p.rank = n && rank ? rank + static_cast<size_t>(r) * n : nullptr;
     p.lse = lse ? lse + r : nullptr;
     vsmp::logprob_parts(p.B, V, dtype, vsmp::ctx_cus(ctx), &p.P, &p.L);
-    if (p.P > 1 && !vsmp::ops_scratch(ctx, st, &p.s)) return -1;
+    if (!(p.P > 1 ? vsmp::ops_scratch(ctx, st, &p.s) : vsmp::ops_warm(ctx, st))) return -1;
     vsmp::launch_logprobs(p, dtype, st);
     if (!vsmp::hip_ok(hipGetLastError(), "logprobs launch")) return -1;
   }
