@@ -265,3 +265,14 @@ def test_any_first_call_holds_the_scratch(warm):
         torch.cuda.synchronize()
         for a, b in zip(got, fresh.logprobs(x, ids)):
             assert torch.equal(a, b)
+
+
+def test_an_empty_mask_table_is_refused(ctx):
+    """A table without masks is no way to say that rows are not masked."""
+    import torch
+
+    x = torch.zeros(2, 64, device="cuda")
+    none = torch.zeros(0, 2, dtype=torch.int32, device="cuda")
+    for kw in (dict(), dict(mask_row=torch.zeros(2, dtype=torch.int32, device="cuda"))):
+        with pytest.raises(V.VsmpError, match="mask"):
+            ctx.adjust_logits(x, mask=none, **kw)

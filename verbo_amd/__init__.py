@@ -409,6 +409,8 @@ def _adjust_args(logits, penalty, hist, hist_off, prompt_len, bias_ids, bias, bi
         if mask.dtype != i32 or mask.dim() != 2 or mask.device != dev or mask.stride(1) != 1 or mask.shape[1] < (V + 31) // 32:
             raise VsmpError("mask must be an int32 tensor [masks, >= ceil(V / 32)] with contiguous rows on the logits' device")
         n_masks = mask.shape[0]
+        if n_masks < 1:  # its address would be NULL, which is no masks at all
+            raise VsmpError("mask must hold at least one mask")
         ldm = mask.stride(0) if n_masks > 1 else mask.shape[1]
         mp = mask.data_ptr()
     rest = (_array_of(prompt_len, i32, B, "prompt_len", dev), _array_of(bias_ids, i32, 0, "bias_ids", dev),
