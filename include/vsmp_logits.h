@@ -54,7 +54,7 @@ typedef struct {
  *       device int[B] with each row's mask in it (negative: the row is not masked; n_masks or more:
  *       nothing is allowed), or NULL where row r's mask is mask r (n_masks >= B). mask NULL for none.
  *   out, ldo: device fp32 [B][ldo], ldo >= V: `in` itself with ldi = ldo (fp32), or memory that does
- *       not overlap it. Columns V .. ldo - 1 are left as they are. (vsmp_pick_batch reads it where it
+ *       not overlap it (apart as a whole, or rows between its rows at the same stride in bytes). Columns V .. ldo - 1 are left as they are. (vsmp_pick_batch reads it where it
  *       is 16-byte aligned with ldo a multiple of 4.)
  *   left: NULL, or device int[B]: how many of the row's ids have y > -inf. A row with 0 has nothing to
  *       pick from (vsmp_pick_batch is not defined on it).

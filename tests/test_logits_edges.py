@@ -276,3 +276,22 @@ def test_an_empty_mask_table_is_refused(ctx):
     for kw in (dict(), dict(mask_row=torch.zeros(2, dtype=torch.int32, device="cuda"))):
         with pytest.raises(V.VsmpError, match="mask"):
             ctx.adjust_logits(x, mask=none, **kw)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_adjusted_rows_between_the_logits(ctx, dtype):
+    """Logits and output in one buffer, row by row in turn, share no byte."""
+    import torch
+
+    B, n = 5, 6001
+    rng = np.random.default_rng(7)
+    x = dev(rng.normal(0, 3, (B, n)).astype(np.float32), dtype)
+    step = 4 * (2 * n + 3)  # bytes from a row to the next
+    buf = torch.zeros(B * step, dtype=torch.uint8, device="cuda").view(B, step)
+    size = x.element_size()
+    src = buf[:, :n * size].view(x.dtype)
+    src.copy_(x)
+    out = buf[:, 4 * (n + 1):4 * (2 * n + 1)].view(torch.float32)
+    bias = dict(bias_ids=dev(np.arange(B, dtype=np.int32)), bias=torch.ones(B, device="cuda"), bias_off=dev(np.arange(B + 1, dtype=np.int32)))
+    got = ctx.adjust_logits(src, out=out, **bias)
+    assert got is out and torch.equal(got, ctx.adjust_logits(x, **bias)) and torch.equal(src, x)

@@ -48,13 +48,15 @@ int check_adjust(const AdjustArgs& a, int dtype, bool pen_per_row, const vsmp_pe
     if (!(pen->repeat > 0.0f) || !std::isfinite(pen->repeat) || !std::isfinite(pen->presence) || !std::isfinite(pen->frequency))
       return set_error("vsmp: penalties must be finite, repeat above 0");
   }
-  // the rows in memory: the same ones, or none of the others' bytes
-  const char* i0 = static_cast<const char*>(a.in);
-  const char* i1 = i0 + (static_cast<size_t>(a.B - 1) * a.ldi + a.V) * elem_size(dtype);
-  const char* o0 = reinterpret_cast<const char*>(a.out);
-  const char* o1 = o0 + (static_cast<size_t>(a.B - 1) * a.ldo + a.V) * sizeof(float);
+  // the rows in memory: the same ones, or none of the others' bytes (apart as wholes, or row by row in turn)
+  const long long size = static_cast<long long>(elem_size(dtype)), il = a.V * size, ol = a.V * 4LL, is = a.ldi * size, os = a.ldo * 4;
+  const uintptr_t i0 = reinterpret_cast<uintptr_t>(a.in), o0 = reinterpret_cast<uintptr_t>(a.out);
+  const uintptr_t i1 = i0 + (a.B - 1) * is + il, o1 = o0 + (a.B - 1) * os + ol;
   const bool in_place = i0 == o0 && dtype == VSMP_F32 && a.ldi == a.ldo;
-  if (!in_place && i0 < o1 && o0 < i1) return set_error("vsmp: out must be the fp32 logits themselves or not overlap them");
+  if (!in_place && i0 < o1 && o0 < i1) {
+    const long long at = (static_cast<long long>(o0 - i0) % is + is) % is;  // an output row's place in the logits' stride
+    if (is != os || at < il || at + ol > is) return set_error("vsmp: out must be the fp32 logits themselves or not overlap them");
+  }
   return 0;
 }
 
