@@ -1,4 +1,5 @@
 """Arguments of the operators around the pick and of the serving loop's requests, on the CPU. No GPU calls."""
+import numpy as np
 import pytest
 
 from test_logits_capi import ADJUST, X, refused
@@ -28,3 +29,15 @@ def test_request_takes_prompt_lengths_within_the_prompt(prompt, prompt_len):
 ])
 def test_adjust_refuses_outputs_that_overlap_rows_of_logits(change):
     assert "overlap" in refused("vsmp_adjust_logits", ADJUST, **change)
+
+
+@pytest.mark.parametrize("bad", [V.Penalty(repeat=0.0), V.Penalty(repeat=-1.0), V.Penalty(repeat=float("inf")),
+                                 V.Penalty(presence=float("nan")), V.Penalty(frequency=-float("inf"))])
+def test_per_row_penalties_are_checked_as_shared_ones_are(bad):
+    with pytest.raises(V.VsmpError, match="finite, repeat above 0"):
+        V.to_device_penalties([V.Penalty(1.2, 0.5, 0.25, 8), bad], "cpu")
+    with pytest.raises(V.VsmpError, match="finite, repeat above 0"):
+        V.to_device_penalties(np.array([(bad.repeat, bad.presence, bad.frequency, 0)], V.PENALTY_DTYPE), "cpu")
+    with pytest.raises(V.VsmpError, match="finite, repeat above 0"):
+        decode.Request([1], decode.Opts(), penalty=bad)
+    assert V.to_device_penalties([], "cpu").numel() == 0

@@ -360,14 +360,22 @@ def _array_of(t, dtype, n, name, device):
     return t.data_ptr()
 
 
-def to_device_penalties(rows, device="cuda"):
-    """Upload a PENALTY_DTYPE array, or a list of Penalty, as a device byte tensor for per-row penalties."""
-    import torch
-
+def _penalty_rows(rows):
+    """A PENALTY_DTYPE array of such an array or of a list of Penalty, each of them what a shared one has to be."""
     if not isinstance(rows, np.ndarray):
         rows = np.array([(p.repeat, p.presence, p.frequency, p.window) for p in rows], dtype=PENALTY_DTYPE)
     a = np.ascontiguousarray(rows, dtype=PENALTY_DTYPE)
-    return torch.from_numpy(a.view(np.uint8).copy()).to(device)
+    if not all(np.isfinite(a[f]).all() for f in ("repeat", "presence", "frequency")) or not (a["repeat"] > 0).all():
+        raise VsmpError("penalties must be finite, repeat above 0")
+    return a
+
+
+def to_device_penalties(rows, device="cuda"):
+    """Upload a PENALTY_DTYPE array, or a list of Penalty (finite, repeat above 0), as a device byte tensor for per-row
+    penalties."""
+    import torch
+
+    return torch.from_numpy(_penalty_rows(rows).view(np.uint8).copy()).to(device)
 
 
 def _adjust_args(logits, penalty, hist, hist_off, prompt_len, bias_ids, bias, bias_off, mask, mask_row, out, left, stream,

@@ -27,7 +27,7 @@ import ctypes
 
 import numpy as np
 
-from . import Params, Penalty, VsmpError, _adjust_args, _err, load_library, to_device_penalties
+from . import Params, Penalty, VsmpError, _adjust_args, _err, _penalty_rows, load_library, to_device_penalties
 
 __all__ = ["Opts", "Request", "BatchDecoder", "params_of"]
 
@@ -62,6 +62,8 @@ class Request:
         self.repeat_last = int(repeat_last)
         self.arrival = int(arrival)
         self.penalty = penalty
+        if penalty is not None:
+            _penalty_rows([penalty])  # refused here, not in the middle of a loop that serves others too
         self.prompt_len = int(prompt_len)
         if not 0 <= self.prompt_len <= self.prompt.size:
             raise VsmpError("need 0 <= prompt_len <= the prompt's ids")
