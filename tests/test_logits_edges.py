@@ -4,7 +4,7 @@ import pytest
 
 import verbo_amd as V
 from helpers import log, mode_ctx
-from test_logits_ops import check_adjusted, dev, plain_adjust, plain_logprobs
+from test_logits_ops import check_adjusted, dev, plain_adjust, plain_logprobs, q4_weights
 from verbo_amd import decode
 
 pytestmark = pytest.mark.gpu
@@ -295,3 +295,54 @@ def test_adjusted_rows_between_the_logits(ctx, dtype):
     bias = dict(bias_ids=dev(np.arange(B, dtype=np.int32)), bias=torch.ones(B, device="cuda"), bias_off=dev(np.arange(B + 1, dtype=np.int32)))
     got = ctx.adjust_logits(src, out=out, **bias)
     assert got is out and torch.equal(got, ctx.adjust_logits(x, **bias)) and torch.equal(src, x)
+
+
+def test_outputs_belong_to_the_callers_stream(ctx):
+    """A call on a stream of its own does not take memory that the current stream may still be using, and what it
+    returns is not handed to that stream again while the current one may be using it."""
+    import torch
+
+    B, n, D = 64, 40000, 256
+    x = torch.randn(B, n, device="cuda")
+    half = x.bfloat16()
+    ids = torch.zeros(B, 1, dtype=torch.int32, device="cuda")
+    q, s, z, _ = q4_weights(1, n, D, 64)
+    hidden = torch.randn(B, D, device="cuda").bfloat16()
+    d = decode.BatchDecoder.with_slots(B, n)
+    rows = torch.arange(B, dtype=torch.int32, device="cuda")
+    head = torch.randn(n, D, device="cuda").bfloat16()
+    side = torch.cuda.Stream()
+    calls = [lambda st: ctx.adjust_logits(half, stream=st), lambda st: d.adjust_rows(half, rows, stream=st),
+             lambda st: ctx.head_logits_q4(hidden, q, s, 64, stream=st), lambda st: ctx.head_logits(hidden, head, stream=st)]
+    for call in calls:
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        want = call(None)  # the context's scratch is there from here on
+        torch.cuda.synchronize()
+        old = torch.empty(B, n, device="cuda")
+        at = old.data_ptr()
+        del old  # free for the current stream alone
+        got = call(side)
+        assert got.data_ptr() != at
+        side.synchronize()
+        assert torch.equal(got, want)
+        torch.cuda._sleep(50_000_000)  # the current stream is busy with `got`
+        keep = got + 0.0
+        at = got.data_ptr()
+        del got
+        with torch.cuda.stream(side):
+            again = torch.empty(B, n, device="cuda")
+        assert again.data_ptr() != at
+        again.fill_(7.0)
+        torch.cuda.synchronize()
+        assert torch.equal(keep, want)
+        del again, keep, want
+    for call in (lambda st: ctx.logprobs(x, ids, stream=st), lambda st: (ctx.pick_batch(x, V.Params(temp=0.0), stream=st),)):
+        call(None)
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        old = [torch.empty(B, device="cuda") for _ in range(16)]
+        at = [t.data_ptr() for t in old]
+        del old
+        assert not {t.data_ptr() for t in call(side)} & set(at)
+        torch.cuda.synchronize()

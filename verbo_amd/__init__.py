@@ -252,7 +252,7 @@ def _batch_args(logits, params, hist, hist_off, u_mode, u, rng_state, counter, o
     if logits.stride(1) != 1:
         raise VsmpError("logits rows must be contiguous")
     if out is None:
-        out = torch.empty(B, dtype=torch.int32, device=logits.device)
+        out = _t().output((B,), torch.int32, logits.device, stream)
     if isinstance(params, Params):
         pp, per_row = ctypes.addressof(params), 0
     else:
@@ -313,6 +313,7 @@ class _Torch:
         self.codes = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # vsmp_dtype
         self._raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         self._current = torch.cuda.current_stream
+        self._use = torch.cuda.stream
 
     def stream(self, stream, device):
         """The address of `stream`, or of torch's current one on `device`."""
@@ -320,10 +321,21 @@ class _Torch:
             return stream.cuda_stream
         return self._raw(device.index) if self._raw is not None else self._current(device).cuda_stream
 
-    def rows16(self, B, V, device):
-        """A new float32 [B, V] whose rows are padded to 16 bytes, and their stride."""
+    def output(self, shape, dtype, device, stream):
+        """A new tensor that a call on `stream` (None: the current one) writes. On a stream of its own the call takes
+        that stream's memory, since the current one may still be using what it has freed; once the tensor is freed,
+        the memory waits for the work of both."""
+        if stream is None or stream.cuda_stream == self.stream(None, device):
+            return self.empty(shape, dtype=dtype, device=device)
+        with self._use(stream):
+            t = self.empty(shape, dtype=dtype, device=device)
+        t.record_stream(self._current(device))
+        return t
+
+    def rows16(self, B, V, device, stream):
+        """Such an output of float32 [B, V] whose rows are padded to 16 bytes, and their stride."""
         ld = (V + 3) // 4 * 4
-        t = self.empty((B, ld), dtype=self.float32, device=device)
+        t = self.output((B, ld), self.float32, device, stream)
         return (t if ld == V else t[:, :V]), ld
 
 
@@ -387,7 +399,7 @@ def _adjust_args(logits, penalty, hist, hist_off, prompt_len, bias_ids, bias, bi
     code, ld = _rows_of(logits, "logits", dev)
     B, V = logits.shape
     if out is None:  # rows on 16 bytes, so that pick_batch can take them
-        out, ldo = T.rows16(B, V, dev)
+        out, ldo = T.rows16(B, V, dev, stream)
     else:
         ocode, ldo = _rows_of(out, "out", dev)
         if ocode != 0 or out.shape != logits.shape:
@@ -469,7 +481,7 @@ class Context:
 
         B, D, V = _head_shapes(hidden, head)
         if logits is None:  # rows padded to 16 bytes, so that pick_batch can take them
-            logits = torch.empty(B, (V + 3) // 4 * 4, dtype=torch.float32, device=hidden.device)[:, :V]
+            logits = _t().rows16(B, V, hidden.device, stream)[0]
         _check_rows(logits, torch.float32, "logits")
         st = stream if stream is not None else torch.cuda.current_stream(hidden.device)
         if _lib.vsmp_head_logits(self._h, hidden.data_ptr(), hidden.stride(0), head.data_ptr(), head.stride(0), B, V, D,
@@ -486,7 +498,7 @@ class Context:
 
         B, D, V = _head_shapes(hidden, head)
         if out is None:
-            out = torch.empty(B, dtype=torch.int32, device=hidden.device)
+            out = _t().output((B,), torch.int32, hidden.device, stream)
         if logits is not None:
             _check_rows(logits, torch.float32, "logits")
         if isinstance(params, Params):
@@ -542,7 +554,7 @@ class Context:
         dev = logits.device
         code, ld = _rows_of(logits, "logits", dev)
         B, V = logits.shape
-        lse = T.empty((B,), dtype=T.float32, device=dev)
+        lse = T.output((B,), T.float32, dev, stream)
         lp = rk = None
         n = ldj = 0
         if ids is not None:
@@ -552,8 +564,8 @@ class Context:
             if n > 1 and ids.stride(1) != 1:
                 raise VsmpError("ids must have contiguous rows")
             ldj = ids.stride(0) if B > 1 else n
-            lp = T.empty((B, n), dtype=T.float32, device=dev)
-            rk = T.empty((B, n), dtype=T.int32, device=dev) if rank else None
+            lp = T.output((B, n), T.float32, dev, stream)
+            rk = T.output((B, n), T.int32, dev, stream) if rank else None
         if _lib.vsmp_logprobs(self._h, logits.data_ptr(), code, ld, B, V, ids.data_ptr() if n else None, ldj, n,
                               lp.data_ptr() if n else None, rk.data_ptr() if n and rk is not None else None,
                               lse.data_ptr(), T.stream(stream, dev)) != 0:
@@ -588,7 +600,7 @@ class Context:
                 raise VsmpError("zeros must be uint8 of the scales' shape with contiguous rows")
             ldz = zeros.stride(0) if V > 1 else zeros.shape[1]
         if logits is None:  # rows padded to 16 bytes, so that pick_batch can take them
-            logits, ldl = T.rows16(B, V, dev)
+            logits, ldl = T.rows16(B, V, dev, stream)
         else:
             lcode, ldl = _rows_of(logits, "logits", dev)
             if lcode != 0 or logits.shape != (B, V):
