@@ -4,7 +4,7 @@ import pytest
 
 import verbo_amd as V
 from helpers import log, mode_ctx
-from test_logits_ops import check_adjusted, dev, plain_adjust, plain_logprobs, q4_weights
+from test_logits_ops import check_adjusted, check_head, dev, plain_adjust, plain_logprobs, q4_weights
 from verbo_amd import decode
 
 pytestmark = pytest.mark.gpu
@@ -346,3 +346,18 @@ def test_outputs_belong_to_the_callers_stream(ctx):
         del old
         assert not {t.data_ptr() for t in call(side)} & set(at)
         torch.cuda.synchronize()
+
+
+# ---- the head with 4-bit weights ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("G,zeros,scales,dtype", [(32, True, "f32", "bf16"), (64, False, "bf16", "f16"), (128, True, "f16", "bf16")])
+def test_head_q4_every_small_hidden_size(ctx, G, zeros, scales, dtype):
+    """Every hidden size below 256, which is staged whole, with batches around 16 rows."""
+    rng = np.random.default_rng(G)
+    for D in range(G, 256, G):
+        q, s, z, w = q4_weights(D, 131, D, G, scales, zeros)
+        for B in (1, 15, 16, 17, 33):
+            hidden = dev(rng.normal(0, 1, (B, D)).astype(np.float32), dtype)
+            log("small head", G, D, B)
+            check_head(ctx.head_logits_q4(hidden, q, s, G, zeros=z), hidden, s, z, w, G)

@@ -91,115 +91,107 @@ __device__ __forceinline__ void swap16(uint32_t& a, uint32_t& b) {
   b = r[1];
 }
 
-// The small hidden sizes: a workgroup of four waves takes 16 rows and 128 columns, x and the scales staged in
-// LDS by chunks of KC in two buffers, the next chunk's weights loaded while one is multiplied.
+// The small hidden sizes (D < 256): a workgroup of four waves takes 16 rows and 128 columns, x and the scales staged
+// in LDS once while the weights are on their way to registers.
 //
-// H: f16 hidden states (else bf16). G: group. ZP: zero points given. KC: hidden
-// elements per chunk.
-template <bool H, int G, bool ZP, int KC>
+// H: f16 hidden states (else bf16). G: group. ZP: zero points given.
+constexpr int kTileD = 256;              // hidden elements that the stage holds
+constexpr int kTileStr = kTileD + 8;     // halfwords per x row in LDS: 16 rows' reads fall on distinct banks
+constexpr int tile_groups(int g) { return kTileD / g; }
+constexpr int tile_lds(int rows, int g, bool zp) {
+  return rows * kTileStr * 2 + tile_groups(g) * 16 * 4 + kQBn * tile_groups(g) * 4 * (zp ? 2 : 1);
+}
+template <bool H, int G, bool ZP>
 __global__ __launch_bounds__(kQNt) void k_head_q4_tile(HeadQ4Args a, int rows_ld) {
-  constexpr int MB = 1;               // blocks of 16 rows
-  constexpr int kStr = KC + 8;        // halfwords per x row in LDS: 16 rows' reads fall on distinct banks
-  constexpr int kBlk = KC / 128;      // blocks of 128 per chunk
-  constexpr int kGc = KC / G;         // groups per chunk
-  constexpr int kGb = 128 / G;        // groups per block
-  constexpr int kPr = KC / 8;         // 16-byte pieces of an x row per chunk
-  constexpr int kQx = MB * 16 * kPr / kQNt;
+  constexpr int kBlk = kTileD / 128;       // blocks of 128
+  constexpr int kGc = tile_groups(G);
+  constexpr int kGb = 128 / G;             // groups per block
+  constexpr int kPr = kTileD / 8;          // 16-byte pieces of an x row
+  constexpr int kQx = 16 * kPr / kQNt;
   constexpr int kQs = kQBn * kGc / kQNt;
-  constexpr int kSteps = G / 32;      // MFMAs per group
+  constexpr int kSteps = G / 32;           // MFMAs per group
 
+  // x [rows_ld][kTileStr], X [kGc][16], scales [kBlk][kQBn][kGb], offsets the same
   extern __shared__ __align__(16) unsigned char lds[];
-  // two stages of: x [rows_ld][kStr], X [kGc][MB * 16], scales [kBlk][kQBn][kGb], offsets the same
-  const int xbytes = rows_ld * kStr * 2;
-  constexpr int kXsBytes = kGc * MB * 16 * 4, kScBytes = kQBn * kGc * 4;
-  const int stage = xbytes + kXsBytes + kScBytes * (ZP ? 2 : 1);
-  auto sx = [&](int b) { return reinterpret_cast<uint16_t*>(lds + b * stage); };
-  auto sX = [&](int b) { return reinterpret_cast<float*>(lds + b * stage + xbytes); };
-  auto sS = [&](int b) { return reinterpret_cast<float*>(lds + b * stage + xbytes + kXsBytes); };
-  auto sO = [&](int b) { return reinterpret_cast<float*>(lds + b * stage + xbytes + kXsBytes + kScBytes); };
+  uint16_t* sx = reinterpret_cast<uint16_t*>(lds);
+  float* sX = reinterpret_cast<float*>(lds + rows_ld * kTileStr * 2);
+  float* sS = sX + kGc * 16;
+  float* sO = sS + kQBn * kGc;
 
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, c16 = lane & 15, h = lane >> 4;
-  const int m0 = blockIdx.y * (MB * 16), rows = min(rows_ld, a.B - m0);
+  const int m0 = blockIdx.y * 16, rows = min(rows_ld, a.B - m0);
   const int n0 = blockIdx.x * kQBn;
   const uint16_t* x = a.x + m0 * a.ldx;
-  const int D = a.D, nch = (D + KC - 1) / KC, groups = D / G;
-
-  // where the lane's pieces come from
-  const uint8_t* wq[kQNs];
-#pragma unroll
-  for (int s = 0; s < kQNs; ++s) wq[s] = a.q + min(n0 + (wv * kQNs + s) * 16 + c16, a.V - 1) * a.ldq;
+  const int D = a.D, groups = D / G;
 
   u32x4 w[kQNs][kBlk];
-  auto load_w = [&](int c, int s, int b) {
-    const int byte = min(c * (KC / 2) + b * 64 + h * 16, D / 2 - 16);
-    w[s][b] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wq[s] + byte));
-  };
+#pragma unroll
+  for (int s = 0; s < kQNs; ++s) {
+    const uint8_t* q = a.q + min(n0 + (wv * kQNs + s) * 16 + c16, a.V - 1) * a.ldq;
+#pragma unroll
+    for (int b = 0; b < kBlk; ++b)  // past D: some weights or others, x is zero there
+      w[s][b] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(q + min(b * 64 + h * 16, D / 2 - 16)));
+  }
+
   u32x4 px[kQx];
   float ps[kQs], pz[ZP ? kQs : 1];
-  auto load_xs = [&](int c) {
 #pragma unroll
-    for (int q = 0; q < kQx; ++q) {
-      const int p = tid + q * kQNt, r = p / kPr, k = c * KC + 8 * (p % kPr);
-      px[q] = u32x4{0u, 0u, 0u, 0u};
-      if (r < rows && k < D) px[q] = *reinterpret_cast<const u32x4*>(x + r * a.ldx + k);
+  for (int q = 0; q < kQx; ++q) {
+    const int p = tid + q * kQNt, r = p / kPr, k = 8 * (p % kPr);
+    px[q] = u32x4{0u, 0u, 0u, 0u};
+    if (r < rows && k < D) px[q] = *reinterpret_cast<const u32x4*>(x + r * a.ldx + k);
+  }
+#pragma unroll
+  for (int q = 0; q < kQs; ++q) {
+    const int i = tid + q * kQNt, g = min(i % kGc, groups - 1);
+    const long long col = min(n0 + i / kGc, a.V - 1);
+    ps[q] = scale_at(a.sc, a.sc_type, col * a.lds + g);
+    if (ZP) pz[q] = static_cast<float>(a.z[col * a.ldz + g]);
+  }
+#pragma unroll
+  for (int q = 0; q < kQx; ++q) {
+    const int p = tid + q * kQNt, r = p / kPr, k8 = p % kPr;
+    const u32x4 v = px[q];
+    float s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s += half_val<H>(v[j] & 0xFFFFu) + half_val<H>(v[j] >> 16);
+#pragma unroll
+    for (int d = 1; d < G / 8; d <<= 1) s += __shfl_xor(s, d);
+    if (r < rows) {
+      u32x4 o;
+      o.x = (v.x & 0xFFFFu) | (v.z << 16);
+      o.y = (v.x >> 16) | (v.z & 0xFFFF0000u);
+      o.z = (v.y & 0xFFFFu) | (v.w << 16);
+      o.w = (v.y >> 16) | (v.w & 0xFFFF0000u);
+      *reinterpret_cast<u32x4*>(&sx[r * kTileStr + 8 * k8]) = o;
+      if (k8 % (G / 8) == 0) sX[k8 / (G / 8) * 16 + r] = ZP ? s : -24.0f * s;
     }
+  }
 #pragma unroll
-    for (int q = 0; q < kQs; ++q) {
-      const int i = tid + q * kQNt, g = min(c * kGc + i % kGc, groups - 1);
-      const long long col = min(n0 + i / kGc, a.V - 1);
-      ps[q] = scale_at(a.sc, a.sc_type, col * a.lds + g);
-      if (ZP) pz[q] = static_cast<float>(a.z[col * a.ldz + g]);
-    }
-  };
-  auto store_xs = [&](int b) {
-#pragma unroll
-    for (int q = 0; q < kQx; ++q) {
-      const int p = tid + q * kQNt, r = p / kPr, k8 = p % kPr;
-      const u32x4 v = px[q];
-      float s = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s += half_val<H>(v[j] & 0xFFFFu) + half_val<H>(v[j] >> 16);
-#pragma unroll
-      for (int d = 1; d < G / 8; d <<= 1) s += __shfl_xor(s, d);
-      if (r < rows) {
-        u32x4 o;
-        o.x = (v.x & 0xFFFFu) | (v.z << 16);
-        o.y = (v.x >> 16) | (v.z & 0xFFFF0000u);
-        o.z = (v.y & 0xFFFFu) | (v.w << 16);
-        o.w = (v.y >> 16) | (v.w & 0xFFFF0000u);
-        *reinterpret_cast<u32x4*>(&sx(b)[r * kStr + 8 * k8]) = o;
-        if (k8 % (G / 8) == 0) sX(b)[k8 / (G / 8) * (MB * 16) + r] = ZP ? s : -24.0f * s;
-      }
-    }
-#pragma unroll
-    for (int q = 0; q < kQs; ++q) {
-      const int i = tid + q * kQNt, g = i % kGc, col = i / kGc;
-      const int at = (g / kGb * kQBn + col) * kGb + g % kGb;
-      sS(b)[at] = ps[q];
-      if (ZP) sO(b)[at] = -16.0f - pz[q];
-    }
-  };
+  for (int q = 0; q < kQs; ++q) {
+    const int i = tid + q * kQNt, g = i % kGc, col = i / kGc;
+    const int at = (g / kGb * kQBn + col) * kGb + g % kGb;
+    sS[at] = ps[q];
+    if (ZP) sO[at] = -16.0f - pz[q];
+  }
+  __syncthreads();
 
   const Widen<H> widen;
-  f32x4 acc[kQNs][MB];
+  f32x4 acc[kQNs];
 #pragma unroll
-  for (int s = 0; s < kQNs; ++s)
-#pragma unroll
-    for (int i = 0; i < MB; ++i) acc[s][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s = 0; s < kQNs; ++s) acc[s] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
   // the lane's x row and its offset in a block: k of step t is (t's) + kl
-  int xa[MB];
   const int kl = G == 32 ? 8 * h : (G == 64 ? 32 * (h & 1) + 16 * (h >> 1) : 32 * h);
+  const int xa = min(c16, rows - 1) * kTileStr + kl;
 #pragma unroll
-  for (int i = 0; i < MB; ++i) xa[i] = min(16 * i + c16, rows - 1) * kStr + kl;
-
-  auto block = [&](int buf, int b, auto reload) {
+  for (int b = 0; b < kBlk; ++b) {
+    if (b * 128 >= D) break;
     uint32_t t[kQNs][4];
     float sc[kQNs][kGb], of[kQNs][kGb];
 #pragma unroll
     for (int s = 0; s < kQNs; ++s) {
       t[s][0] = w[s][b].x, t[s][1] = w[s][b].y, t[s][2] = w[s][b].z, t[s][3] = w[s][b].w;
-      reload(s);
       if constexpr (G <= 64) {
         swap32(t[s][0], t[s][2]);
         swap32(t[s][1], t[s][3]);
@@ -211,73 +203,43 @@ __global__ __launch_bounds__(kQNt) void k_head_q4_tile(HeadQ4Args a, int rows_ld
       const int col = (wv * kQNs + s) * 16 + c16;
 #pragma unroll
       for (int g = 0; g < kGb; ++g) {
-        sc[s][g] = sS(buf)[(b * kQBn + col) * kGb + g];
-        of[s][g] = ZP ? sO(buf)[(b * kQBn + col) * kGb + g] : 0.0f;
+        sc[s][g] = sS[(b * kQBn + col) * kGb + g];
+        of[s][g] = ZP ? sO[(b * kQBn + col) * kGb + g] : 0.0f;
       }
     }
 #pragma unroll
     for (int g = 0; g < kGb; ++g) {
-      f32x4 X[MB], P[kQNs][MB];
-#pragma unroll
-      for (int i = 0; i < MB; ++i)
-        X[i] = *reinterpret_cast<const f32x4*>(&sX(buf)[(b * kGb + g) * (MB * 16) + 16 * i + 4 * h]);
+      const f32x4 X = *reinterpret_cast<const f32x4*>(&sX[(b * kGb + g) * 16 + 4 * h]);
+      f32x4 P[kQNs];
 #pragma unroll
       for (int u = 0; u < kSteps; ++u) {
         const int step = g * kSteps + u;
         const int k = b * 128 + (G == 32 ? 32 * step : (G == 64 ? 64 * g + 8 * u : 8 * step));
-        u32x4 A[MB];
-#pragma unroll
-        for (int i = 0; i < MB; ++i) A[i] = *reinterpret_cast<const u32x4*>(&sx(buf)[xa[i] + k]);
+        const u32x4 A = *reinterpret_cast<const u32x4*>(&sx[xa + k]);
 #pragma unroll
         for (int s = 0; s < kQNs; ++s) {
-          const u32x4 wb = widen(t[s][step]);
+          f32x4 c = u ? P[s] : X;
+          if (ZP && u == 0) {
 #pragma unroll
-          for (int i = 0; i < MB; ++i) {
-            f32x4 c = u ? P[s][i] : X[i];
-            if (ZP && u == 0) {
-#pragma unroll
-              for (int r = 0; r < 4; ++r) c[r] *= of[s][g];
-            }
-            P[s][i] = mfma<H>(A[i], wb, c);
+            for (int r = 0; r < 4; ++r) c[r] *= of[s][g];
           }
+          P[s] = mfma<H>(A, widen(t[s][step]), c);
         }
       }
 #pragma unroll
       for (int s = 0; s < kQNs; ++s)
 #pragma unroll
-        for (int i = 0; i < MB; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[s][i][r] = __builtin_fmaf(sc[s][g], P[s][i][r], acc[s][i][r]);
-    }
-  };
-
-#pragma unroll
-  for (int b = 0; b < kBlk; ++b)
-#pragma unroll
-    for (int s = 0; s < kQNs; ++s) load_w(0, s, b);
-  load_xs(0);
-  store_xs(0);
-  if (nch > 1) load_xs(1);
-  for (int c = 0; c < nch; ++c) {
-    __syncthreads();  // chunk c's stage is written, chunk c - 1's no longer read
-#pragma unroll
-    for (int b = 0; b < kBlk; ++b)
-      if (c * KC + b * 128 < D) block(c & 1, b, [&](int s) { if (c + 1 < nch) load_w(c + 1, s, b); });
-    if (c + 1 < nch) {
-      store_xs((c + 1) & 1);
-      if (c + 2 < nch) load_xs(c + 2);
+        for (int r = 0; r < 4; ++r) acc[s][r] = __builtin_fmaf(sc[s][g], P[s][r], acc[s][r]);
     }
   }
 #pragma unroll
   for (int s = 0; s < kQNs; ++s) {
     const int col = n0 + (wv * kQNs + s) * 16 + c16;
 #pragma unroll
-    for (int i = 0; i < MB; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = 16 * i + 4 * h + r;
-        if (col < a.V && row < rows) a.out[(m0 + row) * a.ldo + col] = acc[s][i][r];
-      }
+    for (int r = 0; r < 4; ++r) {
+      const int row = 4 * h + r;
+      if (col < a.V && row < rows) a.out[(m0 + row) * a.ldo + col] = acc[s][r];
+    }
   }
 }
 
@@ -619,14 +581,10 @@ void launch_rows(const HeadQ4Args& a, int cus, hipStream_t st) {
 
 template <bool H, int G, bool ZP>
 void launch_tile(const HeadQ4Args& a, hipStream_t st) {
-  constexpr int KC = 256;
-  const int rows_ld = a.B < 16 ? a.B : 16;
-  const int stage = rows_ld * (KC + 8) * 2 + KC / G * 16 * 4 + kQBn * (KC / G) * 4 * (ZP ? 2 : 1);
+  const int rows_ld = std::min(a.B, 16);
   const dim3 grid((a.V + kQBn - 1) / kQBn, (a.B + 15) / 16);
-  constexpr int kMost = 2 * (16 * (KC + 8) * 2 + KC / G * 16 * 4 + kQBn * (KC / G) * 4 * (ZP ? 2 : 1));
-  static DynLdsOnce configured;
-  allow_dyn_lds(configured, {reinterpret_cast<const void*>(k_head_q4_tile<H, G, ZP, KC>)}, kMost);
-  hipLaunchKernelGGL((k_head_q4_tile<H, G, ZP, KC>), grid, dim3(kQNt), 2 * stage, st, a, rows_ld);
+  static_assert(tile_lds(16, 32, true) <= 64 * 1024, "the stage fits the default limit of dynamic LDS");
+  hipLaunchKernelGGL((k_head_q4_tile<H, G, ZP>), grid, dim3(kQNt), tile_lds(rows_ld, G, ZP), st, a, rows_ld);
 }
 
 // The rows of a workgroup: the fewest of 4, 16 and 32 that hold the batch; for larger ones 64, or 32 where the x of
