@@ -4,7 +4,7 @@ import pytest
 
 import verbo_amd as V
 from helpers import log, mode_ctx
-from test_logits_ops import check_adjusted, check_head, dev, plain_adjust, plain_logprobs, q4_weights
+from test_logits_ops import check_adjusted, check_head, dev, pack, plain_adjust, plain_logprobs, q4_weights
 from verbo_amd import decode
 
 pytestmark = pytest.mark.gpu
@@ -361,3 +361,52 @@ def test_head_q4_every_small_hidden_size(ctx, G, zeros, scales, dtype):
             hidden = dev(rng.normal(0, 1, (B, D)).astype(np.float32), dtype)
             log("small head", G, D, B)
             check_head(ctx.head_logits_q4(hidden, q, s, G, zeros=z), hidden, s, z, w, G)
+
+
+# ---- far operands --------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("D,scales", [(64, "f32"), (640, "f32"), (640, "bf16")])
+def test_head_q4_operands_far_apart(ctx, D, scales):
+    """Hidden rows 2^30 elements apart, and columns of the weights, scales and zero points as far apart as they may
+    be: column and row offsets beyond 2^32 bytes."""
+    import torch
+
+    if torch.cuda.mem_get_info()[0] < 120 << 30:
+        pytest.skip("needs 120 GB of device memory")
+    n, G = 300, 32
+    q, s, z, w = q4_weights(D, n, D, G, scales, True)
+
+    def far(t, ld):
+        rows, cols = t.shape
+        v = torch.empty((rows - 1) * ld + cols, dtype=t.dtype, device="cuda").as_strided((rows, cols), (ld, 1))
+        v.copy_(t)
+        return v
+
+    fq, fs, fz = far(q, (1 << 26) - 16), far(s, (1 << 24) - 1), far(z, (1 << 26) - 1)
+    for B in (3, 9, 70):
+        hidden = torch.randn(B, D, device="cuda").bfloat16()
+        log("far head", D, B)
+        fh = far(hidden, 1 << 30) if B < 70 else hidden
+        got = ctx.head_logits_q4(fh, fq, fs, G, zeros=fz)
+        check_head(got, hidden, s, z, w, G)
+        assert torch.equal(got, ctx.head_logits_q4(hidden, q, s, G, zeros=z))
+        del fh
+
+
+def test_masks_far_apart(ctx):
+    """A table whose masks lie 2^30 words apart."""
+    import torch
+
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of device memory")
+    n, ld = 5000, 1 << 30
+    rng = np.random.default_rng(5)
+    allow = [rng.random(n) < 0.5 for _ in range(4)]
+    near = dev(pack(allow, n, (n + 31) // 32))
+    table = torch.empty(3 * ld + near.shape[1], dtype=torch.int32, device="cuda").as_strided(near.shape, (ld, 1))
+    table.copy_(near)
+    x = torch.randn(6, n, device="cuda")
+    row = dev(np.array([3, -1, 0, 2, 3, 1], np.int32))
+    assert torch.equal(ctx.adjust_logits(x, mask=table, mask_row=row), ctx.adjust_logits(x, mask=near, mask_row=row))
+    assert torch.equal(ctx.adjust_logits(x[:4], mask=table), ctx.adjust_logits(x[:4], mask=near))
