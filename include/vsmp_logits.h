@@ -43,7 +43,7 @@ typedef struct {
  * each step rounded to fp32. Ids outside [0, V) in histories and biases are ignored.
  *   in, dtype, ldi: device logits, row r at element r * ldi (ldi >= V).
  *   pen, pen_per_row: NULL for no penalties; 0 -> a HOST pointer to one struct used by every row;
- *       1 -> a DEVICE array of B structs.
+ *       1 -> a DEVICE array of B structs (aligned to 4 bytes).
  *   hist, hist_off: device CSR of histories, oldest first, as vsmp_pick_batch's; both NULL for none.
  *   prompt_len: device int[B], the number of ids at the start of row r's history that are its prompt
  *       (they count for `repeat` alone), or NULL for 0.

@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from test_logits_capi import ADJUST, X, refused
+from test_logits_capi import ADJUST, OTHER, X, refused
 
 import verbo_amd as V
 from verbo_amd import decode
@@ -41,3 +41,8 @@ def test_per_row_penalties_are_checked_as_shared_ones_are(bad):
     with pytest.raises(V.VsmpError, match="finite, repeat above 0"):
         decode.Request([1], decode.Opts(), penalty=bad)
     assert V.to_device_penalties([], "cpu").numel() == 0
+
+
+@pytest.mark.parametrize("shift", [1, 2, 3])
+def test_adjust_refuses_per_row_penalties_off_their_alignment(shift):
+    assert "per-row penalties" in refused("vsmp_adjust_logits", ADJUST, pen=OTHER + shift, per_row=1)

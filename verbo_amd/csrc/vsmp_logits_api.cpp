@@ -48,6 +48,8 @@ int check_adjust(const AdjustArgs& a, int dtype, bool pen_per_row, const vsmp_pe
     if (!(pen->repeat > 0.0f) || !std::isfinite(pen->repeat) || !std::isfinite(pen->presence) || !std::isfinite(pen->frequency))
       return set_error("vsmp: penalties must be finite, repeat above 0");
   }
+  // a row's struct is read with scalar loads, which take an address's low two bits for zero
+  if (pen_per_row && !aligned(pen, 4)) return set_error("vsmp: per-row penalties must be aligned to 4 bytes");
   // the rows in memory: the same ones, or none of the others' bytes (apart as wholes, or row by row in turn)
   const long long size = static_cast<long long>(elem_size(dtype)), il = a.V * size, ol = a.V * 4LL, is = a.ldi * size, os = a.ldo * 4;
   const uintptr_t i0 = reinterpret_cast<uintptr_t>(a.in), o0 = reinterpret_cast<uintptr_t>(a.out);
