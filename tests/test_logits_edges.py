@@ -326,13 +326,14 @@ def test_outputs_belong_to_the_callers_stream(ctx):
         assert got.data_ptr() != at
         side.synchronize()
         assert torch.equal(got, want)
-        torch.cuda._sleep(50_000_000)  # the current stream is busy with `got`
-        keep = got + 0.0
+        torch.cuda._sleep(400_000_000)  # the current stream is busy with `got`
+        keep, used = got + 0.0, torch.cuda.Event()
+        used.record()
         at = got.data_ptr()
         del got
         with torch.cuda.stream(side):
             again = torch.empty(B, n, device="cuda")
-        assert again.data_ptr() != at
+        assert again.data_ptr() != at or used.query()  # free again only once the current stream has read it
         again.fill_(7.0)
         torch.cuda.synchronize()
         assert torch.equal(keep, want)
@@ -410,3 +411,107 @@ def test_masks_far_apart(ctx):
     row = dev(np.array([3, -1, 0, 2, 3, 1], np.int32))
     assert torch.equal(ctx.adjust_logits(x, mask=table, mask_row=row), ctx.adjust_logits(x, mask=near, mask_row=row))
     assert torch.equal(ctx.adjust_logits(x[:4], mask=table), ctx.adjust_logits(x[:4], mask=near))
+
+
+# ---- the largest sizes, the smallest values ----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_the_largest_vocabulary(ctx, dtype):
+    """Rows of 2^20 logits: adjusted, and their log-probabilities and ranks."""
+    import torch
+
+    n, B = 1 << 20, 2
+    rng = np.random.default_rng(3)
+    x = rng.normal(0, 3, (B, n)).astype(np.float32)
+    xd = dev(x, dtype)
+    xs = xd.float().cpu().numpy()
+    hists = [rng.integers(0, n, 5000), np.array([0, n - 1, n - 1, 77])]
+    flat, off = np.concatenate(hists).astype(np.int32), np.array([0, 5000, 5004], np.int32)
+    masks = [None, rng.random(n) < 0.5]
+    left = torch.empty(B, dtype=torch.int32, device="cuda")
+    pen = V.Penalty(1.25, 0.5, 0.25, 4000)
+    log("largest", dtype)
+    y = ctx.adjust_logits(xd, pen, dev(flat), dev(off), mask=dev(pack(masks[1:], n, n // 32)), mask_row=dev(np.array([-1, 0], np.int32)),
+                          left=left)
+    check_adjusted(y, left, *plain_adjust(xs, [pen], hists, None, None, masks))
+    ids = np.concatenate([np.argsort(-xs, 1, kind="stable")[:, :4], np.tile([0, n - 1, n, n // 2], (B, 1))], 1).astype(np.int32)
+    lp, rank, lse = ctx.logprobs(xd, dev(ids))
+    wl, _, wz, tol = plain_logprobs(xs, ids)
+    assert np.array_equal(rank.cpu().numpy(), plain_ranks(xs, ids))
+    assert (np.abs(lse.cpu().numpy() - wz) <= tol + 2.0 ** -24 * np.abs(wz)).all()
+    g, fin = lp.cpu().numpy(), np.isfinite(wl)
+    # the bound of the sums, and a rounding each of the difference from the largest logit and of the result
+    with np.errstate(invalid="ignore"):
+        most = tol[:, None] + 2.0 ** -24 * (4 * np.abs(wl) + tol[:, None])
+        assert (np.abs(g - wl) <= most)[fin].all() and np.array_equal(g[~fin], wl[~fin])
+
+
+@pytest.mark.parametrize("D", [64, 256])
+def test_head_q4_the_largest_vocabulary(ctx, D):
+    n, G = 1 << 20, 64
+    import torch
+
+    q, s, z, w = q4_weights(D, n, D, G, "bf16", True)
+    hidden = torch.randn(2, D, device="cuda").bfloat16()
+    got = ctx.head_logits_q4(hidden, q, s, G, zeros=z)
+    check_head(got, hidden, s, z, w, G)
+
+
+def test_denormal_logits(ctx):
+    """Logits and adjusted values below the smallest normal float keep their bits, order and ties."""
+    n = 5000
+    rng = np.random.default_rng(9)
+    x = (rng.integers(-40, 41, (3, n)) * np.float32(2.0 ** -149)).astype(np.float32)
+    x[1] = rng.integers(-3, 4, n).astype(np.float32) * np.float32(2.0 ** -126)
+    x[2, ::7] = -0.0
+    ids = np.concatenate([rng.integers(0, n, (3, 50)), np.argsort(-x, 1, kind="stable")[:, :8]], 1).astype(np.int32)
+    lp, rank, lse = ctx.logprobs(dev(x), dev(ids))
+    assert np.array_equal(rank.cpu().numpy(), plain_ranks(x, ids))
+    h, off = rng.integers(0, n, 9000).astype(np.int32), np.array([0, 3000, 6000, 9000], np.int32)
+    got = ctx.adjust_logits(dev(x), V.Penalty(repeat=1.5), dev(h), dev(off)).cpu().numpy()
+    want = x.copy()
+    for r in range(3):
+        s = np.unique(h[off[r]:off[r + 1]])
+        want[r, s] = np.where(x[r, s] > 0, x[r, s] / np.float32(1.5), x[r, s] * np.float32(1.5))
+    assert np.array_equal(got.view(np.int32), want.view(np.int32))
+
+
+@pytest.mark.parametrize("D,B", [(96, 5), (640, 3), (640, 9), (640, 30), (640, 64)])
+def test_head_q4_rows_do_not_touch_each_other(ctx, D, B):
+    """A row of NaN (the documentation asks for finite hidden states) leaves the other rows' bits alone."""
+    import torch
+
+    q, s, z, _ = q4_weights(D, 333, D, 32, "f32", True)
+    hidden = torch.randn(B, D, device="cuda").bfloat16()
+    want = ctx.head_logits_q4(hidden, q, s, 32, zeros=z)
+    hidden[B // 2] = NAN
+    got = ctx.head_logits_q4(hidden, q, s, 32, zeros=z)
+    rest = [r for r in range(B) if r != B // 2]
+    assert torch.equal(got[rest], want[rest]) and torch.isnan(got[B // 2]).all()
+
+
+def test_every_slot_without_a_slot_list():
+    """vsmp_bsampler_adjust_rows with rows NULL: row i is slot i, for more slots than one launch counts."""
+    import torch
+
+    n, slots = 7, 9001
+    rng = np.random.default_rng(4)
+    d = decode.BatchDecoder([decode.Opts(temp=0.0)] * slots, n, repeat_last=1, cap=4)
+    said = []
+    live = torch.ones(slots, dtype=torch.int32, device="cuda")
+    for _ in range(7):
+        said.append(rng.integers(0, n, slots).astype(np.int32))
+        d.accept(dev(said[-1]), live, torch.cuda.current_stream())
+    x = rng.normal(0, 2, (slots, n)).astype(np.float32)
+    xd, out, left = dev(x), torch.empty(slots, n, device="cuda"), torch.empty(slots, dtype=torch.int32, device="cuda")
+    pens = V.to_device_penalties(np.array([(1.0, 0.5, 0.25, 0)] * slots, V.PENALTY_DTYPE))
+    prompt = torch.from_numpy((np.arange(slots) % 9).astype(np.int32)).cuda()
+    rc = d.lib.vsmp_bsampler_adjust_rows(d._h, xd.data_ptr(), 0, n, n, None, slots, pens.data_ptr(), 1, prompt.data_ptr(), None, None,
+                                         None, None, 0, 0, None, out.data_ptr(), n, left.data_ptr(),
+                                         torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    want = x.copy()
+    rows = np.where(np.arange(slots) % 9 < 7)[0]  # the last id is not the prompt's
+    want[rows, said[-1][rows]] -= np.float32(0.75)
+    assert np.array_equal(out.cpu().numpy(), want) and (left == n).all()
