@@ -18,8 +18,9 @@
 //
 // What bounds it: few rows read their weights and scales once from HBM (1 x 128,256 x 4,096 in groups of 32: 57 us,
 // 5.2 TB/s; 4 x 151,936 x 2,048: 33 us, 5.0 TB/s); small hidden sizes the launch, the staging of x and the few units a
-// wave has (1 x 151,936 x 896: 24 us, 3.3 TB/s); many rows the conversions, the scaling and the LDS reads beside
-// the MFMAs (64 x 151,936 x 2,048: 91 us, 440 TFLOP/s).
+// wave has (1 x 151,936 x 896: 25 us, 3.3 TB/s); more rows the staging of x too, a round trip for each 16-byte piece
+// of a thread (16 x 128,256 x 4,096: 64 us, 4.4 TB/s), and many rows the conversions, the scaling and the LDS reads
+// beside the MFMAs (64 x 151,936 x 2,048: 93 us, 428 TFLOP/s).
 //
 // k_head_q4 takes hidden sizes from 256 on, k_head_q4_tile the smaller ones.
 #include <algorithm>
@@ -257,8 +258,9 @@ constexpr int few_waves(int rt, int group, bool zp, int st) {
 // flight, across the end of a pair too (the last units are loaded again there and their products dropped). The
 // last unit ends at D: it overlaps the one before where D is no multiple of 256, and x is zero there.
 //
-// A unit of a column is one line of 128 bytes, which eight neighbouring lanes load, so that a load touches 8 lines;
-// loaded as the products need them, 16 bytes of a column in lanes 16 apart, every 16 lanes touch 16 lines, and the
+// A unit of a column is 128 bytes, which eight neighbouring lanes load: one line where ldq is a multiple of 128, so
+// that a load touches 8 lines (up to 16 where it is not, as for hidden sizes of 896 and 576). Loaded as the products
+// need them, 16 bytes of a column in lanes 16 apart, every 16 lanes touch 16 lines, and the
 // weights' stream alone was 1.2 to 1.3 times as long (1 x 128,256 x 4,096 70.6 against 56.8 us, 4 x 151,936 x 2,048
 // 42.1 / 33.0, timing only). The lanes exchange them through LDS of the wave's own; piece p of column c lies at
 // p ^ c, so that neither side meets a bank twice. Scales and zero points of a unit are loaded with it, a column's
@@ -588,9 +590,9 @@ void launch_tile(const HeadQ4Args& a, hipStream_t st) {
 }
 
 // The rows of a workgroup: the fewest of 4, 16 and 32 that hold the batch; for larger ones 64, or 32 where the x of
-// 32 rows fits whole and that of 64 does not (64 x 151,936 x 2,048 100 us in two groups of 32 against 115 in chunks of
-// 64; where neither fits, 40 x 128,256 x 4,096 164 / 121 and 64 rows 261 / 214; 24 rows of 4,096 in chunks of 32 90 us
-// against 120 in two groups of 16).
+// 32 rows fits whole and that of 64 does not (64 x 151,936 x 2,048 93 us in two groups of 32 against 125 in chunks of
+// 64; where neither fits, 40 x 128,256 x 4,096 170 / 131 and 64 rows 200 / 164; where both do, 64 x 151,936 x 1,024 53 /
+// 45; 24 rows of 4,096 in chunks of 32 91 us against 123 in two groups of 16).
 template <bool H, int G>
 void launch_group(const HeadQ4Args& a, int cus, hipStream_t st) {
   if (a.D < 256) {

@@ -73,10 +73,11 @@ constexpr uint32_t kSeen = 0x80000000u;  // a slot's mark of a prompt id; the bi
 // flight while the lists are read. An element without a mark costs its LDS read alone. Logits of four
 // that the mask forbids are not read.
 //
-// Bound by the logits' read and the output's write: 512 x 128,256 f16 without histories 73 us (5.4 TB/s), 256 x
-// 151,936 fp32 54 us (5.8 TB/s), with 512 ids of history a row 56 us. Histories are read by every part of their row:
-// 512 x 128,256 with 5,000 ids a row 79 us. 64 x 151,936 with 40 tokens allowed a row 16.0 us, 20.2 where forbidden
-// logits are read too.
+// Many rows are bound by the logits' read and the output's write: 512 x 128,256 f16 without histories 74 us
+// (5.3 TB/s), 256 x 151,936 fp32 53 us (5.8 TB/s), with 512 ids of history a row 55 us. Histories are read by every
+// part of their row: 512 x 128,256 f16 with 5,000 ids a row 104 us. Few rows are bound by loads that follow one
+// another: mask row, mask words, logits, penalties and offsets, ids, biases. 64 x 151,936 with 40 tokens allowed a
+// row 16.0 us, 20.2 where forbidden logits are read too.
 template <class E, bool BIAS>
 __global__ __launch_bounds__(kNt) void k_adjust(AdjustArgs a) {
   __shared__ __align__(16) uint32_t s_cnt[kAdjustParts];
@@ -303,8 +304,9 @@ __device__ __forceinline__ float next_up(float v) {
 }
 
 // One part of a row, a step of four 16-byte groups per thread at a time, the next step's in flight while one
-// is summed. Bound by the logits' read where there are many: 2,048 x 128,256 bf16 83 us without ids (6.3 TB/s), 86 us
-// with one id a row; few rows by latencies and the parts' hand-off: one row of 151,936 fp32 4.1 us, with 20 ids 6.6.
+// is summed. Bound by the logits' read where there are many: 2,048 x 128,256 bf16 84 us without ids (6.3 TB/s), 83 to
+// 96 us with one id a row (the likeliest, any); few rows by latencies and the parts' hand-off: one row of 151,936 fp32
+// 4.2 us, with its 20 likeliest ids 6.8.
 //
 // Ranks: a wave keeps the asked ids' logits one in a lane and counts, per step, the logits before each. Only ids
 // that the step's largest logit reaches can gain, and the ids that are asked for are mostly the likeliest, so
@@ -312,7 +314,9 @@ __device__ __forceinline__ float next_up(float v) {
 // four rows' maxima) are listed in LDS and compared one by one with all ids above that line at once; the ids
 // below it are taken one by one, each compared with all of the step's logits. The latter takes one comparison
 // and one addition per logit: where ties do not matter, v >= t before the id and v >= the next float above t
-// after it. They matter in the id's own group, whose equal logits before the id the id's lane counts first.
+// after it. They matter in the id's own group, whose equal logits before the id the id's lane counts first. An id
+// that is not among the likeliest so costs a pass over nearly every step: 21 ids anywhere in 2,048 x 128,256 517 us, the
+// 20 likeliest 97.
 template <class E>
 __global__ __launch_bounds__(kNt) void k_logprobs(LogprobArgs a) {
   constexpr int N = 16 / E::kSize, G = 4;  // elements per group, groups per step
@@ -384,7 +388,10 @@ __global__ __launch_bounds__(kNt) void k_logprobs(LogprobArgs a) {
 #pragma unroll
       for (int k = 0; k < N; ++k) s += exp_rel(v[g][k], rel);
     z = {m, s};
-    if (e0 == lo) take_ids();  // after the first step's sums: the ids' logits were loaded behind it
+    // After the first step's sums, which do not wait for the ids' logits. (Those logits' loads do wait for the first
+    // step's: the row's end makes the latter conditional, and a wait for the ids cannot count past them; in fp32 the
+    // compiled code waits for each of the four in its branch.)
+    if (e0 == lo) take_ids();
     if (!a.rank) continue;
     float rm = mx;  // the largest of each row of 16 lanes
     rm = fmaxf(rm, ror<8>(rm));
