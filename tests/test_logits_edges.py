@@ -515,3 +515,23 @@ def test_every_slot_without_a_slot_list():
     rows = np.where(np.arange(slots) % 9 < 7)[0]  # the last id is not the prompt's
     want[rows, said[-1][rows]] -= np.float32(0.75)
     assert np.array_equal(out.cpu().numpy(), want) and (left == n).all()
+
+
+def test_a_stream_is_known_by_its_address(ctx):
+    """Every call takes any object that has a stream's address, whether it allocates its output or not."""
+    import types
+
+    import torch
+
+    x, ids = torch.randn(3, 5000, device="cuda"), torch.zeros(3, 2, dtype=torch.int32, device="cuda")
+    side = torch.cuda.Stream()
+    bare = types.SimpleNamespace(cuda_stream=side.cuda_stream)
+    calls = [lambda st: ctx.adjust_logits(x, stream=st), lambda st: ctx.logprobs(x, ids, stream=st)[0],
+             lambda st: ctx.pick_batch(x[:, :5000], V.Params(temp=0.0), stream=st)]
+    for call in calls:
+        want = call(None)
+        torch.cuda.synchronize()
+        for st in (bare, side, torch.cuda.default_stream(), torch.cuda.current_stream()):
+            got = call(st)
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)

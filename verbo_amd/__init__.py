@@ -313,7 +313,7 @@ class _Torch:
         self.codes = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # vsmp_dtype
         self._raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         self._current = torch.cuda.current_stream
-        self._use = torch.cuda.stream
+        self._use, self._external = torch.cuda.stream, torch.cuda.ExternalStream
 
     def stream(self, stream, device):
         """The address of `stream`, or of torch's current one on `device`."""
@@ -327,7 +327,8 @@ class _Torch:
         the memory waits for the work of both."""
         if stream is None or stream.cuda_stream == self.stream(None, device):
             return self.empty(shape, dtype=dtype, device=device)
-        with self._use(stream):
+        # by its address: of a stream, the calls ask for no more than that
+        with self._use(self._external(stream.cuda_stream, device=device)):
             t = self.empty(shape, dtype=dtype, device=device)
         t.record_stream(self._current(device))
         return t
