@@ -535,3 +535,25 @@ def test_a_stream_is_known_by_its_address(ctx):
             got = call(st)
             torch.cuda.synchronize()
             assert torch.equal(got, want)
+
+
+def test_serve_follows_a_penalty_that_changes():
+    """A request's penalty and prompt length changed between steps, in place or replaced, hold from the next pick on."""
+    import torch
+
+    n = 12
+    base = torch.linspace(3.0, 0.0, n, device="cuda")
+    req = decode.Request([0], decode.Opts(max_tokens=6, temp=0.0), repeat_last=0, penalty=V.Penalty(presence=9.0))
+
+    def logits(js, steps, last):
+        if steps[0] == 2:
+            req.penalty.presence = 0.0
+        if steps[0] == 4:
+            req.penalty = V.Penalty(presence=9.0)
+        if steps[0] == 5:
+            req.prompt_len = 1
+        return base.expand(1, n).contiguous()
+
+    toks, _ = decode.BatchDecoder.with_slots(1, n).serve([req], logits)[0]
+    # 0 is the prompt; 1 and 2 penalised apart from it; nothing penalised; 0, 1 and 2 penalised; 0 said by itself too
+    assert toks == [1, 2, 0, 0, 3, 4]

@@ -246,7 +246,7 @@ class BatchDecoder:
         stopped = [False] * len(requests)
         steps = [0] * len(requests)
         last = [-1] * len(requests)
-        held, pens, own = None, None, None  # the requests whose penalties and prompt lengths are on the device
+        held, pens, own = None, None, None  # the requests, penalties and prompt lengths that are on the device
         self.schedule = []
         step = 0
         while queue or live:
@@ -266,10 +266,11 @@ class BatchDecoder:
             rows = torch.tensor(slots, dtype=torch.int32, device=dev)
             lg = logits_fn(reqs, [steps[j] for j in reqs], [last[j] for j in reqs])
             if any(requests[j].penalty is not None for j in reqs):
-                if reqs != held:
-                    pens = to_device_penalties([requests[j].penalty or Penalty() for j in reqs], dev)
-                    own = torch.tensor([requests[j].prompt_len for j in reqs], dtype=torch.int32, device=dev)
-                    held = reqs
+                now = _penalty_rows([requests[j].penalty or Penalty() for j in reqs])
+                lens = [requests[j].prompt_len for j in reqs]
+                if (reqs, now.tobytes(), lens) != held:  # by value: a caller may change a request as it goes
+                    pens, own = to_device_penalties(now, dev), torch.tensor(lens, dtype=torch.int32, device=dev)
+                    held = reqs, now.tobytes(), lens
                 lg = self.adjust_rows(lg, rows, pens, prompt_len=own, stream=stream)
             self.pick_rows(lg, rows, out[:len(slots)], stream)
             self.schedule.append(list(zip(reqs, slots)))
