@@ -15,16 +15,24 @@ The operators around the pick (include/vsmp_logits.h):
     x = ctx.adjust_logits(x, Penalty(presence=.5), hist=h, hist_off=o, mask=m, out=x, left=left)
     ids = ctx.pick_batch(x, Params(temp=.8, top_k=50))
     logprob, rank, lse = ctx.logprobs(x, ids[:, None])
+
+Beams and the states behind them (include/vsmp_beam.h):
+
+    step = ctx.beam_select(logits, scores, n, stop_ids=(2,))        # logits: cuda [G * W, V], scores: cuda [G, W]
+    ctx.reorder_rows(Planes(caches, token_dim=2), step.parent, n)   # caches: cuda [rows, heads, tokens, width] each
+    pages, ok = ctx.pages_step(pages, step.parent, add=1, cache=Planes(pools, token_dim=1))
+    pages, moved, live = ctx.pages_compact(pages, cache=Planes(pools, token_dim=1))
 """
 import ctypes
 import os
+from collections import namedtuple
 from pathlib import Path
 
 import numpy as np
 
 from .workloads import SAMPLING_DTYPE
 
-__all__ = ["Context", "Sampler", "Params", "Penalty", "PENALTY_DTYPE", "RowInfo", "Debug", "VsmpError", "pick_batch_noalloc", "load_library", "U_SUPPLIED", "U_COUNTER",
+__all__ = ["Context", "Sampler", "Params", "Penalty", "PENALTY_DTYPE", "BeamStep", "Planes", "Pages", "RowInfo", "Debug", "VsmpError", "pick_batch_noalloc", "load_library", "U_SUPPLIED", "U_COUNTER",
            "U_XORSHIFT", "ROW_INFO_DTYPE", "SAMPLING_DTYPE"]
 __version__ = "0.1.0"
 
@@ -96,6 +104,22 @@ class Debug(ctypes.Structure):
         ("cand_cap", ctypes.c_int),
         ("pen_bits", ctypes.c_void_p),
     ]
+
+
+class _PlanesArg(ctypes.Structure):
+    """vsmp_planes."""
+
+    _fields_ = [("planes", ctypes.c_void_p), ("n_planes", ctypes.c_int), ("rows", ctypes.c_int),
+                ("row_stride", ctypes.c_longlong), ("pieces", ctypes.c_int), ("piece_stride", ctypes.c_longlong),
+                ("tokens", ctypes.c_int), ("token_bytes", ctypes.c_int)]
+
+
+class _PagesArg(ctypes.Structure):
+    """vsmp_pages."""
+
+    _fields_ = [("rows", ctypes.c_int), ("row_pages", ctypes.c_int), ("n_pages", ctypes.c_int),
+                ("page_tokens", ctypes.c_int), ("table", ctypes.c_void_p), ("ldt", ctypes.c_longlong),
+                ("lens", ctypes.c_void_p), ("ref", ctypes.c_void_p)]
 
 
 ROW_INFO_DTYPE = np.dtype([("id", "i4"), ("path", "i4"), ("k", "i4"), ("keep_minp", "i4"), ("keep", "i4"),
@@ -171,6 +195,12 @@ def load_library():
         "vsmp_head_logits_q4": (ctypes.c_int, [_P, _P, ctypes.c_int, ctypes.c_longlong, _P, ctypes.c_longlong, _P,
                                                ctypes.c_int, ctypes.c_longlong, _P, ctypes.c_longlong, ctypes.c_int,
                                                ctypes.c_int, ctypes.c_int, ctypes.c_int, _P, ctypes.c_longlong, _P]),
+        "vsmp_beam_select": (ctypes.c_int, [_P, _P, ctypes.c_int, ctypes.c_longlong, ctypes.c_int, ctypes.c_int,
+                                            ctypes.c_int, _P, ctypes.c_int, _P, ctypes.c_int, _P, _P, _P, _P, _P, _P,
+                                            _P, _P]),
+        "vsmp_reorder_rows": (ctypes.c_int, [_P, _P, _P, ctypes.c_int, _P, _P]),
+        "vsmp_pages_step": (ctypes.c_int, [_P, _P, _P, _P, _P, ctypes.c_int, _P, _P, _P]),
+        "vsmp_pages_compact": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -442,6 +472,110 @@ def _adjust_args(logits, penalty, hist, hist_off, prompt_len, bias_ids, bias, bi
     return (logits.data_ptr(), code, ld), (B, V), (pp, per_row), (h, ho), rest, out
 
 
+BeamStep = namedtuple("BeamStep", "token parent score end_token end_parent end_score n_end")
+BeamStep.__doc__ = """What Context.beam_select returns: for each group the n best continuations that go on (token, parent: the
+row, both int32 [G, n]; score: float32 [G, n]) and those that a stop token ends (the same, n_end of them: int32 [G])."""
+
+
+class Planes:
+    """vsmp_planes: device tensors of one shape, strides and type whose rows (dimension 0) hold tokens, such as the keys
+    and values of every layer; kept by a program beside them. token_dim: the dimension that counts tokens, with a
+    token's values side by side behind it and whole tokens one after the other; None: a row is one token, whole.
+    Dimensions before it must have one stride in common (heads that lie apart)."""
+
+    def __init__(self, tensors, token_dim=None):
+        import torch
+
+        self.tensors = list(tensors)
+        if not self.tensors:
+            raise VsmpError("planes need at least one tensor")
+        t = self.tensors[0]
+        if not t.is_cuda or t.dim() < 1 or t.numel() == 0:
+            raise VsmpError("planes must be device tensors with at least one row and element")
+        for u in self.tensors:
+            if u.shape != t.shape or u.stride() != t.stride() or u.dtype != t.dtype or u.device != t.device:
+                raise VsmpError("planes must have one shape, one type, the same strides and one device")
+        size, n = t.element_size(), t.dim()
+        dim = None if token_dim is None else int(token_dim) + (n if token_dim < 0 else 0)
+        if dim is not None and not 1 <= dim < n:
+            raise VsmpError("token_dim must be a dimension of the planes behind the first")
+
+        def together(dims):
+            """(entries, stride) of dimensions that one stride walks through; None if none does."""
+            dims = [(k, d) for k, d in dims if k > 1]
+            if any(a[1] != b[0] * b[1] for a, b in zip(dims, dims[1:])):
+                return None
+            count = 1
+            for k, _ in dims:
+                count *= k
+            return count, dims[-1][1] if dims else 0
+
+        shape, stride = t.shape, t.stride()
+        dims = list(zip(shape, stride))
+        cut = dim + 1 if dim is not None else n
+        if dim is None:  # as many of the last dimensions as lie side by side
+            width = 1
+            while cut > 1 and (shape[cut - 1] == 1 or stride[cut - 1] == width):
+                cut -= 1
+                width *= shape[cut]
+            tokens, token = 1, width
+            inner, outer = (width, 1), together(dims[1:cut])
+        else:
+            inner = together(dims[cut:])
+            tokens, token = shape[dim], inner[0] if inner else 0
+            outer = together(dims[1:dim])
+        if inner is None or (inner[0] > 1 and inner[1] != 1) or (tokens > 1 and stride[dim] != token):
+            raise VsmpError("a token's values must lie side by side, and tokens one after the other")
+        if outer is None:
+            raise VsmpError("the dimensions before the tokens must have one stride in common")
+        self.device, self.rows, self.tokens, self.token_dim = t.device, shape[0], tokens, dim
+        self._ptrs = torch.tensor([u.data_ptr() for u in self.tensors], dtype=torch.int64).to(t.device)
+        # the addresses are there for every stream from here on
+        torch.cuda.current_stream(t.device).synchronize()
+        self._arg = _PlanesArg(self._ptrs.data_ptr(), len(self.tensors), shape[0], stride[0] * size if shape[0] > 1 else 0, outer[0],
+                               outer[1] * size, tokens, token * size)
+        self._addr = ctypes.addressof(self._arg)
+
+
+class Pages:
+    """vsmp_pages: a cache in pages as its rows use it. table: int32 [rows, row_pages], a row's page numbers (contiguous
+    rows); lens: int32 [rows], its tokens; ref: int32 [n_pages], how many hold each page; page_tokens: tokens of a page.
+    The tensors are the program's; Context.pages_step and pages_compact read one such state and write another."""
+
+    def __init__(self, table, lens, ref, page_tokens):
+        T = _t()
+        dev = table.device
+        if table.dtype != T.int32 or table.dim() != 2 or not table.is_cuda or (table.shape[1] > 1 and table.stride(1) != 1):
+            raise VsmpError("table must be a 2-D int32 device tensor with contiguous rows")
+        rows, cap = table.shape
+        for t, name in ((lens, "lens"), (ref, "ref")):
+            if t.dim() != 1:
+                raise VsmpError(f"{name} must be one-dimensional")
+            _array_of(t, T.int32, rows if name == "lens" else 1, name, dev)
+        if lens.numel() != rows:
+            raise VsmpError("lens must hold an entry for each row of the table")
+        self.table, self.lens, self.ref, self.page_tokens, self.device = table, lens, ref, int(page_tokens), dev
+        self._arg = _PagesArg(rows, cap, ref.numel(), self.page_tokens, table.data_ptr(), table.stride(0) if rows > 1 else cap,
+                              lens.data_ptr(), ref.data_ptr())
+        self._addr = ctypes.addressof(self._arg)
+
+    @classmethod
+    def empty(cls, rows, row_pages, n_pages, page_tokens, device="cuda"):
+        """A pool of free pages, and rows without tokens."""
+        import torch
+
+        return cls(torch.full((rows, row_pages), -1, dtype=torch.int32, device=device), torch.zeros(rows, dtype=torch.int32, device=device),
+                   torch.zeros(n_pages, dtype=torch.int32, device=device), page_tokens)
+
+    def like(self, rows=None, stream=None):
+        """Memory for a state of this pool, of as many rows or of `rows`: what a step writes into. `stream`: that of the
+        step."""
+        T = _t()
+        n = self.lens.numel() if rows is None else int(rows)
+        return Pages(T.output((n, self.table.shape[1]), T.int32, self.device, stream), T.output((n,), T.int32, self.device, stream),
+                     T.output((self.ref.numel(),), T.int32, self.device, stream), self.page_tokens)
+
+
 class Context:
     """A vsmp_ctx on one device: scratch for batched picks, staging for host picks."""
 
@@ -612,6 +746,95 @@ class Context:
                                     group, B, V, D, logits.data_ptr(), ldl, T.stream(stream, dev)) != 0:
             raise _err()
         return logits
+
+    def beam_select(self, logits, scores, n=None, stop_ids=(), stream=None):
+        """vsmp_beam_select: one step of beam search. logits: device [G * W, V] (float32, bfloat16 or float16; rows
+        contiguous), the rows of a group one after the other; scores: float32 [G, W], -inf for a row that is not live;
+        n: beams of the next step (default W); stop_ids: at most 16 tokens that end a sequence. Returns a BeamStep."""
+        T = _t()
+        self._check_device(logits)
+        dev = logits.device
+        code, ld = _rows_of(logits, "logits", dev)
+        B, V = logits.shape
+        if scores.dim() != 2 or scores.numel() != B:
+            raise VsmpError("scores must be a float32 tensor [G, W] with an entry for each row of logits")
+        G, W = scores.shape
+        n = W if n is None else int(n)
+        if n < 1:
+            raise VsmpError("need n >= 1 beams of the next step")
+        stops = (ctypes.c_int * len(stop_ids))(*stop_ids) if len(stop_ids) else None
+        sp = _array_of(scores, T.float32, B, "scores", dev)
+        # one allocation for what the step returns: the n-wide arrays one after the other, then the counts
+        k = G * n
+        buf = T.output((6 * k + G,), T.int32, dev, stream)
+        at = [buf[i * k:(i + 1) * k].view(G, n) for i in range(6)]
+        out = BeamStep(at[0], at[1], at[2].view(T.float32), at[3], at[4], at[5].view(T.float32), buf[6 * k:])
+        p = buf.data_ptr()
+        if _lib.vsmp_beam_select(self._h, logits.data_ptr(), code, ld, G, W, V, sp, n, stops, len(stop_ids), p, p + 4 * k, p + 8 * k,
+                                 p + 12 * k, p + 16 * k, p + 20 * k, p + 24 * k, T.stream(stream, dev)) != 0:
+            raise _err()
+        return out
+
+    def reorder_rows(self, planes, parent, width, lens=None, stream=None):
+        """vsmp_reorder_rows: in every plane of `planes` (a Planes) row i takes what row parent[i] held, in place. parent:
+        int32 [rows], row numbers within each group of `width` rows; others leave their row as it is. lens: int32
+        [rows], the tokens that each row held before; None: all."""
+        T = _t()
+        dev = planes.device
+        if self.device >= 0 and dev.index != self.device:
+            raise VsmpError(f"expected tensors on the context's device ({self.device})")
+        if _lib.vsmp_reorder_rows(self._h, planes._addr, _array_of(parent, T.int32, planes.rows, "parent", dev), int(width),
+                                  _array_of(lens, T.int32, planes.rows, "lens", dev), T.stream(stream, dev)) != 0:
+            raise _err()
+
+    def _pages(self, pages, cache):
+        dev = pages.device
+        if self.device >= 0 and dev.index != self.device:
+            raise VsmpError(f"expected tensors on the context's device ({self.device})")
+        if cache is not None and cache.device != dev:
+            raise VsmpError("the cache must be on the pages' device")
+        return dev, cache._addr if cache is not None else None
+
+    def pages_step(self, pages, parent=None, add=0, cache=None, out=None, stream=None):
+        """vsmp_pages_step: the step of a cache in pages from the state `pages` (a Pages, left as it is). Row i takes the
+        pages of row parent[i] (int32, one for each row of the next state; None: its own; outside the rows: none) and
+        grows by add[i] tokens, or is cut by -add[i] (an int32 tensor, or an int for every row). cache: a Planes whose
+        rows are the pages, so that begun pages which rows share are copied; None: tables alone. out: a Pages for the
+        next state (default: new, a row for each parent). Returns (the next state, ok int32 [rows]: 0 for a row that
+        did not get its pages)."""
+        T = _t()
+        dev, cp = self._pages(pages, cache)
+        if out is None:
+            out = pages.like(None if parent is None else parent.numel(), stream)
+        rows = out.lens.numel()
+        every = 0
+        if isinstance(add, int):
+            add, every = None, add
+        if parent is None and add is None and rows != pages.lens.numel():
+            raise VsmpError("without parents the next state has the rows of this one")
+        ok = T.output((rows,), T.int32, dev, stream)
+        if out.device != dev:
+            raise VsmpError("out must be on the pages' device")
+        if _lib.vsmp_pages_step(self._h, pages._addr, out._addr, _array_of(parent, T.int32, rows, "parent", dev),
+                                _array_of(add, T.int32, rows, "add", dev), every, cp, ok.data_ptr(), T.stream(stream, dev)) != 0:
+            raise _err()
+        return out, ok
+
+    def pages_compact(self, pages, cache=None, out=None, stream=None):
+        """vsmp_pages_compact: the pages in use moved together into the pool's first, from the state `pages` (left as it
+        is), in every plane of `cache`. Returns (the next state: `out`, or a new Pages; moved int32 [n_pages]: each
+        page's new number, -1 for a free one; live int32 [1]: how many are in use)."""
+        T = _t()
+        dev, cp = self._pages(pages, cache)
+        if out is None:
+            out = pages.like(stream=stream)
+        if out.device != dev:
+            raise VsmpError("out must be on the pages' device")
+        n = pages.ref.numel()
+        moved, live = T.output((n,), T.int32, dev, stream), T.output((1,), T.int32, dev, stream)
+        if _lib.vsmp_pages_compact(self._h, pages._addr, out._addr, cp, moved.data_ptr(), live.data_ptr(), T.stream(stream, dev)) != 0:
+            raise _err()
+        return out, moved, live
 
     def read_probe(self, t, stream=None):
         """vsmp_read_probe: stream the bytes of device tensor `t` through a plain read kernel on

@@ -16,7 +16,8 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libvsmp.so"
-SOURCES = ["vsmp_kernels.hip", "vsmp_head.hip", "vsmp_logits.hip", "vsmp_head_q4.hip", "vsmp_api.cpp", "vsmp_logits_api.cpp",
+SOURCES = ["vsmp_kernels.hip", "vsmp_head.hip", "vsmp_logits.hip", "vsmp_head_q4.hip", "vsmp_beam.hip", "vsmp_states.hip",
+           "vsmp_api.cpp", "vsmp_logits_api.cpp", "vsmp_beam_api.cpp",
            "sampler.cpp", "decode.cpp"]
 ARCH = os.environ.get("VSMP_OFFLOAD_ARCH", "gfx950")
 

@@ -17,6 +17,7 @@
 #include "vsmp_common.hpp"
 #include "vsmp_error.hpp"
 #include "vsmp_internal.hpp"
+#include "vsmp_beam.hpp"
 #include "vsmp_logits.hpp"
 
 namespace vsmp {
@@ -143,6 +144,11 @@ struct vsmp_ctx {
   // the operators around the pick (ops_scratch): one allocation of a fixed size, its tickets zero between calls
   unsigned char* o_scr = nullptr;
   size_t n_oscr = 0;
+  // beams and a cache in pages (beam_scratch, page_scratch): likewise
+  unsigned char* b_scr = nullptr;
+  size_t n_bscr = 0;
+  unsigned char* c_scr = nullptr;
+  size_t n_cscr = 0;
   // host-pointer path (vsmp_pick_host): one pinned host area, mapped into the device's address
   // space (hs_dev), holding the row, the history, its offsets and the draw, then the id and the row
   // diagnostics: the kernels read their inputs from it and write their results into it, with no
@@ -905,6 +911,52 @@ bool ops_warm(vsmp_ctx* c, hipStream_t st) {
   return c->o_scr || capturing(st) || ops_scratch(c, st, &s);
 }
 
+// One allocation of `bytes` as p, zeroed on `st` by the call that makes it.
+static bool fixed_scratch(unsigned char*& p, size_t& cap, size_t bytes, hipStream_t st) {
+  if (!p && capturing(st)) {
+    set_error("vsmp: the context has no scratch for this operator yet: issue the call once before capturing it");
+    return false;
+  }
+  return grow(p, cap, bytes, true, "scratch", st);
+}
+
+bool beam_scratch(vsmp_ctx* c, hipStream_t st, BeamScratch* out) {
+  constexpr size_t kTick = sizeof(unsigned) * kBeamPad * kBeamSlots, kKey = sizeof(unsigned long long) * kBeamMax * kBeamSlots,
+                   kSum = sizeof(double) * kBeamSlots, kMax = sizeof(float) * kBeamSlots;
+  if (!fixed_scratch(c->b_scr, c->n_bscr, kTick + kKey + kSum + kMax, st)) return false;
+  out->tick = reinterpret_cast<unsigned*>(c->b_scr);
+  out->key = reinterpret_cast<unsigned long long*>(c->b_scr + kTick);
+  out->sum = reinterpret_cast<double*>(c->b_scr + kTick + kKey);
+  out->max = reinterpret_cast<float*>(c->b_scr + kTick + kKey + kSum);
+  return true;
+}
+
+bool page_scratch(vsmp_ctx* c, hipStream_t st, PageScratch* out) {
+  unsigned char* at = nullptr;
+  auto take = [&at](auto*& p, size_t n) {
+    p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(at);
+    at += (n * sizeof(*p) + 127) & ~size_t{127};
+  };
+  auto lay = [&] {
+    take(out->delta, kPagesMax);
+    take(out->writers, kPagesMax);
+    take(out->order, kPagesMax);
+    take(out->bits, kPagesMax / 64);
+    take(out->before, kPagesMax / 64 + 1);
+    take(out->moves, kPagesMax);
+    take(out->room, kPagesMax);
+    take(out->copies, kPageRows);
+    take(out->n_copies, 1);
+    take(out->tick, 1);
+  };
+  lay();
+  const size_t bytes = reinterpret_cast<uintptr_t>(at);
+  if (!fixed_scratch(c->c_scr, c->n_cscr, bytes, st)) return false;
+  at = c->c_scr;
+  lay();
+  return true;
+}
+
 // A stream passed with a context must belong to the context's device (its scratch lives there).
 bool stream_on_device(const vsmp_ctx* c, hipStream_t st) {
   if (!c || !st) return true;  // a null context is rejected by the call; the null stream is the device's own
@@ -962,7 +1014,8 @@ void vsmp_ctx_free(vsmp_ctx* c) {
   (void)hipDeviceSynchronize();
   void* bufs[] = {c->x_flag, c->x_u,    c->x_buf,    c->s_cand, c->s_cnt,   c->s_npen,   c->s_max,
                   c->s_min,  c->s_bits, c->g_rows,   c->t_scr,  c->h_probe,  c->h_full,
-                  c->h_tk,   c->h_rmode, c->h_rcand, c->h_rcnt, c->p_scr, c->o_scr};
+                  c->h_tk,   c->h_rmode, c->h_rcand, c->h_rcnt, c->p_scr, c->o_scr,
+                  c->b_scr,  c->c_scr};
   for (void* p : bufs)
     if (p) (void)hipFree(p);
   for (unsigned char* h : c->hs_host)

@@ -64,6 +64,12 @@ bool ops_scratch(vsmp_ctx* c, hipStream_t st, OpScratch* out);
 // need none themselves but are promised to bring it. false (error set) when it could not be allocated.
 bool ops_warm(vsmp_ctx* c, hipStream_t st);
 
+// The scratch of vsmp_beam_select, and that of vsmp_pages_step and vsmp_pages_compact (vsmp_beam.hpp), as ops_scratch's.
+struct BeamScratch;
+struct PageScratch;
+bool beam_scratch(vsmp_ctx* c, hipStream_t st, BeamScratch* out);
+bool page_scratch(vsmp_ctx* c, hipStream_t st, PageScratch* out);
+
 // vsmp_adjust_logits's argument checks, and its work for arguments that pass them: rows with histories of
 // their own (hist_off with B + 1 entries) or, with hist_len, with sequences' regions (see pick_batch).
 // pen_per_row: pen is a device array of B. Both return 0 or -1 (error set).

@@ -1,0 +1,460 @@
+// States that follow their beams: rows of planes moved in place (k_reorder), and a cache in pages: a step's forks,
+// cuts and growth (k_pages_fork, k_pages_take, k_page_copy) and compaction (k_pages_scan, k_pages_pair, k_pages_move).
+#include <algorithm>
+
+#include "vsmp_beam.hpp"
+
+namespace vsmp {
+namespace {
+
+constexpr int kNt = 256;
+
+template <class T>
+__device__ __forceinline__ T agent_load(const T* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <class T>
+__device__ __forceinline__ void agent_store(T* p, T v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <class T>
+__device__ __forceinline__ T agent_add(T* p, T v) {
+  return __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// idx / n, with m = (2^32 - 1) / n: m n >= 2^32 - n, so that idx m / 2^32 is less than one below idx / n.
+__device__ __forceinline__ uint32_t divide(uint32_t idx, uint32_t n, uint32_t m) {
+  const uint32_t q = __umulhi(idx, m);
+  return idx - q * n >= n ? q + 1 : q;
+}
+
+// ---- k_reorder -------------------------------------------------------------------------------------------
+
+// A column of B bytes over a group's rows belongs to one thread, which loads it from every parent before it stores it in
+// any row: in place without a wait. Rows that stay are neither read nor written for themselves; a parent with several
+// children is read by each of their loads, from memory once.
+template <int MAXW, int B>
+__global__ __launch_bounds__(kNt) void k_reorder(ReorderArgs a) {
+  typedef uint32_t vec __attribute__((ext_vector_type(B / 4), aligned(1)));
+  __shared__ long long s_from[MAXW], s_to[MAXW];  // of the rows that move: where their parents and they lie in a plane
+  __shared__ int s_bytes[MAXW];                   // and what they take of each piece
+  __shared__ int s_n, s_most, s_least;
+  const int tid = threadIdx.x, first = a.row0 + static_cast<int>(blockIdx.y) * a.width;
+  if (tid < 64) {
+    int p = tid, bytes = 0;
+    if (tid < a.width) {
+      p = a.parent[first + tid] - first;
+      if (p != tid && static_cast<unsigned>(p) < static_cast<unsigned>(a.width))
+        bytes = (a.len ? min(max(a.len[first + p], 0), a.p.tokens) : a.p.tokens) * a.p.token_bytes;
+    }
+    const unsigned long long moves = __ballot(bytes > 0);
+    int most = bytes, least = bytes > 0 ? bytes : 0x7FFFFFFF;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+      most = max(most, __shfl_xor(most, d));
+      least = min(least, __shfl_xor(least, d));
+    }
+    if (bytes > 0) {
+      const int k = __popcll(moves & ((1ull << tid) - 1ull));
+      s_from[k] = (first + p) * a.p.row_stride;
+      s_to[k] = (first + tid) * a.p.row_stride;
+      s_bytes[k] = bytes;
+    }
+    if (tid == 0) {
+      s_n = __popcll(moves);
+      s_most = most;
+      s_least = least;
+    }
+  }
+  __syncthreads();
+  const int n = s_n;
+  if (n == 0) return;
+  const uint32_t cols = (static_cast<uint32_t>(s_most) + B - 1) / B, m = 0xFFFFFFFFu / cols, least = static_cast<uint32_t>(s_least);
+  const uint32_t pieces = static_cast<uint32_t>(a.p.pieces), mp = 0xFFFFFFFFu / pieces;
+  const uint32_t total = static_cast<uint32_t>(a.p.n_planes) * pieces * cols;
+  for (uint32_t idx = blockIdx.x * kNt + tid; idx < total; idx += gridDim.x * kNt) {
+    const uint32_t run = divide(idx, cols, m), at = (idx - run * cols) * B;
+    const uint32_t plane = divide(run, pieces, mp), piece = run - plane * pieces;
+    char* base = static_cast<char*>(a.p.planes[a.plane0 + plane]) + piece * a.p.piece_stride + at;
+    if (at + B <= least) {
+      vec v[MAXW];
+#pragma unroll
+      for (int i = 0; i < MAXW; ++i)
+        if (i < n) v[i] = *reinterpret_cast<const vec*>(base + s_from[i]);
+#pragma unroll
+      for (int i = 0; i < MAXW; ++i)
+        if (i < n) *reinterpret_cast<vec*>(base + s_to[i]) = v[i];
+    } else {  // the end of some row's tokens: byte by byte, each a column of its own
+      for (int k = 0; k < B; ++k) {
+        uint8_t v[MAXW];
+#pragma unroll
+        for (int i = 0; i < MAXW; ++i)
+          if (i < n && at + k < static_cast<uint32_t>(s_bytes[i])) v[i] = *reinterpret_cast<const uint8_t*>(base + k + s_from[i]);
+#pragma unroll
+        for (int i = 0; i < MAXW; ++i)
+          if (i < n && at + k < static_cast<uint32_t>(s_bytes[i])) *reinterpret_cast<uint8_t*>(base + k + s_to[i]) = v[i];
+      }
+    }
+  }
+}
+
+// ---- a cache in pages ------------------------------------------------------------------------------------
+
+struct RowPlan {
+  int src;         // the parent's row in `from`, or -1
+  int len, want;   // tokens taken over, and wanted (len where they do not fit the table)
+  bool fits;
+};
+__device__ __forceinline__ int held(const vsmp_pages& p, int row) {
+  return min(max(p.lens[row], 0), p.row_pages * p.page_tokens);
+}
+__device__ __forceinline__ RowPlan row_plan(const PageArgs& a, int i) {
+  RowPlan r;
+  r.src = a.parent ? a.parent[i] : i;
+  if (r.src < 0 || r.src >= a.from.rows) r.src = -1;
+  r.len = r.src >= 0 ? held(a.from, r.src) : 0;
+  const long long want = max(static_cast<long long>(r.len) + (a.add ? a.add[i] : a.add_all), 0ll);
+  r.fits = want <= static_cast<long long>(a.to.row_pages) * a.to.page_tokens;
+  r.want = r.fits ? static_cast<int>(want) : r.len;
+  return r;
+}
+__device__ __forceinline__ int pages_of(int tokens, int page_tokens) { return (tokens + page_tokens - 1) / page_tokens; }
+__device__ __forceinline__ bool is_page(int p, int n) { return static_cast<unsigned>(p) < static_cast<unsigned>(n); }
+
+// The next tables, as far as pages are taken over; what each page gains in holders; for begun pages the rows that grow in
+// them. Integer atomics, whose order does not matter, where a row's old page and its new one differ: the pages that a
+// row shares with its parent cost none.
+__global__ __launch_bounds__(kNt) void k_pages_fork(PageArgs a) {
+  const int i = blockIdx.x, T = a.to.page_tokens, P = a.to.n_pages;
+  RowPlan r{-1, 0, 0, true};
+  if (i < a.to.rows) r = row_plan(a, i);
+  const int keep = pages_of(min(r.len, r.want), T), had = i < a.from.rows ? pages_of(held(a.from, i), T) : 0;
+  const int* take = a.from.table + max(r.src, 0) * a.from.ldt;
+  const int* old = a.from.table + i * a.from.ldt;
+  int* out = a.to.table + i * a.to.ldt;
+  const int n = i < a.to.rows ? a.to.row_pages : had;
+  for (int j = threadIdx.x; j < n; j += kNt) {
+    const int was = j < had ? old[j] : -1, now = j < keep ? take[j] : -1;
+    if (was != now) {
+      if (is_page(was, P)) agent_add(&a.s.delta[was], -1);
+      if (is_page(now, P)) agent_add(&a.s.delta[now], 1);
+    }
+    if (i < a.to.rows) out[j] = now;
+    if (j == r.len / T && r.want > r.len && r.len % T && is_page(now, P)) {
+      agent_add(&a.s.writers[now], 1);
+      __hip_atomic_fetch_max(&a.s.order[now], static_cast<unsigned long long>(r.len) << 32 | static_cast<uint32_t>(~i), __ATOMIC_RELAXED,
+                             __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+}
+
+constexpr int kTakeNt = 1024;
+constexpr int kTakePages = 4 * kTakeNt;  // pages of a workgroup
+
+// Sum over the workgroup's threads before this one; *total: over all.
+__device__ __forceinline__ int scan_before(int v, int* total) {
+  __shared__ int s_sum[kTakeNt / 64];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  int at = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(at, d);
+    if (lane >= d) at += o;
+  }
+  __syncthreads();
+  if (lane == 63) s_sum[wv] = at;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kTakeNt / 64; ++w) {
+    before += w < wv ? s_sum[w] : 0;
+    all += s_sum[w];
+  }
+  *total = all;
+  return before + at - v;
+}
+
+// The next ref, and the free pages as bits; then, in the last workgroup, what each row needs, the pages it gets, lens,
+// ok and the list of copies.
+__global__ __launch_bounds__(kTakeNt) void k_pages_take(PageArgs a) {
+  __shared__ int s_start[kPageRows];         // pages that the rows before this one ask for
+  __shared__ int s_first[kPageRows];         // where in the table a row's new pages begin
+  __shared__ int s_before[kPagesMax / 64];   // free pages before each word
+  __shared__ int s_last;
+  const int tid = threadIdx.x, lane = tid & 63, P = a.to.n_pages, T = a.to.page_tokens, R = a.to.rows;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int p = blockIdx.x * kTakePages + k * kTakeNt + tid;
+    int ref = 1;
+    if (p < P) {
+      const int d = a.s.delta[p];
+      ref = a.from.ref[p] + d;
+      if (d) a.s.delta[p] = 0;
+      agent_store(&a.to.ref[p], ref);
+    }
+    const unsigned long long is_free = __ballot(ref <= 0);
+    if (lane == 0 && p < P) agent_store(&a.s.bits[p >> 6], is_free);
+  }
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  __syncthreads();
+  if (tid == 0) s_last = agent_add(a.s.tick, 1u) == gridDim.x - 1;
+  __syncthreads();
+  if (!s_last) return;
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  if (tid == 0) agent_store(a.s.tick, 0u);
+
+  // the rows' needs
+  int asked = 0, copies = 0;  // so far
+  int need_[kPageRows / kTakeNt];
+  bool away_[kPageRows / kTakeNt];
+#pragma unroll
+  for (int k = 0; k < kPageRows / kTakeNt; ++k) {
+    need_[k] = 0;
+    away_[k] = false;
+    if (k * kTakeNt >= R) continue;
+    const int i = k * kTakeNt + tid;
+    if (i < R) {
+      const RowPlan r = row_plan(a, i);
+      if (r.want > r.len) {
+        const int q = r.len % T ? a.to.table[i * a.to.ldt + r.len / T] : -1;
+        if (is_page(q, P))
+          away_[k] = agent_load(&a.to.ref[q]) != a.s.writers[q] ||
+                     a.s.order[q] != (static_cast<unsigned long long>(r.len) << 32 | static_cast<uint32_t>(~i));
+        s_first[i] = pages_of(r.len, T) - away_[k];
+        need_[k] = pages_of(r.want, T) - s_first[i];
+      }
+    }
+    int total;
+    const int at = scan_before(need_[k], &total);
+    if (i < R) s_start[i] = asked + at;
+    asked += total;
+  }
+  // how many pages are free, and before each thread's words
+  const int words = (P + 63) / 64, mine = (words + kTakeNt - 1) / kTakeNt;
+  int count = 0;
+  for (int w = tid * mine; w < min(words, (tid + 1) * mine); ++w) count += __popcll(agent_load(&a.s.bits[w]));
+  int n_free;
+  int rank = scan_before(count, &n_free);
+  for (int w = tid * mine; w < min(words, (tid + 1) * mine); ++w) {
+    s_before[w] = rank;
+    rank += __popcll(agent_load(&a.s.bits[w]));
+  }
+#pragma unroll
+  for (int k = 0; k < kPageRows / kTakeNt; ++k) {
+    if (k * kTakeNt >= R) continue;
+    const int i = k * kTakeNt + tid;
+    bool copied = false;
+    RowPlan r{};
+    if (i < R) {
+      r = row_plan(a, i);
+      const bool given = need_[k] == 0 || s_start[i] + need_[k] <= n_free;
+      a.to.lens[i] = given ? r.want : r.len;
+      if (a.ok) a.ok[i] = r.fits && given;
+      copied = given && away_[k];
+      if (r.want > r.len && r.len % T) {
+        const int q = a.to.table[i * a.to.ldt + r.len / T];
+        if (is_page(q, P)) {
+          a.s.writers[q] = 0;
+          a.s.order[q] = 0;
+        }
+      }
+    }
+    int total;
+    const int at = scan_before(copied ? 1 : 0, &total);
+    if (copied) {
+      const int q = a.to.table[i * a.to.ldt + r.len / T];
+      agent_add(&a.to.ref[q], -1);
+      a.s.copies[copies + at] = {q, i, r.len / T, r.len % T};
+    }
+    copies += total;
+  }
+  if (tid == 0) *a.s.n_copies = copies;
+  __syncthreads();
+  // the free page of rank k goes to the row that asks for the k-th page; a wave takes a word, a lane a page
+  for (int w = tid >> 6; w < words && s_before[w] < asked; w += kTakeNt / 64) {
+    const unsigned long long b = agent_load(&a.s.bits[w]);
+    const int k = s_before[w] + __popcll(b & ((1ull << lane) - 1ull));
+    if (!(b >> lane & 1ull) || k >= asked) continue;
+    // the last row that starts at or before it: rows that ask for nothing start where the next one does
+    int lo = 0, hi = R - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (s_start[mid] <= k) lo = mid;
+      else hi = mid - 1;
+    }
+    if ((lo + 1 < R ? s_start[lo + 1] : asked) > n_free) continue;  // the row does not get all of its pages, and so none
+    a.to.table[lo * a.to.ldt + s_first[lo] + (k - s_start[lo])] = w * 64 + lane;
+    agent_store(&a.to.ref[w * 64 + lane], 1);
+  }
+}
+
+// Tokens of a page into another page of a plane: one chunk, four 16-byte columns a thread.
+__device__ __forceinline__ void copy_tokens(const PlaneArgs& c, int plane, int src, int dst, int tokens, uint32_t chunk) {
+  typedef uint32_t vec __attribute__((ext_vector_type(4), aligned(1)));
+  const uint32_t run = static_cast<uint32_t>(tokens) * static_cast<uint32_t>(c.token_bytes);
+  const uint32_t cols = (run + 15) / 16, m = 0xFFFFFFFFu / cols;
+  const uint32_t total = cols * static_cast<uint32_t>(c.pieces);
+  char* base = static_cast<char*>(c.planes[plane]);
+  const char* from = base + src * c.row_stride;
+  char* to = base + dst * c.row_stride;
+  vec v[4];
+  long long off[4];
+  int n[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t idx = chunk * (kNt * 4) + k * kNt + threadIdx.x;
+    n[k] = 0;
+    if (idx < total) {
+      const uint32_t piece = divide(idx, cols, m), at = (idx - piece * cols) * 16;
+      off[k] = piece * c.piece_stride + at;
+      n[k] = static_cast<int>(min(run - at, 16u));
+      if (n[k] == 16) v[k] = *reinterpret_cast<const vec*>(from + off[k]);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (n[k] == 16) {
+      *reinterpret_cast<vec*>(to + off[k]) = v[k];
+    } else {
+      for (int b = 0; b < n[k]; ++b) to[off[k] + b] = from[off[k] + b];
+    }
+  }
+}
+__device__ __forceinline__ uint32_t chunks_of(const PlaneArgs& c, int tokens) {
+  const uint32_t cols = (static_cast<uint32_t>(tokens) * static_cast<uint32_t>(c.token_bytes) + 15) / 16;
+  return (cols * static_cast<uint32_t>(c.pieces) + kNt * 4 - 1) / (kNt * 4);
+}
+
+__global__ __launch_bounds__(kNt) void k_page_copy(PageArgs a) {
+  const uint32_t chunks = chunks_of(a.cache, a.cache.tokens), per = chunks * static_cast<uint32_t>(a.cache.n_planes);
+  const unsigned long long total = static_cast<unsigned long long>(*a.s.n_copies) * per;
+  for (unsigned long long u = blockIdx.x; u < total; u += gridDim.x) {
+    const PageCopy c = a.s.copies[u / per];
+    const uint32_t rest = static_cast<uint32_t>(u % per), plane = rest / chunks, chunk = rest % chunks;
+    if (chunk >= chunks_of(a.cache, c.tokens)) continue;
+    const long long row = c.row;
+    copy_tokens(a.cache, static_cast<int>(plane), c.src, a.to.table[row * a.to.ldt + c.at], c.tokens, chunk);
+  }
+}
+
+// ---- compaction ------------------------------------------------------------------------------------------
+
+// The pages in use as bits; in the last workgroup, how many are in use before each word.
+__global__ __launch_bounds__(kTakeNt) void k_pages_scan(PageArgs a) {
+  __shared__ int s_last;
+  const int tid = threadIdx.x, lane = tid & 63, P = a.to.n_pages;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int p = blockIdx.x * kTakePages + k * kTakeNt + tid;
+    const unsigned long long used = __ballot(p < P && a.from.ref[min(p, P - 1)] > 0);
+    if (lane == 0 && p < P) agent_store(&a.s.bits[p >> 6], used);
+  }
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  __syncthreads();
+  if (tid == 0) s_last = agent_add(a.s.tick, 1u) == gridDim.x - 1;
+  __syncthreads();
+  if (!s_last) return;
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  if (tid == 0) agent_store(a.s.tick, 0u);
+  const int words = (P + 63) / 64, mine = (words + kTakeNt - 1) / kTakeNt;
+  int count = 0;
+  for (int w = tid * mine; w < min(words, (tid + 1) * mine); ++w) count += __popcll(agent_load(&a.s.bits[w]));
+  int total;
+  int at = scan_before(count, &total);
+  for (int w = tid * mine; w < min(words, (tid + 1) * mine); ++w) {
+    a.s.before[w] = at;
+    at += __popcll(agent_load(&a.s.bits[w]));
+  }
+  if (tid == 0) {
+    a.s.before[words] = total;
+    if (a.live) *a.live = total;
+  }
+}
+
+// Pages in use below page p.
+__device__ __forceinline__ int used_before(const PageArgs& a, int p) {
+  return a.s.before[p >> 6] + __popcll(a.s.bits[p >> 6] & ((1ull << (p & 63)) - 1ull));
+}
+__device__ __forceinline__ bool is_used(const PageArgs& a, int p) { return a.s.bits[p >> 6] >> (p & 63) & 1ull; }
+
+// The pages in use at n and beyond, and the free ones below n, in order.
+__global__ __launch_bounds__(kNt) void k_pages_pair(PageArgs a) {
+  const int p = blockIdx.x * kNt + threadIdx.x, P = a.to.n_pages;
+  if (p >= P) return;
+  const int n = a.s.before[(P + 63) / 64], below = used_before(a, p);
+  if (p < n && !is_used(a, p)) a.s.room[p - below] = p;
+  if (p >= n && is_used(a, p)) a.s.moves[below - used_before(a, n)] = p;
+}
+
+__device__ __forceinline__ int moved_to(const PageArgs& a, int p, int n, int kept) {
+  return p < n ? p : a.s.room[used_before(a, p) - kept];
+}
+
+// Tables, ref and moved; the pages' tokens.
+__global__ __launch_bounds__(kNt) void k_pages_move(PageArgs a) {
+  const int P = a.to.n_pages, T = a.to.page_tokens, n = a.s.before[(P + 63) / 64];
+  const int kept = n < P ? used_before(a, n) : n;  // pages in use below n
+  const int moves = n - kept;
+  const uint32_t chunks = chunks_of(a.cache, a.cache.tokens), per = chunks * static_cast<uint32_t>(a.cache.n_planes);
+  // small work first: tables by rows, then the pool
+  for (int i = blockIdx.x; i < a.to.rows; i += gridDim.x) {
+    const int len = held(a.from, i), used = pages_of(len, T);
+    for (int j = threadIdx.x; j < a.to.row_pages; j += kNt) {
+      int p = -1;
+      if (j < used) {
+        p = a.from.table[i * a.from.ldt + j];
+        if (is_page(p, P)) p = is_used(a, p) ? moved_to(a, p, n, kept) : -1;
+      }
+      a.to.table[i * a.to.ldt + j] = p;
+    }
+    if (threadIdx.x == 0) a.to.lens[i] = len;
+  }
+  for (int p = blockIdx.x * kNt + threadIdx.x; p < P; p += gridDim.x * kNt) {
+    const bool used = is_used(a, p);
+    const int to = used ? moved_to(a, p, n, kept) : -1;
+    if (a.moved) a.moved[p] = to;
+    if (used) a.to.ref[to] = a.from.ref[p];
+    if (p >= n) a.to.ref[p] = 0;
+  }
+  if (!a.cache.n_planes) return;
+  const unsigned long long total = static_cast<unsigned long long>(moves) * per;
+  for (unsigned long long u = blockIdx.x; u < total; u += gridDim.x) {
+    const int k = static_cast<int>(u / per);
+    const uint32_t rest = static_cast<uint32_t>(u % per);
+    copy_tokens(a.cache, static_cast<int>(rest / chunks), a.s.moves[k], a.s.room[k], a.cache.tokens, rest % chunks);
+  }
+}
+
+template <int MAXW, int B>
+void go_reorder(const ReorderArgs& a, int groups, int blocks, hipStream_t st) {
+  hipLaunchKernelGGL((k_reorder<MAXW, B>), dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(groups)), dim3(kNt), 0, st, a);
+}
+
+}  // namespace
+
+void launch_reorder(const ReorderArgs& a, int groups, int cus, hipStream_t st) {
+  const int bytes = a.width <= 32 ? 16 : 8;
+  const long long cols = (static_cast<long long>(a.p.tokens) * a.p.token_bytes + bytes - 1) / bytes * a.p.n_planes * a.p.pieces;
+  const long long most = (cols + kNt - 1) / kNt;
+  const int blocks = static_cast<int>(std::max<long long>(1, std::min<long long>(most, (32ll * cus + groups - 1) / groups)));
+  if (a.width <= 4) go_reorder<4, 16>(a, groups, blocks, st);
+  else if (a.width <= 8) go_reorder<8, 16>(a, groups, blocks, st);
+  else if (a.width <= 16) go_reorder<16, 16>(a, groups, blocks, st);
+  else if (a.width <= 32) go_reorder<32, 16>(a, groups, blocks, st);
+  else go_reorder<64, 8>(a, groups, blocks, st);
+}
+
+void launch_pages_step(const PageArgs& a, int cus, hipStream_t st) {
+  hipLaunchKernelGGL(k_pages_fork, dim3(static_cast<unsigned>(std::max(a.from.rows, a.to.rows))), dim3(kNt), 0, st, a);
+  hipLaunchKernelGGL(k_pages_take, dim3(static_cast<unsigned>((a.to.n_pages + kTakePages - 1) / kTakePages)), dim3(kTakeNt), 0, st, a);
+  if (a.cache.n_planes && (a.add || a.add_all > 0))
+    hipLaunchKernelGGL(k_page_copy, dim3(static_cast<unsigned>(8 * cus)), dim3(kNt), 0, st, a);
+}
+
+void launch_pages_compact(const PageArgs& a, int cus, hipStream_t st) {
+  hipLaunchKernelGGL(k_pages_scan, dim3(static_cast<unsigned>((a.to.n_pages + kTakePages - 1) / kTakePages)), dim3(kTakeNt), 0, st, a);
+  hipLaunchKernelGGL(k_pages_pair, dim3(static_cast<unsigned>((a.to.n_pages + kNt - 1) / kNt)), dim3(kNt), 0, st, a);
+  hipLaunchKernelGGL(k_pages_move, dim3(static_cast<unsigned>(8 * cus)), dim3(kNt), 0, st, a);
+}
+
+}  // namespace vsmp
