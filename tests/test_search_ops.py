@@ -160,6 +160,23 @@ def test_select_ties_and_orders(ctx, dtype, kind):
         assert r.token[g].tolist() == tok[go].tolist() and r.parent[g].tolist() == a[go].tolist()
 
 
+@pytest.mark.parametrize("G,W,n,vocab", [(2, 64, 64, 600), (3, 40, 7, 9000), (1, 64, 64, 70000), (1, 2, 64, 400000)])
+def test_select_more_equal_entries_than_are_ranked_at_once(ctx, G, W, n, vocab):
+    """Beams and logits that are all alike, but for some: the lists are merged in order."""
+    import torch
+
+    x = torch.zeros(G * W, vocab, device="cuda")
+    x[:, vocab // 2] = 1.0
+    x[-1, 5] = 3.0
+    log("alike", G, W, n, vocab)
+    r = check_select(ctx, x, np.full((G, W), -2.0, np.float32), n, [0])
+    want = continuations(x.double().cpu().numpy(), np.full((G, W), -2.0), W)
+    for g in range(G):
+        s, a, _, tok = want[g]
+        go = np.flatnonzero(tok != 0)[:n]
+        assert r.token[g].tolist() == tok[go].tolist() and r.parent[g].tolist() == a[go].tolist()
+
+
 def test_select_rows_that_are_not_live(ctx):
     """Rows of -inf, with a NaN, with a +inf; scores of -inf, +inf and NaN; groups with fewer continuations than n and
     with none; masked rows that leave one token."""
