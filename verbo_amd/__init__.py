@@ -764,16 +764,14 @@ class Context:
             raise VsmpError("need n >= 1 beams of the next step")
         stops = (ctypes.c_int * len(stop_ids))(*stop_ids) if len(stop_ids) else None
         sp = _array_of(scores, T.float32, B, "scores", dev)
-        # one allocation for what the step returns: the n-wide arrays one after the other, then the counts
-        k = G * n
-        buf = T.output((6 * k + G,), T.int32, dev, stream)
-        at = [buf[i * k:(i + 1) * k].view(G, n) for i in range(6)]
-        out = BeamStep(at[0], at[1], at[2].view(T.float32), at[3], at[4], at[5].view(T.float32), buf[6 * k:])
-        p = buf.data_ptr()
-        if _lib.vsmp_beam_select(self._h, logits.data_ptr(), code, ld, G, W, V, sp, n, stops, len(stop_ids), p, p + 4 * k, p + 8 * k,
-                                 p + 12 * k, p + 16 * k, p + 20 * k, p + 24 * k, T.stream(stream, dev)) != 0:
+        token, parent, end_token, end_parent = T.output((4, G, n), T.int32, dev, stream).unbind(0)
+        score, end_score = T.output((2, G, n), T.float32, dev, stream).unbind(0)
+        n_end = T.output((G,), T.int32, dev, stream)
+        if _lib.vsmp_beam_select(self._h, logits.data_ptr(), code, ld, G, W, V, sp, n, stops, len(stop_ids), token.data_ptr(), parent.data_ptr(),
+                                 score.data_ptr(), end_token.data_ptr(), end_parent.data_ptr(), end_score.data_ptr(), n_end.data_ptr(),
+                                 T.stream(stream, dev)) != 0:
             raise _err()
-        return out
+        return BeamStep(token, parent, score, end_token, end_parent, end_score, n_end)
 
     def reorder_rows(self, planes, parent, width, lens=None, stream=None):
         """vsmp_reorder_rows: in every plane of `planes` (a Planes) row i takes what row parent[i] held, in place. parent:

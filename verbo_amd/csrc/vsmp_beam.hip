@@ -44,6 +44,7 @@ __device__ __forceinline__ uint64_t lane_xor(uint64_t v, int lane) {
 struct Cand {
   uint64_t s, t;
 };
+__device__ __forceinline__ bool before(uint32_t a, uint32_t b) { return a > b; }
 __device__ __forceinline__ bool before(uint64_t a, uint64_t b) { return a > b; }
 __device__ __forceinline__ bool before(const Cand& a, const Cand& b) {
   return a.s > b.s || (a.s == b.s && a.t > b.t);
@@ -103,6 +104,19 @@ __device__ __forceinline__ void agent_store(T* p, T v) {
 }
 
 __device__ __forceinline__ bool finite(float v) { return __builtin_isfinite(v); }
+// How many of the n entries at p come before c, eight at a time; entries up to the next eight are there.
+template <class T>
+__device__ __forceinline__ int count_before(const T* p, int n, const T& c) {
+  int rank = 0;
+  for (int i = 0; i < n; i += 8) {
+    T o[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o[k] = p[i + k];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) rank += i + k < n && before(o[k], c) ? 1 : 0;
+  }
+  return rank;
+}
 // How many of the lanes' flags below this one are set.
 __device__ __forceinline__ int below(unsigned long long at) {
   return static_cast<int>(__builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(at >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(at), 0u)));
@@ -110,112 +124,99 @@ __device__ __forceinline__ int below(unsigned long long at) {
 
 // ---- k_beam ----------------------------------------------------------------------------------------------
 
-constexpr int kCands = 256;  // continuations that the last part ranks side by side
+constexpr int kCands = 256;    // continuations that the last part ranks side by side
 
-// One part of a row: a step of four 16-byte groups a thread at a time, the next in flight. Each wave collects in LDS the
-// logits that reach its bound, below which none can be among the part's N largest that are no stop tokens. The bound
-// is at first the N-th largest (or one below it) of the lanes' maxima over the first step: the least of the maxima of
-// as many groups of lanes, stop tokens' groups left out of account. Where 64 have collected, the wave sorts them into a
-// list over its lanes, whose N-th is the bound from then on. In the end the waves' logits that reach the largest of their
-// bounds are ranked by comparing each with each, a thread each: mostly they are few more than N.
+// One part of a row: a step of four 16-byte groups a thread at a time, the next in flight; what a row has beyond whole
+// groups, a lane each, in the end. Each wave collects in LDS the logits that reach its bound, below which none can be
+// among the part's N largest that are no stop tokens. The bound is at first the N-th largest (or one below it) of the
+// lanes' maxima over the first step: the least of the maxima of as many groups of lanes, stop tokens' groups left out
+// of account. Where 64 have collected, the wave sorts them into a list over its lanes, whose N-th is the bound from then
+// on. In the end the waves' logits that reach the largest of their bounds are ranked by comparing each with each, a
+// thread each: mostly they are few more than N.
 //
 // The last part of a group ranks its rows' lists by score in the same way: the N-th largest first entry of the lists (of
 // those of a wave's threads) is a bound for all entries. Where more entries than kCands reach it (many equal
 // ones) each wave merges lists in order instead, and the first wave the waves'.
+//
+// A few rows are bound by latencies, those of fetching the code among them: every workgroup runs most of it once. So loops
+// stay rolled where they hardly turn, and nothing is divided by what is not a constant.
 template <class E>
-__global__ __launch_bounds__(kNt) void k_beam(BeamArgs a) {
+__global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
   constexpr int N = 16 / E::kSize, G = 4;
   constexpr int kStep = kNt * N * G;
   union Shared {
     struct {
-      uint64_t wait[kW][128], list[kNt];
+      uint64_t wait[kW][128], list[2 * kNt + 16];  // of 64 that wait and 64 in order a wave, and a row's last 7
     } part;
     struct {
       Cand cand[kCands];
       Cand end[kBeamMax * kBeamStops];
+      unsigned short lists[kBeamMax * kBeamMax];
     } group;
     Cand merge[kW][kBeamMax];
   };
   __shared__ Shared sh;
-  __shared__ float s_m[kW];
-  __shared__ double s_s[kW], s_lse[kBeamMax], s_score[kBeamMax];
-  __shared__ uint64_t s_bound[kW];
-  __shared__ int s_wait[kW], s_n, s_end, s_ended, s_last;
+  __shared__ float s_m[kW], s_s[kW];
+  __shared__ double s_lse[kBeamMax], s_score[kBeamMax];
+  __shared__ uint32_t s_bound[kW];
+  __shared__ int s_n, s_lists, s_end, s_ended, s_last;
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int row = static_cast<int>(blockIdx.x / static_cast<unsigned>(a.P));
-  const int part = static_cast<int>(blockIdx.x % static_cast<unsigned>(a.P));
-  const int group = row / a.W;
-  const int lo = part * a.L, hi = min(a.V, lo + a.L);
+  const int part = static_cast<int>(blockIdx.x), group = static_cast<int>(blockIdx.z);
+  const int first = group * a.W, row = first + static_cast<int>(blockIdx.y);  // the group's first row, and this one
+  const int lo = part * a.L, hi = min(a.V, lo + a.L), whole = hi & ~(N - 1);
   const char* x = static_cast<const char*>(a.x) + row * a.ld * E::kSize;
-
-  auto is_stop = [&](int t) {
-    bool s = false;
-    for (int i = 0; i < a.n_stop; ++i) s |= t == a.stops[i];
-    return s;
-  };
+  const int stop = lane < a.n_stop ? a.stops[lane] : -1;  // a lane each
+  if (tid == 0) s_n = 0;
 
   Lse z{-INFINITY, 0.0f};
   int waiting = 0;               // logits that the wave has collected
+  uint64_t best = 0;             // the lane's entry of the wave's list; 0: none
   uint32_t sure = 0;             // a key that N of its logits reach, no stop tokens among them; 0: none known
   if (finite(a.scores[row])) {
-    uint64_t best = 0;           // the lane's entry of the wave's list; 0: none
-    bool listed = false;
     float bound = -FLT_MAX;
-    int skip = 0;                // stop tokens in this part
-    for (int i = 0; i < a.n_stop; ++i) skip += a.stops[i] >= lo && a.stops[i] < hi ? 1 : 0;
-    auto flush = [&]() {         // the first 64 of those that wait go into the list
-      __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-      const int n = min(waiting, 64);
-      uint64_t v = lane < n ? sh.part.wait[wv][lane] : 0ull;
-      const uint64_t rest = sh.part.wait[wv][64 + lane];
-      waiting -= n;
-      __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-      if (lane < waiting) sh.part.wait[wv][lane] = rest;
-      sort64(v, lane, true);
-      merge64(best, v, lane);
-      listed = true;
-      const uint32_t nth = __builtin_amdgcn_readlane(static_cast<uint32_t>(best >> 32), a.N - 1);
-      if (nth) {
-        sure = nth;
-        bound = fmaxf(bound, key_val(nth));
-      }
-    };
+    const int skip = __popcll(__ballot(stop >= lo && stop < hi));  // stop tokens in this part
     Raw<E, N> r[G];
     auto load = [&](int e0) {
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         const int e = e0 + N * (tid + g * kNt);
-        if (e + N <= hi) {
+        if (e < whole) {
           r[g].load(x, e);
-        } else {  // the row's end: its last elements one by one, then -inf
+        } else {
+          constexpr float kNone[8] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY};
           float v[N];
 #pragma unroll
-          for (int k = 0; k < N; ++k) v[k] = e + k < hi ? E::get(x, e + k) : -INFINITY;
+          for (int k = 0; k < N; ++k) v[k] = kNone[k];
           r[g].set(v);
         }
       }
     };
     load(lo);
-    for (int e0 = lo; e0 < hi; e0 += kStep) {
-      float v[G][N], gm[G];
+    float rest = -INFINITY;
+    if (tid < hi - whole) rest = E::get(x, whole + tid);
+    // i: the wave's logits that reach the bound, u the lane's of token e, go to those that wait
+    auto collect = [&](float u, int e, bool take) {
+      for (int i = 0; i < a.n_stop; ++i) take = take && e != __builtin_amdgcn_readlane(stop, i);
+      const unsigned long long at = __ballot(take);
+      if (take) sh.part.wait[wv][waiting + below(at)] = comp(ord_key(u), static_cast<uint32_t>(e));
+      waiting += __popcll(at);
+    };
+    for (int e0 = lo; e0 < whole; e0 += kStep) {
+      float v[G * N], gm[G];
 #pragma unroll
-      for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int k = 0; k < N; ++k) v[g][k] = r[g].get(k);
-      if (e0 + kStep < hi) load(e0 + kStep);
+      for (int k = 0; k < G * N; ++k) v[k] = r[k / N].get(k % N);
+      if (e0 + kStep < whole) load(e0 + kStep);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        gm[g] = v[g][0];
+        gm[g] = v[g * N];
 #pragma unroll
-        for (int k = 1; k < N; ++k) gm[g] = fmaxf(gm[g], v[g][k]);
+        for (int k = 1; k < N; ++k) gm[g] = fmaxf(gm[g], v[g * N + k]);
       }
       const float mx = fmaxf(fmaxf(gm[0], gm[1]), fmaxf(gm[2], gm[3]));
       const float m = fmaxf(z.m, mx), rel = m == -INFINITY ? 0.0f : m;  // of -inf alone: exp(-inf - 0) = 0, and NaN stays
       float s = z.s * exp_rel(z.m, rel);
 #pragma unroll
-      for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int k = 0; k < N; ++k) s += exp_rel(v[g][k], rel);
+      for (int k = 0; k < G * N; ++k) s += exp_rel(v[k], rel);
       z = {m, s};
       if (e0 == lo && a.N + skip <= 64) {
         // groups of 64 / M lanes, M >= N + skip: their maxima, and the least of those
@@ -233,76 +234,89 @@ __global__ __launch_bounds__(kNt) void k_beam(BeamArgs a) {
           sure = ord_key(t);
         }
       }
-      if (__ballot(mx >= bound)) {
+      if (!__ballot(mx >= bound)) continue;
+      uint32_t hits = 0;  // the lane's logits that reach the bound, a bit each
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-          if (!__ballot(gm[g] >= bound)) continue;
+      for (int k = 0; k < G * N; ++k) hits |= v[k] >= bound ? 1u << k : 0u;
+      while (__ballot(hits != 0u)) {  // one of each lane's at a time
+        const int i = __ffs(static_cast<int>(hits)) - 1;
+        float u[G * N];  // halved by the bits of i
 #pragma unroll
-          for (int k = 0; k < N; ++k) {
-            const int e = e0 + N * (tid + g * kNt) + k;
-            bool take = v[g][k] >= bound;
-            if (!__ballot(take)) continue;
-            take = take && !is_stop(e);
-            const unsigned long long at = __ballot(take);
-            const int pos = waiting + below(at);
-            if (take) sh.part.wait[wv][pos] = comp(ord_key(v[g][k]), static_cast<uint32_t>(e));
-            waiting += __popcll(at);
-            if (waiting > 64) flush();
-          }
+        for (int k = 0; k < G * N; ++k) u[k] = v[k];
+#pragma unroll
+        for (int d = G * N / 2; d; d >>= 1)
+#pragma unroll
+          for (int k = 0; k < d; ++k) u[k] = i & d ? u[k + d] : u[k];
+        collect(u[0], e0 + N * (tid + (i / N) * kNt) + i % N, hits != 0u && u[0] >= bound);
+        hits &= hits - 1u;
+        if (waiting <= 64) continue;
+        // the first 64 of those that wait go into the list
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+        uint64_t w = sh.part.wait[wv][lane];
+        const uint64_t left = sh.part.wait[wv][64 + lane];
+        waiting -= 64;
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+        if (lane < waiting) sh.part.wait[wv][lane] = left;
+        sort64(w, lane, true);
+        merge64(best, w, lane);
+        const uint32_t nth = __builtin_amdgcn_readlane(static_cast<uint32_t>(best >> 32), a.N - 1);
+        if (nth) {
+          sure = nth;
+          bound = fmaxf(bound, key_val(nth));
         }
-        // what comes in later steps has higher tokens: among equal logits it is behind those that N have reached
-        if (sure) bound = fmaxf(bound, next_up(key_val(sure)));
       }
+      // what comes in later steps has higher tokens: among equal logits it is behind those that N have reached
+      if (sure) bound = fmaxf(bound, next_up(key_val(sure)));
     }
-    if (listed) {  // in order, so that no more than N of them count
-      flush();
-      if (waiting) flush();
-      waiting = __popcll(__ballot(best != 0 && lane < a.N));
-      if (lane < waiting) sh.part.wait[wv][lane] = best;
+    if (whole < hi && wv == 0) {
+      const float m = fmaxf(z.m, rest), rel = m == -INFINITY ? 0.0f : m;
+      z = {m, z.s * exp_rel(z.m, rel) + exp_rel(rest, rel)};
+      collect(rest, whole + lane, rest >= bound);  // at most 7: there is room
     }
   }
   // the waves' sums and logits as the part's
   z = wave_lse(z);
   if (lane == 0) {
     s_m[wv] = z.m;
-    s_s[wv] = static_cast<double>(z.s);
+    s_s[wv] = z.s;
     s_bound[wv] = sure;
-    s_wait[wv] = waiting;
   }
-  if (tid == 0) s_n = 0;
   __syncthreads();
   const int slot = row * a.P + part;
   {
-    const uint64_t most = max(max(s_bound[0], s_bound[1]), max(s_bound[2], s_bound[3]));
-    const uint64_t key = lane < s_wait[wv] ? sh.part.wait[wv][lane] : 0ull;
-    const bool take = key != 0 && key >> 32 >= most;
-    const unsigned long long at = __ballot(take);
-    int first = 0;
-    if (lane == 0 && at) first = atomicAdd(&s_n, __popcll(at));
-    first = __builtin_amdgcn_readfirstlane(first);
-    if (take) sh.part.list[first + below(at)] = key;
+    const uint32_t most = max(max(s_bound[0], s_bound[1]), max(s_bound[2], s_bound[3]));
+    auto give = [&](uint64_t key) {
+      const bool take = key != 0 && key >> 32 >= most;
+      const unsigned long long at = __ballot(take);
+      if (!at) return;
+      int to = 0;
+      if (lane == 0) to = atomicAdd(&s_n, __popcll(at));
+      to = __builtin_amdgcn_readfirstlane(to) + below(at);
+      if (take) sh.part.list[to] = key;
+    };
+    give(lane < waiting ? sh.part.wait[wv][lane] : 0ull);
+    if (waiting > 64) give(lane + 64 < waiting ? sh.part.wait[wv][lane + 64] : 0ull);
+    if (__ballot(best != 0)) give(best);
   }
   __syncthreads();
   // hand over through the device's memory: agent-scope stores, completed before the ticket is taken; the part
   // with the group's last ticket reads them with agent-scope loads after an acquire, and clears the ticket
   const int n = s_n;
-  if (tid < n) {
-    const uint64_t key = sh.part.list[tid];
-    int rank = 0;
-    for (int i = 0; i < n; ++i) rank += sh.part.list[i] > key ? 1 : 0;
+#pragma unroll 1
+  for (int t = tid; t < max(n, a.N); t += kNt) {
+    const uint64_t key = t < n ? sh.part.list[t] : 0ull;
+    const int rank = t < n ? count_before(sh.part.list, n, key) : t;
     if (rank < a.N) agent_store(&a.s.key[slot * a.N + rank], static_cast<unsigned long long>(key));
-  } else if (tid < a.N) {
-    agent_store(&a.s.key[slot * a.N + tid], 0ull);
   }
-  if (tid == 0) {
-    float m = s_m[0];
-#pragma unroll
-    for (int w = 1; w < kW; ++w) m = fmaxf(m, s_m[w]);
+  if (wv == kW - 1) {  // (the last wave has no logits to rank, mostly)
+    const float m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
     double s = 0.0;
 #pragma unroll
-    for (int w = 0; w < kW; ++w) s += m == -INFINITY ? s_s[w] : s_s[w] * static_cast<double>(exp_rel(s_m[w], m));
-    agent_store(&a.s.max[slot], m);
-    agent_store(&a.s.sum[slot], s);
+    for (int w = 0; w < kW; ++w) s += static_cast<double>(m == -INFINITY ? s_s[w] : s_s[w] * exp_rel(s_m[w], m));
+    if (lane == 0) {
+      agent_store(&a.s.max[slot], m);
+      agent_store(&a.s.sum[slot], s);
+    }
   }
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
@@ -311,30 +325,32 @@ __global__ __launch_bounds__(kNt) void k_beam(BeamArgs a) {
   if (tid == 0) {
     const unsigned t = __hip_atomic_fetch_add(&a.s.tick[group * kBeamPad], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     s_last = static_cast<int>(t) == a.W * a.P - 1;
-    s_n = s_end = s_ended = 0;
+    s_n = s_lists = s_end = s_ended = 0;
   }
   __syncthreads();
   if (!s_last) return;
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
   if (tid == 0) agent_store(&a.s.tick[group * kBeamPad], 0u);
-  const int first = group * a.W;  // the group's first row
   const int lists = a.W * a.P, entries = lists * a.N;
+  const bool few = entries <= kNt;  // an entry a thread
   const unsigned long long* keys = a.s.key + static_cast<long long>(first) * a.P * a.N;
 
   // what does not wait for the rows' sums is loaded first
-  constexpr int kAhead = 4;
-  uint64_t key[kAhead], head[kAhead];
-#pragma unroll
-  for (int k = 0; k < kAhead; ++k) {
-    const int e = tid + k * kNt;
-    key[k] = e < entries ? agent_load(&keys[e]) : 0ull;
-    head[k] = e < lists ? agent_load(&keys[e * a.N]) : 0ull;
-  }
+  const uint64_t mine = few && tid < entries ? agent_load(&keys[tid]) : 0ull;
+  const uint64_t head = tid < lists ? agent_load(&keys[tid * a.N]) : 0ull;
+  const int n_ends = a.end_token ? a.W * a.n_stop : 0;
+  auto stop_logit = [&](int i, int* b, int* t) {  // of beam b's row, of the stop token t
+    *b = static_cast<int>(divide(static_cast<uint32_t>(i), static_cast<uint32_t>(a.n_stop), a.m_stop));
+    *t = a.stops[i - *b * a.n_stop];
+    return E::get(static_cast<const char*>(a.x) + (first + *b) * a.ld * E::kSize, *t);
+  };
+  float end_x = -INFINITY;
+  int end_b = 0, end_t = 0;
+  if (tid < n_ends) end_x = stop_logit(tid, &end_b, &end_t);
   // lse of each row, its parts side by side in lanes; NaN for a row that is not live
-  int S = 1;
-  while (S < a.P) S <<= 1;
-  for (int i = tid; i < a.W * S + kNt - 1 - (a.W * S - 1) % kNt; i += kNt) {
-    const int b = i / S, p = i % S;
+#pragma unroll 1
+  for (int i0 = 0; i0 < a.W << a.log_s; i0 += kNt) {
+    const int b = (i0 + tid) >> a.log_s, p = (i0 + tid) & ((1 << a.log_s) - 1);
     float m = -INFINITY, sc = 0.0f;
     double s = 0.0;
     if (b < a.W && p < a.P) {
@@ -343,9 +359,11 @@ __global__ __launch_bounds__(kNt) void k_beam(BeamArgs a) {
       sc = a.scores[first + b];
     }
     float top = m;
-    for (int d = S >> 1; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-    if (m != top) s *= m == -INFINITY ? 1.0 : exp(static_cast<double>(m) - static_cast<double>(top));  // (a sum at -inf is 0 or NaN)
-    for (int d = S >> 1; d; d >>= 1) s += __shfl_xor(s, d);
+#pragma unroll 1
+    for (int d = 1 << a.log_s >> 1; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    if (m != -INFINITY) s *= static_cast<double>(exp_rel(m, top));  // (a sum at -inf is 0 or NaN)
+#pragma unroll 1
+    for (int d = 1 << a.log_s >> 1; d; d >>= 1) s += __shfl_xor(s, d);
     if (b < a.W && p == 0) {
       const double lse = static_cast<double>(top) + log(s);
       s_lse[b] = finite(sc) && __builtin_isfinite(lse) ? lse : NAN;
@@ -353,64 +371,60 @@ __global__ __launch_bounds__(kNt) void k_beam(BeamArgs a) {
     }
   }
   __syncthreads();
+  auto beam_of = [&](int l) { return static_cast<int>(divide(static_cast<uint32_t>(l), static_cast<uint32_t>(a.P), a.m_parts)); };
   auto entry = [&](uint64_t key, int b) {
     const double lse = s_lse[b];
     if (!key || lse != lse) return none();
     return Cand{ord_f64(s_score[b] + (static_cast<double>(comp_val(key)) - lse)),
                 static_cast<uint64_t>(63 - b) << 52 | key >> 32 << 20 | (key & 0xFFFFFu)};
   };
-  auto put = [&](int* token, int* parent, float* score, int at, const Cand& c, bool there) {
+  auto put = [&](int* token, int* parent, float* score, int at, const Cand& c) {
     const long long o = static_cast<long long>(group) * a.N + at;
-    token[o] = there ? static_cast<int>(~static_cast<uint32_t>(c.t) & 0xFFFFFu) : -1;
-    parent[o] = a.row0 + first + (there ? 63 - static_cast<int>(c.t >> 52) : at % a.W);
-    score[o] = there ? static_cast<float>(f64_ord(c.s)) : -INFINITY;
+    int b = at;
+    while (b >= a.W) b -= a.W;
+    token[o] = c.s ? static_cast<int>(~static_cast<uint32_t>(c.t) & 0xFFFFFu) : -1;
+    parent[o] = a.row0 + first + (c.s ? 63 - static_cast<int>(c.t >> 52) : b);
+    score[o] = c.s ? static_cast<float>(f64_ord(c.s)) : -INFINITY;
   };
-  // the N-th of the first entries that a wave's threads have: the largest of the waves' is a bound for all entries
-  uint64_t bound;
-  {
-    uint64_t top = 0;
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const uint64_t s = tid + k * kNt < lists ? entry(head[k], (tid + k * kNt) / a.P).s : 0ull;
-      top = s > top ? s : top;
-    }
-    for (int l = tid + kAhead * kNt; l < lists; l += kNt) {
-      const uint64_t s = entry(agent_load(&keys[l * a.N]), l / a.P).s;
-      top = s > top ? s : top;
-    }
-    if (wv * 64 < lists) sort64(top, lane, false);
-    if (lane == a.N - 1) s_bound[wv] = top;
-    __syncthreads();
-    bound = max(max(max(s_bound[0], s_bound[1]), max(s_bound[2], s_bound[3])), static_cast<uint64_t>(1));
-  }
+  // the N-th of the first entries that a wave's threads have, their scores as fp32 below them (next to zero as well): the
+  // largest of the waves' is a bound for all entries
+  auto below_score = [&](uint64_t key, int l) {
+    const Cand c = entry(key, beam_of(l));
+    return c.s ? ord_key(static_cast<float>(f64_ord(c.s))) - 2u : 0u;
+  };
+  uint32_t top = tid < lists ? below_score(head, tid) : 0u;
+#pragma unroll 1
+  for (int l = tid + kNt; l < lists; l += kNt) top = max(top, below_score(agent_load(&keys[l * a.N]), l));
+  if (wv * 64 < lists) sort64(top, lane, false);
+  if (lane == a.N - 1) s_bound[wv] = top;
+  __syncthreads();
+  const uint32_t most = max(max(s_bound[0], s_bound[1]), max(s_bound[2], s_bound[3]));
+  const uint64_t bound = most ? ord_f64(static_cast<double>(key_val(most))) : 1ull;
   // the stop tokens' continuations; N others come before those that do not reach the bound
-  if (a.end_token) {
-    for (int i = tid; i < a.W * a.n_stop; i += kNt) {
-      const int b = i / a.n_stop, t = a.stops[i % a.n_stop];
-      const float u = E::get(static_cast<const char*>(a.x) + (first + b) * a.ld * E::kSize, t);
-      const Cand c = u > -INFINITY ? entry(comp(ord_key(u), static_cast<uint32_t>(t)), b) : none();
-      if (c.s >= bound) sh.group.end[atomicAdd(&s_end, 1)] = c;
-    }
+#pragma unroll 1
+  for (int i = tid; i < n_ends; i += kNt) {
+    if (i >= kNt) end_x = stop_logit(i, &end_b, &end_t);
+    const Cand c = end_x > -INFINITY ? entry(comp(ord_key(end_x), static_cast<uint32_t>(end_t)), end_b) : none();
+    if (c.s >= bound) sh.group.end[atomicAdd(&s_end, 1)] = c;
   }
-  auto collect = [&](uint64_t key, int e) {
-    const Cand c = key ? entry(key, e / (a.P * a.N)) : none();
-    const bool take = c.s >= bound;
-    const unsigned long long at = __ballot(take);
-    if (!at) return;
-    int to = 0;
-    if (lane == 0) to = atomicAdd(&s_n, __popcll(at));
-    to = __builtin_amdgcn_readfirstlane(to) + below(at);
-    if (take && to < kCands) sh.group.cand[to] = c;
-  };
-#pragma unroll
-  for (int k = 0; k < kAhead; ++k)
-    if (k * kNt < entries) collect(key[k], min(tid + k * kNt, entries - 1));
-  for (int e0 = kAhead * kNt; e0 < entries; e0 += kAhead * kNt) {
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) key[k] = e0 + tid + k * kNt < entries ? agent_load(&keys[e0 + tid + k * kNt]) : 0ull;
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k)
-      if (e0 + k * kNt < entries) collect(key[k], min(e0 + tid + k * kNt, entries - 1));
+  // the entries that reach it: of all lists, or of those whose first one does
+  int some = lists;
+  if (!few) {
+#pragma unroll 1
+    for (int l = tid; l < lists; l += kNt)
+      if (entry(agent_load(&keys[l * a.N]), beam_of(l)).s >= bound) sh.group.lists[atomicAdd(&s_lists, 1)] = static_cast<unsigned short>(l);
+    __syncthreads();
+    some = s_lists;
+  }
+#pragma unroll 1
+  for (int i = tid; i < some * a.N; i += kNt) {
+    const int at = static_cast<int>(divide(static_cast<uint32_t>(i), static_cast<uint32_t>(a.N), a.m_n));
+    const int l = few ? at : sh.group.lists[at];
+    const Cand c = entry(few ? mine : agent_load(&keys[l * a.N + (i - at * a.N)]), beam_of(l));
+    if (c.s >= bound) {
+      const int to = atomicAdd(&s_n, 1);
+      if (to < kCands) sh.group.cand[to] = c;
+    }
   }
   __syncthreads();
   int c_n = s_n;  // continuations in sh.group.cand, the first N among them
@@ -418,48 +432,48 @@ __global__ __launch_bounds__(kNt) void k_beam(BeamArgs a) {
   if (c_n > kCands) {
     Cand c = none();
     __syncthreads();
+#pragma unroll 1
     for (int l = wv; l < lists; l += kW) {
-      const Cand top = entry(agent_load(&keys[l * a.N]), l / a.P);
-      if (top.s < bound) continue;
+      const int b = beam_of(l);
+      if (entry(agent_load(&keys[l * a.N]), b).s < bound) continue;
       uint64_t k = 0;
       if (63 - lane < a.N) k = agent_load(&keys[l * a.N + 63 - lane]);
-      merge64(c, entry(k, l / a.P), lane);
+      merge64(c, entry(k, b), lane);
     }
     sh.merge[wv][lane] = c;
     __syncthreads();
     if (wv == 0)
+#pragma unroll 1
       for (int w = 1; w < kW; ++w) merge64(c, sh.merge[w][63 - lane], lane);
     __syncthreads();
     if (wv == 0) sh.group.cand[lane] = c;
     c_n = a.N;
     __syncthreads();
   }
+#pragma unroll 1
   for (int t = tid; t < max(c_n, a.N); t += kNt) {
-    if (t >= c_n) {
-      put(a.token, a.parent, a.score, t, none(), false);
-      continue;
-    }
-    const Cand c = sh.group.cand[t];
-    int rank = 0;
-    for (int i = 0; i < c_n; ++i) rank += before(sh.group.cand[i], c) ? 1 : 0;
-    if (rank < a.N) put(a.token, a.parent, a.score, rank, c, true);
+    const Cand c = t < c_n ? sh.group.cand[t] : none();
+    const int rank = t < c_n ? count_before(sh.group.cand, c_n, c) : t;
+    if (rank < a.N) put(a.token, a.parent, a.score, rank, c);
   }
   if (!a.end_token) return;
-  // an end is one of the first N of all if fewer come before it, ends or not; those that do are among the candidates
-  int mine = 0;
-  for (int t = tid; t < ends; t += kNt) {
+  // an end is one of the first N of all if fewer come before it, ends or not; those that do are among the candidates.
+  // (The second wave begins with them: the first has the others to rank, mostly.)
+  int ended = 0;
+#pragma unroll 1
+  for (int t = (tid - 64) & (kNt - 1); t < ends; t += kNt) {
     const Cand c = sh.group.end[t];
-    int others = 0, rank = 0;
-    for (int i = 0; i < c_n; ++i) others += before(sh.group.cand[i], c) ? 1 : 0;
-    if (others >= a.N) continue;
-    for (int i = 0; i < ends; ++i) rank += before(sh.group.end[i], c) ? 1 : 0;
-    if (others + rank >= a.N) continue;
-    put(a.end_token, a.end_parent, a.end_score, rank, c, true);
-    ++mine;
+    int rank = count_before(sh.group.cand, c_n, c);
+    if (rank >= a.N) continue;
+    const int among = count_before(sh.group.end, ends, c);
+    if (rank + among >= a.N) continue;
+    put(a.end_token, a.end_parent, a.end_score, among, c);
+    ++ended;
   }
-  if (mine) atomicAdd(&s_ended, mine);
+  if (ended) atomicAdd(&s_ended, ended);
   __syncthreads();
-  for (int t = s_ended + tid; t < a.N; t += kNt) put(a.end_token, a.end_parent, a.end_score, t, none(), false);
+#pragma unroll 1
+  for (int t = s_ended + tid; t < a.N; t += kNt) put(a.end_token, a.end_parent, a.end_score, t, none());
   if (tid == 0) a.n_end[group] = s_ended;
 }
 
@@ -477,8 +491,13 @@ void beam_parts(int B, int V, int dtype, int cus, int* P, int* L) {
   *P = (V + *L - 1) / *L;
 }
 
-void launch_beam(const BeamArgs& a, int dtype, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>(a.G) * static_cast<unsigned>(a.W) * static_cast<unsigned>(a.P));
+void launch_beam(BeamArgs a, int dtype, hipStream_t st) {
+  a.m_parts = 0xFFFFFFFFu / static_cast<uint32_t>(a.P);
+  a.m_n = 0xFFFFFFFFu / static_cast<uint32_t>(a.N);
+  a.m_stop = a.n_stop ? 0xFFFFFFFFu / static_cast<uint32_t>(a.n_stop) : 0u;
+  a.log_s = 0;
+  while (1 << a.log_s < a.P) ++a.log_s;
+  const dim3 grid(static_cast<unsigned>(a.P), static_cast<unsigned>(a.W), static_cast<unsigned>(a.G));
   if (dtype == VSMP_F32)
     hipLaunchKernelGGL(k_beam<F32>, grid, dim3(kNt), 0, st, a);
   else if (dtype == VSMP_BF16)

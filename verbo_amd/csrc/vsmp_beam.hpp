@@ -27,6 +27,12 @@ struct BeamScratch {
   float* max;                // [kBeamSlots]
 };
 
+// idx / n, with m = (2^32 - 1) / n: m n >= 2^32 - n, so that idx m / 2^32 is less than one below idx / n.
+__device__ __forceinline__ uint32_t divide(uint32_t idx, uint32_t n, uint32_t m) {
+  const uint32_t q = __umulhi(idx, m);
+  return idx - q * n >= n ? q + 1 : q;
+}
+
 struct BeamArgs {
   const void* x;
   long long ld;
@@ -36,6 +42,8 @@ struct BeamArgs {
   const float* scores;
   int stops[kBeamStops];
   int n_stop;
+  uint32_t m_parts, m_n, m_stop;  // (2^32 - 1) / P, N, n_stop (launch_beam)
+  int log_s;                      // lanes of a row's parts in the last part, a power of two
   int* token;
   int* parent;
   float* score;
@@ -98,7 +106,7 @@ struct PageArgs {
 
 // Parts and part length of vsmp_beam_select's rows: B = G * W.
 void beam_parts(int B, int V, int dtype, int cus, int* P, int* L);
-void launch_beam(const BeamArgs& a, int dtype, hipStream_t st);
+void launch_beam(BeamArgs a, int dtype, hipStream_t st);
 void launch_reorder(const ReorderArgs& a, int groups, int cus, hipStream_t st);
 void launch_pages_step(const PageArgs& a, int cus, hipStream_t st);
 void launch_pages_compact(const PageArgs& a, int cus, hipStream_t st);

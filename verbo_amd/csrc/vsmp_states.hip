@@ -22,12 +22,6 @@ __device__ __forceinline__ T agent_add(T* p, T v) {
   return __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// idx / n, with m = (2^32 - 1) / n: m n >= 2^32 - n, so that idx m / 2^32 is less than one below idx / n.
-__device__ __forceinline__ uint32_t divide(uint32_t idx, uint32_t n, uint32_t m) {
-  const uint32_t q = __umulhi(idx, m);
-  return idx - q * n >= n ? q + 1 : q;
-}
-
 // ---- k_reorder -------------------------------------------------------------------------------------------
 
 // A column of B bytes over a group's rows belongs to one thread, which loads it from every parent before it stores it in
