@@ -764,13 +764,13 @@ class Context:
             raise VsmpError("need n >= 1 beams of the next step")
         stops = (ctypes.c_int * len(stop_ids))(*stop_ids) if len(stop_ids) else None
         sp = _array_of(scores, T.float32, B, "scores", dev)
-        token, parent, end_token, end_parent = T.output((4, G, n), T.int32, dev, stream).unbind(0)
-        score, end_score = T.output((2, G, n), T.float32, dev, stream).unbind(0)
+        token, parent, end_token, end_parent, score, end_score = T.output((6, G, n), T.int32, dev, stream).unbind(0)
         n_end = T.output((G,), T.int32, dev, stream)
-        if _lib.vsmp_beam_select(self._h, logits.data_ptr(), code, ld, G, W, V, sp, n, stops, len(stop_ids), token.data_ptr(), parent.data_ptr(),
-                                 score.data_ptr(), end_token.data_ptr(), end_parent.data_ptr(), end_score.data_ptr(), n_end.data_ptr(),
-                                 T.stream(stream, dev)) != 0:
+        p, k = token.data_ptr(), 4 * G * n  # the six lie one after the other
+        if _lib.vsmp_beam_select(self._h, logits.data_ptr(), code, ld, G, W, V, sp, n, stops, len(stop_ids), p, p + k, p + 4 * k, p + 2 * k,
+                                 p + 3 * k, p + 5 * k, n_end.data_ptr(), T.stream(stream, dev)) != 0:
             raise _err()
+        score, end_score = score.view(T.float32), end_score.view(T.float32)
         return BeamStep(token, parent, score, end_token, end_parent, end_score, n_end)
 
     def reorder_rows(self, planes, parent, width, lens=None, stream=None):

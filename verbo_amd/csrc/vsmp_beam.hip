@@ -125,12 +125,12 @@ __device__ __forceinline__ int below(unsigned long long at) {
 // ---- k_beam ----------------------------------------------------------------------------------------------
 
 constexpr int kCands = 256;    // continuations that the last part ranks side by side
+constexpr int kWait = 144;     // logits that a wave has collected: 64 that wait, 64 more or 64 in order, a row's last 7
 
 // One part of a row: a step of four 16-byte groups a thread at a time, the next in flight; what a row has beyond whole
 // groups, a lane each, in the end. Each wave collects in LDS the logits that reach its bound, below which none can be
-// among the part's N largest that are no stop tokens. The bound is at first the N-th largest (or one below it) of the
-// lanes' maxima over the first step: the least of the maxima of as many groups of lanes, stop tokens' groups left out
-// of account. Where 64 have collected, the wave sorts them into a list over its lanes, whose N-th is the bound from then
+// among the part's N largest that are no stop tokens. The bound is at first the N-th largest of the
+// lanes' maxima over the first step, stop tokens left out of account: few more logits reach it. Where 64 have collected, the wave sorts them into a list over its lanes, whose N-th is the bound from then
 // on. In the end the waves' logits that reach the largest of their bounds are ranked by comparing each with each, a
 // thread each: mostly they are few more than N.
 //
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
   constexpr int kStep = kNt * N * G;
   union Shared {
     struct {
-      uint64_t wait[kW][128], list[2 * kNt + 16];  // of 64 that wait and 64 in order a wave, and a row's last 7
+      uint64_t wait[kW][kWait], list[kW * kWait];
     } part;
     struct {
       Cand cand[kCands];
@@ -159,7 +159,7 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
   __shared__ float s_m[kW], s_s[kW];
   __shared__ double s_lse[kBeamMax], s_score[kBeamMax];
   __shared__ uint32_t s_bound[kW];
-  __shared__ int s_n, s_lists, s_end, s_ended, s_last;
+  __shared__ int s_wait[kW], s_n, s_lists, s_end, s_ended, s_last;
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int part = static_cast<int>(blockIdx.x), group = static_cast<int>(blockIdx.z);
   const int first = group * a.W, row = first + static_cast<int>(blockIdx.y);  // the group's first row, and this one
@@ -219,19 +219,12 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
       for (int k = 0; k < G * N; ++k) s += exp_rel(v[k], rel);
       z = {m, s};
       if (e0 == lo && a.N + skip <= 64) {
-        // groups of 64 / M lanes, M >= N + skip: their maxima, and the least of those
-        const int M = a.N + skip;
-        float t = mx == mx ? mx : -INFINITY;
-        auto with = [&](float o, bool within) { t = within ? fmaxf(t, o) : fminf(t, o); };
-        with(__uint_as_float(lane_xor<32>(__float_as_uint(t), lane)), M <= 32);
-        with(__uint_as_float(lane_xor<16>(__float_as_uint(t), lane)), M <= 16);
-        with(__uint_as_float(lane_xor<8>(__float_as_uint(t), lane)), M <= 8);
-        with(__uint_as_float(lane_xor<4>(__float_as_uint(t), lane)), M <= 4);
-        with(__uint_as_float(lane_xor<2>(__float_as_uint(t), lane)), M <= 2);
-        with(__uint_as_float(lane_xor<1>(__float_as_uint(t), lane)), M <= 1);
-        if (t > -INFINITY) {
-          bound = t;
-          sure = ord_key(t);
+        uint32_t top = ord_key(mx == mx ? mx : -INFINITY);
+        sort64(top, lane, false);
+        top = __builtin_amdgcn_readlane(top, a.N + skip - 1);
+        if (key_val(top) > -INFINITY) {
+          bound = key_val(top);
+          sure = top;
         }
       }
       if (!__ballot(mx >= bound)) continue;
@@ -271,8 +264,11 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
     if (whole < hi && wv == 0) {
       const float m = fmaxf(z.m, rest), rel = m == -INFINITY ? 0.0f : m;
       z = {m, z.s * exp_rel(z.m, rel) + exp_rel(rest, rel)};
-      collect(rest, whole + lane, rest >= bound);  // at most 7: there is room
+      collect(rest, whole + lane, rest >= bound);
     }
+    const int listed = min(__popcll(__ballot(best != 0ull)), a.N);
+    if (lane < listed) sh.part.wait[wv][waiting + lane] = best;
+    waiting += listed;
   }
   // the waves' sums and logits as the part's
   z = wave_lse(z);
@@ -280,9 +276,172 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
     s_m[wv] = z.m;
     s_s[wv] = z.s;
     s_bound[wv] = sure;
+    s_wait[wv] = waiting;
   }
   __syncthreads();
   const int slot = row * a.P + part;
+  const int lists = a.W * a.P, entries = lists * a.N;
+  const unsigned long long* keys = a.s.key + static_cast<long long>(first) * a.P * a.N;
+  const int n_ends = a.end_token ? a.W * a.n_stop : 0;
+  // pieces of both ways to go on from here
+  auto part_sum = [&](float* m) {
+    *m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+    double s = 0.0;
+#pragma unroll
+    for (int w = 0; w < kW; ++w) s += static_cast<double>(*m == -INFINITY ? s_s[w] : s_s[w] * exp_rel(s_m[w], *m));
+    return s;
+  };
+  auto last_of_group = [&]() {  // one thread: whether the group's other parts are done
+    const unsigned t = __hip_atomic_fetch_add(&a.s.tick[group * kBeamPad], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (static_cast<int>(t) != lists - 1) return 0;
+    agent_store(&a.s.tick[group * kBeamPad], 0u);
+    return 1;
+  };
+  auto stop_logit = [&](int i, int* b, int* t) {  // of beam b's row, of the stop token t
+    *b = static_cast<int>(divide(static_cast<uint32_t>(i), static_cast<uint32_t>(a.n_stop), a.m_stop));
+    *t = a.stops[i - *b * a.n_stop];
+    return E::get(static_cast<const char*>(a.x) + (first + *b) * a.ld * E::kSize, *t);
+  };
+  auto keep_lse = [&](int b, float top, double s, float sc) {  // NaN for a row that is not live
+    const double lse = static_cast<double>(top) + log(s);
+    s_lse[b] = finite(sc) && __builtin_isfinite(lse) ? lse : NAN;
+    s_score[b] = static_cast<double>(sc);
+  };
+  auto beam_of = [&](int l) { return static_cast<int>(divide(static_cast<uint32_t>(l), static_cast<uint32_t>(a.P), a.m_parts)); };
+  auto entry = [&](uint64_t key, int b) {
+    const double lse = s_lse[b];
+    if (!key || lse != lse) return none();
+    return Cand{ord_f64(s_score[b] + (static_cast<double>(comp_val(key)) - lse)),
+                static_cast<uint64_t>(63 - b) << 52 | key >> 32 << 20 | (key & 0xFFFFFu)};
+  };
+  auto end_entry = [&](float u, int b, int t) { return u > -INFINITY ? entry(comp(ord_key(u), static_cast<uint32_t>(t)), b) : none(); };
+  // its score as fp32 below it, next to zero as well; a key (0: nothing). From such a key a bound for scores
+  auto below_score = [&](const Cand& c) { return c.s ? ord_key(static_cast<float>(f64_ord(c.s))) - 2u : 0u; };
+  auto score_bound = [&](uint32_t k) { return k ? ord_f64(static_cast<double>(key_val(k))) : static_cast<uint64_t>(1); };
+  auto put = [&](int* token, int* parent, float* score, int at, const Cand& c) {
+    const long long o = static_cast<long long>(group) * a.N + at;
+    int b = at;
+    while (b >= a.W) b -= a.W;
+    token[o] = c.s ? static_cast<int>(~static_cast<uint32_t>(c.t) & 0xFFFFFu) : -1;
+    parent[o] = a.row0 + first + (c.s ? 63 - static_cast<int>(c.t >> 52) : b);
+    score[o] = c.s ? static_cast<float>(f64_ord(c.s)) : -INFINITY;
+  };
+
+  if (a.alone) {  // small groups: the first wave does the rest by itself, without waiting for others
+    if (wv != 0) return;
+    const uint32_t most = max(max(s_bound[0], s_bound[1]), max(s_bound[2], s_bound[3]));
+    int n = 0;
+    uint64_t has[kW];
+#pragma unroll
+    for (int w = 0; w < kW; ++w) has[w] = lane < s_wait[w] ? sh.part.wait[w][lane] : 0ull;
+#pragma unroll
+    for (int w = 0; w < kW; ++w) {
+      uint64_t key = has[w];
+      for (int i = lane;;) {
+        const bool take = key != 0 && key >> 32 >= most;
+        const unsigned long long at = __ballot(take);
+        if (take) sh.part.list[n + below(at)] = key;
+        n += __popcll(at);
+        i += 64;
+        if (i - lane >= s_wait[w]) break;
+        key = i < s_wait[w] ? sh.part.wait[w][i] : 0ull;
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+#pragma unroll 1
+    for (int t = lane; t < max(n, a.N); t += 64) {
+      const uint64_t key = t < n ? sh.part.list[t] : 0ull;
+      const int rank = t < n ? count_before(sh.part.list, n, key) : t;
+      if (rank < a.N) agent_store(&a.s.key[slot * a.N + rank], static_cast<unsigned long long>(key));
+    }
+    float m;
+    double s = part_sum(&m);
+    int last = 0;
+    if (lane == 0) {
+      agent_store(&a.s.max[slot], m);
+      agent_store(&a.s.sum[slot], s);
+    }
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    if (lane == 0) last = last_of_group();
+    if (!__builtin_amdgcn_readfirstlane(last)) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    constexpr int kOwn = kNt / 64;
+    uint64_t key[kOwn];
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) key[k] = lane + 64 * k < entries ? agent_load(&keys[lane + 64 * k]) : 0ull;
+    const uint64_t head = lane < lists ? agent_load(&keys[lane * a.N]) : 0ull;
+    const int b = lane >> a.log_s, p = lane & ((1 << a.log_s) - 1);
+    float sc = 0.0f, end_x = -INFINITY;
+    int end_b = 0, end_t = 0;
+    m = -INFINITY;
+    s = 0.0;
+    if (b < a.W && p < a.P) {
+      m = agent_load(&a.s.max[(first + b) * a.P + p]);
+      s = agent_load(&a.s.sum[(first + b) * a.P + p]);
+      sc = a.scores[first + b];
+    }
+    if (lane < n_ends) end_x = stop_logit(lane, &end_b, &end_t);
+    float top = m;
+    if (a.log_s > 0) top = fmaxf(top, __uint_as_float(lane_xor<1>(__float_as_uint(top), lane)));
+    if (a.log_s > 1) top = fmaxf(top, __uint_as_float(lane_xor<2>(__float_as_uint(top), lane)));
+    if (a.log_s > 2) top = fmaxf(top, __uint_as_float(lane_xor<4>(__float_as_uint(top), lane)));
+    if (a.log_s > 3) top = fmaxf(top, __uint_as_float(lane_xor<8>(__float_as_uint(top), lane)));
+    if (a.log_s > 4) top = fmaxf(top, __uint_as_float(lane_xor<16>(__float_as_uint(top), lane)));
+    if (a.log_s > 5) top = fmaxf(top, __uint_as_float(lane_xor<32>(__float_as_uint(top), lane)));
+    if (m != -INFINITY) s *= static_cast<double>(exp_rel(m, top));  // (a sum at -inf is 0 or NaN)
+    auto f64 = [](uint64_t v) { return __longlong_as_double(static_cast<long long>(v)); };
+    auto u64 = [](double v) { return static_cast<uint64_t>(__double_as_longlong(v)); };
+    if (a.log_s > 0) s += f64(lane_xor<1>(u64(s), lane));
+    if (a.log_s > 1) s += f64(lane_xor<2>(u64(s), lane));
+    if (a.log_s > 2) s += f64(lane_xor<4>(u64(s), lane));
+    if (a.log_s > 3) s += f64(lane_xor<8>(u64(s), lane));
+    if (a.log_s > 4) s += f64(lane_xor<16>(u64(s), lane));
+    if (a.log_s > 5) s += f64(lane_xor<32>(u64(s), lane));
+    if (b < a.W && p == 0) keep_lse(b, top, s, sc);
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    // the N-th of the lists' first entries: a bound for all entries
+    uint32_t t = lane < lists ? below_score(entry(head, beam_of(lane))) : 0u;
+    sort64(t, lane, false);
+    const uint64_t bound = score_bound(__builtin_amdgcn_readlane(t, a.N - 1));
+    Cand c[kOwn];
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) {
+      const int l = static_cast<int>(divide(static_cast<uint32_t>(min(lane + 64 * k, entries - 1)), static_cast<uint32_t>(a.N), a.m_n));
+      c[k] = entry(key[k], beam_of(l));
+    }
+    int c_n = 0;
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) {
+      const unsigned long long at = __ballot(c[k].s >= bound);
+      if (c[k].s >= bound) sh.group.cand[c_n + below(at)] = c[k];
+      c_n += __popcll(at);
+    }
+    const Cand end = end_entry(end_x, end_b, end_t);
+    const unsigned long long at = __ballot(end.s >= bound);
+    if (end.s >= bound) sh.group.end[below(at)] = end;
+    const int ends = __popcll(at);
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+#pragma unroll 1
+    for (int i = lane; i < max(c_n, a.N); i += 64) {
+      const Cand o = i < c_n ? sh.group.cand[i] : none();
+      const int rank = i < c_n ? count_before(sh.group.cand, c_n, o) : i;
+      if (rank < a.N) put(a.token, a.parent, a.score, rank, o);
+    }
+    if (!a.end_token) return;
+    bool ended = false;
+    if (end.s >= bound) {
+      const int rank = count_before(sh.group.end, ends, end);
+      ended = rank + count_before(sh.group.cand, c_n, end) < a.N;
+      if (ended) put(a.end_token, a.end_parent, a.end_score, rank, end);
+    }
+    const int n_end = __popcll(__ballot(ended));
+    if (lane >= n_end && lane < a.N) put(a.end_token, a.end_parent, a.end_score, lane, none());
+    if (lane == 0) a.n_end[group] = n_end;
+    return;
+  }
+
   {
     const uint32_t most = max(max(s_bound[0], s_bound[1]), max(s_bound[2], s_bound[3]));
     auto give = [&](uint64_t key) {
@@ -294,9 +453,8 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
       to = __builtin_amdgcn_readfirstlane(to) + below(at);
       if (take) sh.part.list[to] = key;
     };
-    give(lane < waiting ? sh.part.wait[wv][lane] : 0ull);
-    if (waiting > 64) give(lane + 64 < waiting ? sh.part.wait[wv][lane + 64] : 0ull);
-    if (__ballot(best != 0)) give(best);
+#pragma unroll 1
+    for (int i = lane; i < (waiting + 63 & ~63); i += 64) give(i < waiting ? sh.part.wait[wv][i] : 0ull);
   }
   __syncthreads();
   // hand over through the device's memory: agent-scope stores, completed before the ticket is taken; the part
@@ -309,10 +467,8 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
     if (rank < a.N) agent_store(&a.s.key[slot * a.N + rank], static_cast<unsigned long long>(key));
   }
   if (wv == kW - 1) {  // (the last wave has no logits to rank, mostly)
-    const float m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-    double s = 0.0;
-#pragma unroll
-    for (int w = 0; w < kW; ++w) s += static_cast<double>(m == -INFINITY ? s_s[w] : s_s[w] * exp_rel(s_m[w], m));
+    float m;
+    const double s = part_sum(&m);
     if (lane == 0) {
       agent_store(&a.s.max[slot], m);
       agent_store(&a.s.sum[slot], s);
@@ -323,27 +479,17 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
   __syncthreads();
   if (tid == 0) {
-    const unsigned t = __hip_atomic_fetch_add(&a.s.tick[group * kBeamPad], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    s_last = static_cast<int>(t) == a.W * a.P - 1;
+    s_last = last_of_group();
     s_n = s_lists = s_end = s_ended = 0;
   }
   __syncthreads();
   if (!s_last) return;
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-  if (tid == 0) agent_store(&a.s.tick[group * kBeamPad], 0u);
-  const int lists = a.W * a.P, entries = lists * a.N;
   const bool few = entries <= kNt;  // an entry a thread
-  const unsigned long long* keys = a.s.key + static_cast<long long>(first) * a.P * a.N;
 
   // what does not wait for the rows' sums is loaded first
   const uint64_t mine = few && tid < entries ? agent_load(&keys[tid]) : 0ull;
   const uint64_t head = tid < lists ? agent_load(&keys[tid * a.N]) : 0ull;
-  const int n_ends = a.end_token ? a.W * a.n_stop : 0;
-  auto stop_logit = [&](int i, int* b, int* t) {  // of beam b's row, of the stop token t
-    *b = static_cast<int>(divide(static_cast<uint32_t>(i), static_cast<uint32_t>(a.n_stop), a.m_stop));
-    *t = a.stops[i - *b * a.n_stop];
-    return E::get(static_cast<const char*>(a.x) + (first + *b) * a.ld * E::kSize, *t);
-  };
   float end_x = -INFINITY;
   int end_b = 0, end_t = 0;
   if (tid < n_ends) end_x = stop_logit(tid, &end_b, &end_t);
@@ -364,47 +510,23 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
     if (m != -INFINITY) s *= static_cast<double>(exp_rel(m, top));  // (a sum at -inf is 0 or NaN)
 #pragma unroll 1
     for (int d = 1 << a.log_s >> 1; d; d >>= 1) s += __shfl_xor(s, d);
-    if (b < a.W && p == 0) {
-      const double lse = static_cast<double>(top) + log(s);
-      s_lse[b] = finite(sc) && __builtin_isfinite(lse) ? lse : NAN;
-      s_score[b] = static_cast<double>(sc);
-    }
+    if (b < a.W && p == 0) keep_lse(b, top, s, sc);
   }
   __syncthreads();
-  auto beam_of = [&](int l) { return static_cast<int>(divide(static_cast<uint32_t>(l), static_cast<uint32_t>(a.P), a.m_parts)); };
-  auto entry = [&](uint64_t key, int b) {
-    const double lse = s_lse[b];
-    if (!key || lse != lse) return none();
-    return Cand{ord_f64(s_score[b] + (static_cast<double>(comp_val(key)) - lse)),
-                static_cast<uint64_t>(63 - b) << 52 | key >> 32 << 20 | (key & 0xFFFFFu)};
-  };
-  auto put = [&](int* token, int* parent, float* score, int at, const Cand& c) {
-    const long long o = static_cast<long long>(group) * a.N + at;
-    int b = at;
-    while (b >= a.W) b -= a.W;
-    token[o] = c.s ? static_cast<int>(~static_cast<uint32_t>(c.t) & 0xFFFFFu) : -1;
-    parent[o] = a.row0 + first + (c.s ? 63 - static_cast<int>(c.t >> 52) : b);
-    score[o] = c.s ? static_cast<float>(f64_ord(c.s)) : -INFINITY;
-  };
-  // the N-th of the first entries that a wave's threads have, their scores as fp32 below them (next to zero as well): the
-  // largest of the waves' is a bound for all entries
-  auto below_score = [&](uint64_t key, int l) {
-    const Cand c = entry(key, beam_of(l));
-    return c.s ? ord_key(static_cast<float>(f64_ord(c.s))) - 2u : 0u;
-  };
-  uint32_t top = tid < lists ? below_score(head, tid) : 0u;
+  // the N-th of the first entries that a wave's threads have, their scores as fp32 below them: the largest of the
+  // waves' is a bound for all entries
+  uint32_t top = tid < lists ? below_score(entry(head, beam_of(tid))) : 0u;
 #pragma unroll 1
-  for (int l = tid + kNt; l < lists; l += kNt) top = max(top, below_score(agent_load(&keys[l * a.N]), l));
+  for (int l = tid + kNt; l < lists; l += kNt) top = max(top, below_score(entry(agent_load(&keys[l * a.N]), beam_of(l))));
   if (wv * 64 < lists) sort64(top, lane, false);
   if (lane == a.N - 1) s_bound[wv] = top;
   __syncthreads();
-  const uint32_t most = max(max(s_bound[0], s_bound[1]), max(s_bound[2], s_bound[3]));
-  const uint64_t bound = most ? ord_f64(static_cast<double>(key_val(most))) : 1ull;
+  const uint64_t bound = score_bound(max(max(s_bound[0], s_bound[1]), max(s_bound[2], s_bound[3])));
   // the stop tokens' continuations; N others come before those that do not reach the bound
 #pragma unroll 1
   for (int i = tid; i < n_ends; i += kNt) {
     if (i >= kNt) end_x = stop_logit(i, &end_b, &end_t);
-    const Cand c = end_x > -INFINITY ? entry(comp(ord_key(end_x), static_cast<uint32_t>(end_t)), end_b) : none();
+    const Cand c = end_entry(end_x, end_b, end_t);
     if (c.s >= bound) sh.group.end[atomicAdd(&s_end, 1)] = c;
   }
   // the entries that reach it: of all lists, or of those whose first one does
@@ -497,6 +619,7 @@ void launch_beam(BeamArgs a, int dtype, hipStream_t st) {
   a.m_stop = a.n_stop ? 0xFFFFFFFFu / static_cast<uint32_t>(a.n_stop) : 0u;
   a.log_s = 0;
   while (1 << a.log_s < a.P) ++a.log_s;
+  a.alone = a.W << a.log_s <= 64 && a.W * a.P * a.N <= kNt && a.W * a.n_stop <= 64 && a.N <= 16;
   const dim3 grid(static_cast<unsigned>(a.P), static_cast<unsigned>(a.W), static_cast<unsigned>(a.G));
   if (dtype == VSMP_F32)
     hipLaunchKernelGGL(k_beam<F32>, grid, dim3(kNt), 0, st, a);

@@ -43,7 +43,8 @@ struct BeamArgs {
   int stops[kBeamStops];
   int n_stop;
   uint32_t m_parts, m_n, m_stop;  // (2^32 - 1) / P, N, n_stop (launch_beam)
-  int log_s;                      // lanes of a row's parts in the last part, a power of two
+  int log_s;                      // lanes of a row's parts in the last part: 2^log_s
+  bool alone;                     // a wave ends a part and a group by itself
   int* token;
   int* parent;
   float* score;
