@@ -135,7 +135,7 @@ constexpr int kWait = 144;     // logits that a wave has collected: 64 that wait
 // thread each: mostly they are few more than N.
 //
 // The last part of a group ranks its rows' lists by score in the same way: the N-th largest first entry of the lists (of
-// those of a wave's threads) is a bound for all entries. Where more entries than kCands reach it (many equal
+// those of a wave's threads; several of each list where there are few) is a bound for all entries. Where more entries than kCands reach it (many equal
 // ones) each wave merges lists in order instead, and the first wave the waves'.
 //
 // A few rows are bound by latencies, those of fetching the code among them: every workgroup runs most of it once. So loops
@@ -201,6 +201,15 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
       if (take) sh.part.wait[wv][waiting + below(at)] = comp(ord_key(u), static_cast<uint32_t>(e));
       waiting += __popcll(at);
     };
+    int known = 64;              // of those that wait, how many the bound takes into account
+    auto sharpen = [&]() {       // the N-th of the first 64 that wait
+      __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+      uint32_t top = lane < waiting ? static_cast<uint32_t>(sh.part.wait[wv][lane] >> 32) : 0u;
+      sort64(top, lane, false);
+      top = __builtin_amdgcn_readlane(top, a.N - 1);
+      sure = max(sure, top);
+      known = waiting;
+    };
     for (int e0 = lo; e0 < whole; e0 += kStep) {
       float v[G * N], gm[G];
 #pragma unroll
@@ -214,14 +223,23 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
       }
       const float mx = fmaxf(fmaxf(gm[0], gm[1]), fmaxf(gm[2], gm[3]));
       const float m = fmaxf(z.m, mx), rel = m == -INFINITY ? 0.0f : m;  // of -inf alone: exp(-inf - 0) = 0, and NaN stays
-      float s = z.s * exp_rel(z.m, rel);
+      // exp(x - rel) as 2^(x log2e - r), one operation less a logit; r is rel log2e rounded, which the sum makes good
+      const float r2 = rel * kLog2e;
+      float s = 0.0f;
+      if (!__ballot(!(fabsf(r2) < 3e38f))) {
 #pragma unroll
-      for (int k = 0; k < G * N; ++k) s += exp_rel(v[k], rel);
-      z = {m, s};
+        for (int k = 0; k < G * N; ++k) s += __builtin_amdgcn_exp2f(fmaf(v[k], kLog2e, -r2));
+        s = fmaf(s, -0.693147181f * fmaf(rel, kLog2e, -r2), s);
+      } else {  // infinite or next to it
+#pragma unroll
+        for (int k = 0; k < G * N; ++k) s += exp_rel(v[k], rel);
+      }
+      z = {m, fmaf(z.s, exp_rel(z.m, rel), s)};
       if (e0 == lo && a.N + skip <= 64) {
         uint32_t top = ord_key(mx == mx ? mx : -INFINITY);
         sort64(top, lane, false);
         top = __builtin_amdgcn_readlane(top, a.N + skip - 1);
+        known = a.N;
         if (key_val(top) > -INFINITY) {
           bound = key_val(top);
           sure = top;
@@ -254,10 +272,12 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
         merge64(best, w, lane);
         const uint32_t nth = __builtin_amdgcn_readlane(static_cast<uint32_t>(best >> 32), a.N - 1);
         if (nth) {
-          sure = nth;
+          sure = max(sure, nth);
           bound = fmaxf(bound, key_val(nth));
+          known = 0;
         }
       }
+      if (waiting > known + max(4, a.N / 2)) sharpen();
       // what comes in later steps has higher tokens: among equal logits it is behind those that N have reached
       if (sure) bound = fmaxf(bound, next_up(key_val(sure)));
     }
@@ -266,6 +286,7 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
       z = {m, z.s * exp_rel(z.m, rel) + exp_rel(rest, rel)};
       collect(rest, whole + lane, rest >= bound);
     }
+    if (waiting > known + 8) sharpen();
     const int listed = min(__popcll(__ballot(best != 0ull)), a.N);
     if (lane < listed) sh.part.wait[wv][waiting + lane] = best;
     waiting += listed;
@@ -307,6 +328,8 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
     s_lse[b] = finite(sc) && __builtin_isfinite(lse) ? lse : NAN;
     s_score[b] = static_cast<double>(sc);
   };
+  const int heads = lists << a.log_j;  // the lists' first entries, 2^log_j of each
+  auto head_of = [&](int i) { return agent_load(&keys[(i >> a.log_j) * a.N + (i & ((1 << a.log_j) - 1))]); };
   auto beam_of = [&](int l) { return static_cast<int>(divide(static_cast<uint32_t>(l), static_cast<uint32_t>(a.P), a.m_parts)); };
   auto entry = [&](uint64_t key, int b) {
     const double lse = s_lse[b];
@@ -371,7 +394,7 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
     uint64_t key[kOwn];
 #pragma unroll
     for (int k = 0; k < kOwn; ++k) key[k] = lane + 64 * k < entries ? agent_load(&keys[lane + 64 * k]) : 0ull;
-    const uint64_t head = lane < lists ? agent_load(&keys[lane * a.N]) : 0ull;
+    const uint64_t head = lane < heads ? head_of(lane) : 0ull;
     const int b = lane >> a.log_s, p = lane & ((1 << a.log_s) - 1);
     float sc = 0.0f, end_x = -INFINITY;
     int end_b = 0, end_t = 0;
@@ -402,7 +425,7 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
     if (b < a.W && p == 0) keep_lse(b, top, s, sc);
     __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
     // the N-th of the lists' first entries: a bound for all entries
-    uint32_t t = lane < lists ? below_score(entry(head, beam_of(lane))) : 0u;
+    uint32_t t = lane < heads ? below_score(entry(head, beam_of(lane >> a.log_j))) : 0u;
     sort64(t, lane, false);
     const uint64_t bound = score_bound(__builtin_amdgcn_readlane(t, a.N - 1));
     Cand c[kOwn];
@@ -489,7 +512,7 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
 
   // what does not wait for the rows' sums is loaded first
   const uint64_t mine = few && tid < entries ? agent_load(&keys[tid]) : 0ull;
-  const uint64_t head = tid < lists ? agent_load(&keys[tid * a.N]) : 0ull;
+  const uint64_t head = tid < heads ? head_of(tid) : 0ull;
   float end_x = -INFINITY;
   int end_b = 0, end_t = 0;
   if (tid < n_ends) end_x = stop_logit(tid, &end_b, &end_t);
@@ -515,10 +538,10 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
   __syncthreads();
   // the N-th of the first entries that a wave's threads have, their scores as fp32 below them: the largest of the
   // waves' is a bound for all entries
-  uint32_t top = tid < lists ? below_score(entry(head, beam_of(tid))) : 0u;
+  uint32_t top = tid < heads ? below_score(entry(head, beam_of(tid >> a.log_j))) : 0u;
 #pragma unroll 1
-  for (int l = tid + kNt; l < lists; l += kNt) top = max(top, below_score(entry(agent_load(&keys[l * a.N]), beam_of(l))));
-  if (wv * 64 < lists) sort64(top, lane, false);
+  for (int i = tid + kNt; i < heads; i += kNt) top = max(top, below_score(entry(head_of(i), beam_of(i >> a.log_j))));
+  if (wv * 64 < heads) sort64(top, lane, false);
   if (lane == a.N - 1) s_bound[wv] = top;
   __syncthreads();
   const uint64_t bound = score_bound(max(max(s_bound[0], s_bound[1]), max(s_bound[2], s_bound[3])));
@@ -601,12 +624,13 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
 
 }  // namespace
 
-void beam_parts(int B, int V, int dtype, int cus, int* P, int* L) {
+void beam_parts(int B, int W, int V, int dtype, int cus, int* P, int* L) {
   const int step = kNt * 4 * (dtype == VSMP_F32 ? 4 : 8);
   const int steps = (V + step - 1) / step;
-  int p = (4 * cus + B - 1) / B;
+  int p = 4 * cus / B;
   if (p > steps) p = steps;
-  if (p > 64) p = 64;  // a lane each reads their results
+  if (p > kNt / W) p = kNt / W;  // the group's last part reads a list a thread
+  if (p > 64) p = 64;            // and a row's sums side by side in a wave
   if (p > kBeamSlots / B) p = kBeamSlots / B;
   if (p < 1) p = 1;
   *L = (steps + p - 1) / p * step;
@@ -619,7 +643,11 @@ void launch_beam(BeamArgs a, int dtype, hipStream_t st) {
   a.m_stop = a.n_stop ? 0xFFFFFFFFu / static_cast<uint32_t>(a.n_stop) : 0u;
   a.log_s = 0;
   while (1 << a.log_s < a.P) ++a.log_s;
-  a.alone = a.W << a.log_s <= 64 && a.W * a.P * a.N <= kNt && a.W * a.n_stop <= 64 && a.N <= 16;
+  // as many first entries of each list as make a sharp bound: few lists have most of the best
+  const int lists = a.W * a.P;
+  a.alone = a.W << a.log_s <= 64 && lists * a.N <= kNt && lists <= 64 && a.W * a.n_stop <= 64 && a.N <= 16;
+  a.log_j = 0;
+  while (2 << a.log_j <= a.N && lists << a.log_j <= (a.alone ? 64 : kNt) / 2) ++a.log_j;
   const dim3 grid(static_cast<unsigned>(a.P), static_cast<unsigned>(a.W), static_cast<unsigned>(a.G));
   if (dtype == VSMP_F32)
     hipLaunchKernelGGL(k_beam<F32>, grid, dim3(kNt), 0, st, a);

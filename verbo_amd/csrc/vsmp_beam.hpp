@@ -44,6 +44,7 @@ struct BeamArgs {
   int n_stop;
   uint32_t m_parts, m_n, m_stop;  // (2^32 - 1) / P, N, n_stop (launch_beam)
   int log_s;                      // lanes of a row's parts in the last part: 2^log_s
+  int log_j;                      // entries of each list that make its bound: 2^log_j
   bool alone;                     // a wave ends a part and a group by itself
   int* token;
   int* parent;
@@ -105,8 +106,8 @@ struct PageArgs {
   PageScratch s;
 };
 
-// Parts and part length of vsmp_beam_select's rows: B = G * W.
-void beam_parts(int B, int V, int dtype, int cus, int* P, int* L);
+// Parts and part length of vsmp_beam_select's rows: B of them, W a group.
+void beam_parts(int B, int W, int V, int dtype, int cus, int* P, int* L);
 void launch_beam(BeamArgs a, int dtype, hipStream_t st);
 void launch_reorder(const ReorderArgs& a, int groups, int cus, hipStream_t st);
 void launch_pages_step(const PageArgs& a, int cus, hipStream_t st);

@@ -140,7 +140,7 @@ int vsmp_beam_select(vsmp_ctx* ctx, const void* logits, int dtype, long long ld,
       a.end_score = end_score + out;
       a.n_end = n_end + g;
     }
-    vsmp::beam_parts(a.G * W, V, dtype, vsmp::ctx_cus(ctx), &a.P, &a.L);
+    vsmp::beam_parts(a.G * W, W, V, dtype, vsmp::ctx_cus(ctx), &a.P, &a.L);
     vsmp::launch_beam(a, dtype, st);
     if (!vsmp::hip_ok(hipGetLastError(), "beam launch")) return -1;
   }
