@@ -73,6 +73,7 @@ struct ReorderArgs {
   const int* parent;         // of the whole batch
   const int* len;            // null: all tokens
   int width;
+  int unit;                  // 0: tokens are whole columns; else bytes that divide a token (launch_reorder)
 };
 
 struct PageCopy {
@@ -109,7 +110,7 @@ struct PageArgs {
 // Parts and part length of vsmp_beam_select's rows: B of them, W a group.
 void beam_parts(int B, int W, int V, int dtype, int cus, int* P, int* L);
 void launch_beam(BeamArgs a, int dtype, hipStream_t st);
-void launch_reorder(const ReorderArgs& a, int groups, int cus, hipStream_t st);
+void launch_reorder(ReorderArgs a, int groups, int cus, hipStream_t st);
 void launch_pages_step(const PageArgs& a, int cus, hipStream_t st);
 void launch_pages_compact(const PageArgs& a, int cus, hipStream_t st);
 

@@ -24,12 +24,47 @@ __device__ __forceinline__ T agent_add(T* p, T v) {
 
 // ---- k_reorder -------------------------------------------------------------------------------------------
 
+template <int B>
+using Column = uint32_t __attribute__((ext_vector_type(B / 4), aligned(1)));
+// A plane's bytes are device memory: the compiler cannot know from an address that is loaded, and would take instructions
+// that serve LDS and the stack as well.
+typedef __attribute__((address_space(1))) char Bytes;
+__device__ __forceinline__ Bytes* plane_at(const PlaneArgs& p, uint32_t i) { return (Bytes*)p.planes[i]; }
+template <class T>
+__device__ __forceinline__ T get(const Bytes* p) {
+  return *(const __attribute__((address_space(1))) T*)p;
+}
+template <class T>
+__device__ __forceinline__ void set(Bytes* p, T v) {
+  *(__attribute__((address_space(1))) T*)p = v;
+}
+
+template <class T>
+using Loose __attribute__((aligned(1))) = T;
+
+// A column in which tokens may end, unit by unit: whole units, since a token is.
+template <int MAXW, int B, class T>
+__device__ __forceinline__ void ends(Bytes* base, uint32_t at, int n, const long long* from, const long long* to, const int* bytes) {
+#pragma unroll 1
+  for (uint32_t k = 0; k < B; k += sizeof(T)) {
+    asm volatile("" ::: "memory");
+    T v[MAXW];
+#pragma unroll
+    for (int i = 0; i < MAXW; ++i)
+      if (i < n && at + k < static_cast<uint32_t>(bytes[i])) v[i] = get<Loose<T>>(base + k + from[i]);
+#pragma unroll
+    for (int i = 0; i < MAXW; ++i)
+      if (i < n && at + k < static_cast<uint32_t>(bytes[i])) set<Loose<T>>(base + k + to[i], v[i]);
+  }
+}
+
 // A column of B bytes over a group's rows belongs to one thread, which loads it from every parent before it stores it in
-// any row: in place without a wait. Rows that stay are neither read nor written for themselves; a parent with several
+// any row: in place without a wait. Where tokens are no whole columns (a.unit: 4, 2 or 1 bytes, which they are in whole), the
+// columns beyond the least of the rows' ends go unit by unit. Rows that stay are neither read nor written for themselves; a parent with several
 // children is read by each of their loads, from memory once.
 template <int MAXW, int B>
 __global__ __launch_bounds__(kNt) void k_reorder(ReorderArgs a) {
-  typedef uint32_t vec __attribute__((ext_vector_type(B / 4), aligned(1)));
+  typedef Column<B> vec;
   __shared__ long long s_from[MAXW], s_to[MAXW];  // of the rows that move: where their parents and they lie in a plane
   __shared__ int s_bytes[MAXW];                   // and what they take of each piece
   __shared__ int s_n, s_most, s_least;
@@ -67,27 +102,30 @@ __global__ __launch_bounds__(kNt) void k_reorder(ReorderArgs a) {
   const uint32_t pieces = static_cast<uint32_t>(a.p.pieces), mp = 0xFFFFFFFFu / pieces;
   const uint32_t total = static_cast<uint32_t>(a.p.n_planes) * pieces * cols;
   for (uint32_t idx = blockIdx.x * kNt + tid; idx < total; idx += gridDim.x * kNt) {
+    asm volatile("" ::: "memory");  // the rows' places are read from LDS when they are used: all of them in registers leave no waves
     const uint32_t run = divide(idx, cols, m), at = (idx - run * cols) * B;
     const uint32_t plane = divide(run, pieces, mp), piece = run - plane * pieces;
-    char* base = static_cast<char*>(a.p.planes[a.plane0 + plane]) + piece * a.p.piece_stride + at;
+    Bytes* base = plane_at(a.p, a.plane0 + plane) + piece * a.p.piece_stride + at;
     if (at + B <= least) {
       vec v[MAXW];
 #pragma unroll
       for (int i = 0; i < MAXW; ++i)
-        if (i < n) v[i] = *reinterpret_cast<const vec*>(base + s_from[i]);
+        if (i < n) v[i] = get<vec>(base + s_from[i]);
 #pragma unroll
       for (int i = 0; i < MAXW; ++i)
-        if (i < n) *reinterpret_cast<vec*>(base + s_to[i]) = v[i];
-    } else {  // the end of some row's tokens: byte by byte, each a column of its own
-      for (int k = 0; k < B; ++k) {
-        uint8_t v[MAXW];
+        if (i < n) set<vec>(base + s_to[i], v[i]);
+    } else if (a.unit) {  // beyond some row's tokens
+      if (a.unit == 4) ends<MAXW, B, uint32_t>(base, at, n, s_from, s_to, s_bytes);
+      else if (a.unit == 2) ends<MAXW, B, uint16_t>(base, at, n, s_from, s_to, s_bytes);
+      else ends<MAXW, B, uint8_t>(base, at, n, s_from, s_to, s_bytes);
+    } else {
+      vec v[MAXW];
 #pragma unroll
-        for (int i = 0; i < MAXW; ++i)
-          if (i < n && at + k < static_cast<uint32_t>(s_bytes[i])) v[i] = *reinterpret_cast<const uint8_t*>(base + k + s_from[i]);
+      for (int i = 0; i < MAXW; ++i)
+        if (i < n && at < static_cast<uint32_t>(s_bytes[i])) v[i] = get<vec>(base + s_from[i]);
 #pragma unroll
-        for (int i = 0; i < MAXW; ++i)
-          if (i < n && at + k < static_cast<uint32_t>(s_bytes[i])) *reinterpret_cast<uint8_t*>(base + k + s_to[i]) = v[i];
-      }
+      for (int i = 0; i < MAXW; ++i)
+        if (i < n && at < static_cast<uint32_t>(s_bytes[i])) set<vec>(base + s_to[i], v[i]);
     }
   }
 }
@@ -284,13 +322,13 @@ __global__ __launch_bounds__(kTakeNt) void k_pages_take(PageArgs a) {
 
 // Tokens of a page into another page of a plane: one chunk, four 16-byte columns a thread.
 __device__ __forceinline__ void copy_tokens(const PlaneArgs& c, int plane, int src, int dst, int tokens, uint32_t chunk) {
-  typedef uint32_t vec __attribute__((ext_vector_type(4), aligned(1)));
+  typedef Column<16> vec;
   const uint32_t run = static_cast<uint32_t>(tokens) * static_cast<uint32_t>(c.token_bytes);
   const uint32_t cols = (run + 15) / 16, m = 0xFFFFFFFFu / cols;
   const uint32_t total = cols * static_cast<uint32_t>(c.pieces);
-  char* base = static_cast<char*>(c.planes[plane]);
-  const char* from = base + src * c.row_stride;
-  char* to = base + dst * c.row_stride;
+  Bytes* base = plane_at(c, static_cast<uint32_t>(plane));
+  const Bytes* from = base + src * c.row_stride;
+  Bytes* to = base + dst * c.row_stride;
   vec v[4];
   long long off[4];
   int n[4];
@@ -302,16 +340,19 @@ __device__ __forceinline__ void copy_tokens(const PlaneArgs& c, int plane, int s
       const uint32_t piece = divide(idx, cols, m), at = (idx - piece * cols) * 16;
       off[k] = piece * c.piece_stride + at;
       n[k] = static_cast<int>(min(run - at, 16u));
-      if (n[k] == 16) v[k] = *reinterpret_cast<const vec*>(from + off[k]);
+      if (n[k] == 16) v[k] = get<vec>(from + off[k]);
     }
   }
 #pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (n[k] == 16) set<vec>(to + off[k], v[k]);
+  // the runs' ends
+#pragma unroll
   for (int k = 0; k < 4; ++k) {
-    if (n[k] == 16) {
-      *reinterpret_cast<vec*>(to + off[k]) = v[k];
-    } else {
-      for (int b = 0; b < n[k]; ++b) to[off[k] + b] = from[off[k] + b];
-    }
+    if (n[k] == 0 || n[k] == 16) continue;
+    int b = 0;
+    for (; b + 4 <= n[k]; b += 4) set<Loose<uint32_t>>(to + off[k] + b, get<Loose<uint32_t>>(from + off[k] + b));
+    for (; b < n[k]; ++b) set(to + off[k] + b, get<uint8_t>(from + off[k] + b));
   }
 }
 __device__ __forceinline__ uint32_t chunks_of(const PlaneArgs& c, int tokens) {
@@ -426,8 +467,9 @@ void go_reorder(const ReorderArgs& a, int groups, int blocks, hipStream_t st) {
 
 }  // namespace
 
-void launch_reorder(const ReorderArgs& a, int groups, int cus, hipStream_t st) {
+void launch_reorder(ReorderArgs a, int groups, int cus, hipStream_t st) {
   const int bytes = a.width <= 32 ? 16 : 8;
+  a.unit = a.p.token_bytes % bytes == 0 ? 0 : a.p.token_bytes % 4 == 0 ? 4 : a.p.token_bytes % 2 == 0 ? 2 : 1;
   const long long cols = (static_cast<long long>(a.p.tokens) * a.p.token_bytes + bytes - 1) / bytes * a.p.n_planes * a.p.pieces;
   const long long most = (cols + kNt - 1) / kNt;
   const int blocks = static_cast<int>(std::max<long long>(1, std::min<long long>(most, (32ll * cus + groups - 1) / groups)));
