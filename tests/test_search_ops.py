@@ -484,13 +484,16 @@ class Cache:
     (8, 5, 64, 16, True, "f32"),
     (1, 3, 2, 5, False, "i32"),
     (33, 4, 4500, 8, False, "i32"),  # more pages than one workgroup's
+    (12, 9, 65536, 2, False, "i32"),
+    (9, 9, 65537, 2, False, "i32"),  # a pool whose step is more than one launch
+    (1025, 3, 1500, 2, False, "i32"),
 ])
 def test_pages_any_steps(ctx, rows, row_pages, n_pages, T, by_head, dtype):
     """Thirty steps of any kind: forks, cuts, ends, growth by one token and by several pages, rows that do not fit."""
     log("pages", rows, n_pages, T)
     rng = np.random.default_rng(rows * 100 + T)
     c = Cache(ctx, rows, row_pages, n_pages, T, by_head=by_head, dtype=dtype)
-    for k in range(30):
+    for k in range(30 if rows < 100 else 4):
         parent = rng.integers(-1, rows + (k % 5 == 4), rows) if k % 3 else rng.integers(0, rows, rows)
         add = rng.choice([-T - 1, -1, 0, 1, 1, 1, 2, T, 3 * T + 1], rows)
         if k % 7 == 6:

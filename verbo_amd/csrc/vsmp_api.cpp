@@ -947,6 +947,7 @@ bool page_scratch(vsmp_ctx* c, hipStream_t st, PageScratch* out) {
     take(out->room, kPagesMax);
     take(out->copies, kPageRows);
     take(out->n_copies, 1);
+    take(out->n_moves, 1);
     take(out->tick, 1);
   };
   lay();

@@ -81,14 +81,15 @@ struct PageCopy {
 };
 
 // Device scratch of vsmp_pages_step and vsmp_pages_compact: allocated by a context's first call of either, never
-// replaced. delta, writers, order and tick are zero between calls.
+// replaced. delta, writers, order, n_moves and tick are zero between calls.
 struct PageScratch {
   int* delta;                   // [kPagesMax]: holders that a page gains
   int* writers;                 // [kPagesMax]: rows that grow in a begun page
   unsigned long long* order;    // [kPagesMax]: the largest of their tokens << 32 | ~row
   unsigned long long* bits;     // [kPagesMax / 64]: pages that are free (step) or in use (compact)
   int* before;                  // [kPagesMax / 64 + 1]: compact: pages in use before each word
-  int* moves;                   // [kPagesMax]: compact: the pages in use at n and beyond
+  int* moves;                   // [kPagesMax]: compact: the pages in use at n and beyond; step: pages whose holders change
+  int* n_moves;                 // step: how many, with repetitions
   int* room;                    // [kPagesMax]: compact: the free pages below n
   PageCopy* copies;             // [kPageRows]
   int* n_copies;
@@ -104,6 +105,7 @@ struct PageArgs {
   int* moved;
   int* live;
   PlaneArgs cache;              // n_planes 0: none
+  uint32_t m_cap;               // (2^32 - 1) / to.row_pages (launch_pages_step)
   PageScratch s;
 };
 
@@ -111,7 +113,7 @@ struct PageArgs {
 void beam_parts(int B, int W, int V, int dtype, int cus, int* P, int* L);
 void launch_beam(BeamArgs a, int dtype, hipStream_t st);
 void launch_reorder(ReorderArgs a, int groups, int cus, hipStream_t st);
-void launch_pages_step(const PageArgs& a, int cus, hipStream_t st);
+void launch_pages_step(PageArgs a, int cus, hipStream_t st);
 void launch_pages_compact(const PageArgs& a, int cus, hipStream_t st);
 
 }  // namespace vsmp

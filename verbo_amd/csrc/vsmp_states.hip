@@ -63,7 +63,7 @@ __device__ __forceinline__ void ends(Bytes* base, uint32_t at, int n, const long
 // columns beyond the least of the rows' ends go unit by unit. Rows that stay are neither read nor written for themselves; a parent with several
 // children is read by each of their loads, from memory once.
 template <int MAXW, int B>
-__global__ __launch_bounds__(kNt) void k_reorder(ReorderArgs a) {
+__global__ __launch_bounds__(kNt, MAXW == 8 ? 4 : 1) void k_reorder(ReorderArgs a) {
   typedef Column<B> vec;
   __shared__ long long s_from[MAXW], s_to[MAXW];  // of the rows that move: where their parents and they lie in a plane
   __shared__ int s_bytes[MAXW];                   // and what they take of each piece
@@ -206,6 +206,29 @@ __device__ __forceinline__ int scan_before(int v, int* total) {
   return before + at - v;
 }
 
+// The free page of rank k goes to the row that asks for the k-th page: a wave takes a word, a lane a page. start: pages
+// that the rows before a row ask for; first: where in the table its new pages begin; before: free pages before each word.
+template <int NT, class Bits>
+__device__ __forceinline__ void give_pages(const PageArgs& a, int words, int asked, int n_free, const int* start, const int* first,
+                                           const int* before, Bits bits) {
+  const int lane = threadIdx.x & 63, R = a.to.rows;
+  for (int w = threadIdx.x >> 6; w < words && before[w] < asked; w += NT / 64) {
+    const unsigned long long b = bits(w);
+    const int k = before[w] + __popcll(b & ((1ull << lane) - 1ull));
+    if (!(b >> lane & 1ull) || k >= asked) continue;
+    // the last row that starts at or before it: rows that ask for nothing start where the next one does
+    int lo = 0, hi = R - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (start[mid] <= k) lo = mid;
+      else hi = mid - 1;
+    }
+    if ((lo + 1 < R ? start[lo + 1] : asked) > n_free) continue;  // the row does not get all of its pages, and so none
+    a.to.table[lo * a.to.ldt + first[lo] + (k - start[lo])] = w * 64 + lane;
+    agent_store(&a.to.ref[w * 64 + lane], 1);
+  }
+}
+
 // The next ref, and the free pages as bits; then, in the last workgroup, what each row needs, the pages it gets, lens,
 // ok and the list of copies.
 __global__ __launch_bounds__(kTakeNt) void k_pages_take(PageArgs a) {
@@ -302,22 +325,125 @@ __global__ __launch_bounds__(kTakeNt) void k_pages_take(PageArgs a) {
   }
   if (tid == 0) *a.s.n_copies = copies;
   __syncthreads();
-  // the free page of rank k goes to the row that asks for the k-th page; a wave takes a word, a lane a page
-  for (int w = tid >> 6; w < words && s_before[w] < asked; w += kTakeNt / 64) {
-    const unsigned long long b = agent_load(&a.s.bits[w]);
-    const int k = s_before[w] + __popcll(b & ((1ull << lane) - 1ull));
-    if (!(b >> lane & 1ull) || k >= asked) continue;
-    // the last row that starts at or before it: rows that ask for nothing start where the next one does
-    int lo = 0, hi = R - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (s_start[mid] <= k) lo = mid;
-      else hi = mid - 1;
+  give_pages<kTakeNt>(a, words, asked, n_free, s_start, s_first, s_before, [&](int w) { return agent_load(&a.s.bits[w]); });
+}
+
+// A step of at most kTakeNt rows over a pool of at most kSmallPages pages in one launch: the tables' entries and the pool
+// in equal shares for all workgroups, the rest in the last one, a thread for each row and each word of free pages. ref
+// is taken over as it is, and the pages whose holders change are listed; the last workgroup makes them good.
+constexpr int kSmallPages = 64 * kTakeNt, kSmallEntries = 1 << 17;
+__global__ __launch_bounds__(kTakeNt) void k_pages_small(PageArgs a) {
+  __shared__ unsigned long long s_bits[kTakeNt];
+  __shared__ int s_before[kTakeNt], s_start[kTakeNt], s_first[kTakeNt];
+  __shared__ int s_last, s_copies;
+  const int tid = threadIdx.x, lane = tid & 63, P = a.to.n_pages, T = a.to.page_tokens, R = a.to.rows, words = (P + 63) / 64;
+  const bool alone = gridDim.x == 1;  // nothing to hand over
+  // the pages of this workgroup
+  for (int p0 = (blockIdx.x * kTakeNt + tid) & ~63; p0 < P; p0 += gridDim.x * kTakeNt) {
+    const int ref = p0 + lane < P ? a.from.ref[p0 + lane] : 1;
+    const unsigned long long is_free = __ballot(ref <= 0);
+    if (p0 + lane < P) agent_store(&a.to.ref[p0 + lane], ref);
+    if (lane == 0) {
+      if (alone) s_bits[p0 >> 6] = is_free;
+      else agent_store(&a.s.bits[p0 >> 6], is_free);
     }
-    if ((lo + 1 < R ? s_start[lo + 1] : asked) > n_free) continue;  // the row does not get all of its pages, and so none
-    a.to.table[lo * a.to.ldt + s_first[lo] + (k - s_start[lo])] = w * 64 + lane;
-    agent_store(&a.to.ref[w * 64 + lane], 1);
   }
+  // the table entries: those of `to`, and the rows beyond it that `from` has
+  const uint32_t cap = static_cast<uint32_t>(a.to.row_pages);
+  const uint32_t entries = static_cast<uint32_t>(max(a.from.rows, R)) * cap, step = gridDim.x * kTakeNt;
+  for (uint32_t e0 = (blockIdx.x * kTakeNt + tid) & ~63u; e0 < entries; e0 += step) {
+    const uint32_t e = min(e0 + lane, entries - 1);
+    const int i = static_cast<int>(divide(e, cap, a.m_cap)), j = static_cast<int>(e - static_cast<uint32_t>(i) * cap);
+    const bool mine = e0 + lane < entries;
+    RowPlan r{-1, 0, 0, true};
+    if (i < R) r = row_plan(a, i);
+    const int keep = pages_of(min(r.len, r.want), T), had = i < a.from.rows ? pages_of(held(a.from, i), T) : 0;
+    const int was = mine && j < had ? a.from.table[i * a.from.ldt + j] : -1;
+    const int now = mine && j < keep ? a.from.table[r.src * a.from.ldt + j] : -1;
+    if (mine && i < R) a.to.table[i * a.to.ldt + j] = now;
+    auto change = [&](int page, bool there, int by) {
+      const unsigned long long at = __ballot(there);
+      if (!at) return;
+      int first = 0;
+      if (lane == 0) first = agent_add(a.s.n_moves, static_cast<int>(__popcll(at)));
+      first = __shfl(first, 0);
+      if (there) {
+        agent_add(&a.s.delta[page], by);
+        agent_store(&a.s.moves[first + __popcll(at & ((1ull << lane) - 1ull))], page);
+      }
+    };
+    change(was, was != now && is_page(was, P), -1);
+    change(now, was != now && is_page(now, P), 1);
+    if (mine && j == r.len / T && r.want > r.len && r.len % T && is_page(now, P)) {
+      agent_add(&a.s.writers[now], 1);
+      __hip_atomic_fetch_max(&a.s.order[now], static_cast<unsigned long long>(r.len) << 32 | static_cast<uint32_t>(~i), __ATOMIC_RELAXED,
+                             __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  __syncthreads();
+  if (!alone) {
+    if (tid == 0) s_last = agent_add(a.s.tick, 1u) == gridDim.x - 1;
+    __syncthreads();
+    if (!s_last) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    if (tid == 0) agent_store(a.s.tick, 0u);
+  }
+
+  // this thread's row, and the begun page that it grows in
+  RowPlan r{-1, 0, 0, true};
+  int begun = -1;
+  if (tid < R) {
+    r = row_plan(a, tid);
+    if (r.want > r.len && r.len % T) begun = a.from.table[r.src * a.from.ldt + r.len / T];
+    if (!is_page(begun, P)) begun = -1;
+  }
+  int writers = 0;
+  unsigned long long order = 0;
+  if (begun >= 0) {
+    writers = agent_load(&a.s.writers[begun]);
+    order = agent_load(&a.s.order[begun]);
+  }
+  const int changes = agent_load(a.s.n_moves);
+  if (!alone && tid < words) s_bits[tid] = agent_load(&a.s.bits[tid]);
+  if (tid == 0) s_copies = 0;
+  __syncthreads();
+  if (tid == 0) agent_store(a.s.n_moves, 0);
+  for (int t = tid; t < changes; t += kTakeNt) {
+    const int p = agent_load(&a.s.moves[t]);
+    const int d = __hip_atomic_exchange(&a.s.delta[p], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (!d) continue;  // a page listed before, or one that as many give up as take
+    const int was = a.from.ref[p], ref = was + d;
+    agent_store(&a.to.ref[p], ref);
+    if ((was <= 0) != (ref <= 0)) atomicXor(&s_bits[p >> 6], 1ull << (p & 63));
+  }
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  __syncthreads();
+  const bool away = begun >= 0 && (agent_load(&a.to.ref[begun]) != writers ||
+                                   order != (static_cast<unsigned long long>(r.len) << 32 | static_cast<uint32_t>(~tid)));
+  const int first = pages_of(r.len, T) - away, need = r.want > r.len ? pages_of(r.want, T) - first : 0;
+  int asked, n_free;
+  const int start = scan_before(need, &asked);
+  const int before = scan_before(tid < words ? __popcll(s_bits[tid]) : 0, &n_free);
+  if (tid < words) s_before[tid] = before;
+  if (tid < R) {
+    s_start[tid] = start;
+    s_first[tid] = first;
+    const bool given = need == 0 || start + need <= n_free;
+    a.to.lens[tid] = given ? r.want : r.len;
+    if (a.ok) a.ok[tid] = r.fits && given;
+    if (begun >= 0) {
+      a.s.writers[begun] = 0;
+      a.s.order[begun] = 0;
+    }
+    if (given && away) {
+      agent_add(&a.to.ref[begun], -1);
+      a.s.copies[atomicAdd(&s_copies, 1)] = {begun, tid, r.len / T, r.len % T};
+    }
+  }
+  __syncthreads();
+  if (tid == 0) *a.s.n_copies = s_copies;
+  give_pages<kTakeNt>(a, words, asked, n_free, s_start, s_first, s_before, [&](int w) { return s_bits[w]; });
 }
 
 // Tokens of a page into another page of a plane: one chunk, four 16-byte columns a thread.
@@ -472,7 +598,7 @@ void launch_reorder(ReorderArgs a, int groups, int cus, hipStream_t st) {
   a.unit = a.p.token_bytes % bytes == 0 ? 0 : a.p.token_bytes % 4 == 0 ? 4 : a.p.token_bytes % 2 == 0 ? 2 : 1;
   const long long cols = (static_cast<long long>(a.p.tokens) * a.p.token_bytes + bytes - 1) / bytes * a.p.n_planes * a.p.pieces;
   const long long most = (cols + kNt - 1) / kNt;
-  const int blocks = static_cast<int>(std::max<long long>(1, std::min<long long>(most, (32ll * cus + groups - 1) / groups)));
+  const int blocks = static_cast<int>(std::max<long long>(1, std::min<long long>(most, (64ll * cus + groups - 1) / groups)));
   if (a.width <= 4) go_reorder<4, 16>(a, groups, blocks, st);
   else if (a.width <= 8) go_reorder<8, 16>(a, groups, blocks, st);
   else if (a.width <= 16) go_reorder<16, 16>(a, groups, blocks, st);
@@ -480,9 +606,17 @@ void launch_reorder(ReorderArgs a, int groups, int cus, hipStream_t st) {
   else go_reorder<64, 8>(a, groups, blocks, st);
 }
 
-void launch_pages_step(const PageArgs& a, int cus, hipStream_t st) {
-  hipLaunchKernelGGL(k_pages_fork, dim3(static_cast<unsigned>(std::max(a.from.rows, a.to.rows))), dim3(kNt), 0, st, a);
-  hipLaunchKernelGGL(k_pages_take, dim3(static_cast<unsigned>((a.to.n_pages + kTakePages - 1) / kTakePages)), dim3(kTakeNt), 0, st, a);
+void launch_pages_step(PageArgs a, int cus, hipStream_t st) {
+  const int rows = std::max(a.from.rows, a.to.rows);
+  const long long entries = static_cast<long long>(rows) * a.to.row_pages;
+  if (rows <= kTakeNt && a.to.n_pages <= kSmallPages && entries <= kSmallEntries) {
+    const long long work = std::max(entries, static_cast<long long>(a.to.n_pages));
+    a.m_cap = 0xFFFFFFFFu / static_cast<uint32_t>(a.to.row_pages);
+    hipLaunchKernelGGL(k_pages_small, dim3(static_cast<unsigned>(std::min<long long>((work + kTakeNt - 1) / kTakeNt, 64))), dim3(kTakeNt), 0, st, a);
+  } else {
+    hipLaunchKernelGGL(k_pages_fork, dim3(static_cast<unsigned>(rows)), dim3(kNt), 0, st, a);
+    hipLaunchKernelGGL(k_pages_take, dim3(static_cast<unsigned>((a.to.n_pages + kTakePages - 1) / kTakePages)), dim3(kTakeNt), 0, st, a);
+  }
   if (a.cache.n_planes && (a.add || a.add_all > 0))
     hipLaunchKernelGGL(k_page_copy, dim3(static_cast<unsigned>(8 * cus)), dim3(kNt), 0, st, a);
 }
@@ -490,7 +624,7 @@ void launch_pages_step(const PageArgs& a, int cus, hipStream_t st) {
 void launch_pages_compact(const PageArgs& a, int cus, hipStream_t st) {
   hipLaunchKernelGGL(k_pages_scan, dim3(static_cast<unsigned>((a.to.n_pages + kTakePages - 1) / kTakePages)), dim3(kTakeNt), 0, st, a);
   hipLaunchKernelGGL(k_pages_pair, dim3(static_cast<unsigned>((a.to.n_pages + kNt - 1) / kNt)), dim3(kNt), 0, st, a);
-  hipLaunchKernelGGL(k_pages_move, dim3(static_cast<unsigned>(8 * cus)), dim3(kNt), 0, st, a);
+  hipLaunchKernelGGL(k_pages_move, dim3(static_cast<unsigned>(16 * cus)), dim3(kNt), 0, st, a);
 }
 
 }  // namespace vsmp
