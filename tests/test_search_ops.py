@@ -615,6 +615,31 @@ def test_pages_far_and_large(ctx):
     np.testing.assert_array_equal(x[moved[src]], src[:, None] * T + np.arange(T))
 
 
+@pytest.mark.parametrize("rows,row_pages", [(8192, 1 << 20), (3000, 40)])
+def test_pages_rows_that_ask_for_more_than_there_is(ctx, rows, row_pages):
+    """Rows that want up to 2^30 tokens each, together more than 32 bits count: the first ones that fit get their pages,
+    none of the others any."""
+    import torch
+
+    P = 1000
+    table = torch.full((1, row_pages), -1, dtype=torch.int32, device="cuda")
+    pages = V.Pages(table.expand(1, row_pages), i32([0]), i32(np.zeros(P)), 1 if row_pages > 40 else 1 << 24)
+    T = pages.page_tokens
+    out = torch.full((1, row_pages), 7, dtype=torch.int32, device="cuda").expand(1, row_pages)
+    # a table of 8,192 rows of 2^20 entries would take 32 GB: the rows beyond the first few ask through add alone
+    n = 64 if row_pages > 40 else rows
+    to = V.Pages(torch.empty(n, row_pages, dtype=torch.int32, device="cuda"), i32(np.zeros(n)), i32(np.zeros(P)), T)
+    want = np.full(n, row_pages * T if row_pages > 40 else 40 * T)
+    want[:2] = 5 * T, 7 * T
+    log("more than there is", rows, row_pages)
+    got, ok = ctx.pages_step(pages, i32(np.full(n, -1)), i32(want), out=to)
+    need = -(-want // T)
+    fits = np.cumsum(need) <= P
+    assert ok.cpu().numpy().tolist() == fits.astype(int).tolist()
+    assert got.lens.cpu().numpy().tolist() == np.where(fits, want, 0).tolist()
+    assert int(got.ref.sum()) == int(need[fits].sum())
+
+
 def test_pages_tables_with_numbers_that_are_no_pages(ctx):
     """Entries outside the pool stand for no page: nothing is read or counted through them, and rows go on with them."""
     P, T = 10, 4

@@ -105,7 +105,8 @@ struct PageArgs {
   int* moved;
   int* live;
   PlaneArgs cache;              // n_planes 0: none
-  uint32_t m_cap;               // (2^32 - 1) / to.row_pages (launch_pages_step)
+  uint32_t m_cap;               // (2^32 - 1) / to.row_pages, and workgroups for the tables (launch_pages_step)
+  int table_wgs;
   PageScratch s;
 };
 

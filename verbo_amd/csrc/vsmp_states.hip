@@ -183,27 +183,41 @@ __global__ __launch_bounds__(kNt) void k_pages_fork(PageArgs a) {
 constexpr int kTakeNt = 1024;
 constexpr int kTakePages = 4 * kTakeNt;  // pages of a workgroup
 
-// Sum over the workgroup's threads before this one; *total: over all.
+// Sums over the lanes up to this one (row shifts by 1, 2, 4 and 8, then the rows' sums handed on).
+__device__ __forceinline__ int scan64(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+  return v;
+}
+// Of K numbers a thread: their sums over the workgroup's threads before this one; total: over all.
+template <int K>
+__device__ __forceinline__ void scan_before(int (&v)[K], int (&total)[K]) {
+  __shared__ int s_sum[K][kTakeNt / 64];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int at[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) at[k] = scan64(v[k]);
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+    if (lane == 63) s_sum[k][wv] = at[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int sums = scan64(lane < kTakeNt / 64 ? s_sum[k][lane] : 0);
+    total[k] = __builtin_amdgcn_readlane(sums, kTakeNt / 64 - 1);
+    v[k] = at[k] - v[k] + (wv ? __builtin_amdgcn_readlane(sums, wv - 1) : 0);
+  }
+}
 __device__ __forceinline__ int scan_before(int v, int* total) {
-  __shared__ int s_sum[kTakeNt / 64];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  int at = v;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(at, d);
-    if (lane >= d) at += o;
-  }
-  __syncthreads();
-  if (lane == 63) s_sum[wv] = at;
-  __syncthreads();
-  int before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < kTakeNt / 64; ++w) {
-    before += w < wv ? s_sum[w] : 0;
-    all += s_sum[w];
-  }
-  *total = all;
-  return before + at - v;
+  int a[1] = {v}, t[1];
+  scan_before<1>(a, t);
+  *total = t[0];
+  return a[0];
 }
 
 // The free page of rank k goes to the row that asks for the k-th page: a wave takes a word, a lane a page. start: pages
@@ -224,7 +238,7 @@ __device__ __forceinline__ void give_pages(const PageArgs& a, int words, int ask
       else hi = mid - 1;
     }
     if ((lo + 1 < R ? start[lo + 1] : asked) > n_free) continue;  // the row does not get all of its pages, and so none
-    a.to.table[lo * a.to.ldt + first[lo] + (k - start[lo])] = w * 64 + lane;
+    agent_store(&a.to.table[lo * a.to.ldt + first[lo] + (k - start[lo])], w * 64 + lane);
     agent_store(&a.to.ref[w * 64 + lane], 1);
   }
 }
@@ -259,7 +273,9 @@ __global__ __launch_bounds__(kTakeNt) void k_pages_take(PageArgs a) {
   if (tid == 0) agent_store(a.s.tick, 0u);
 
   // the rows' needs
-  int asked = 0, copies = 0;  // so far
+  long long wanted = 0;  // so far: rows may ask for more than any pool has, together for more than 32 bits hold
+  int copies = 0;
+  constexpr long long kNever = 1 << 30;
   int need_[kPageRows / kTakeNt];
   bool away_[kPageRows / kTakeNt];
 #pragma unroll
@@ -279,11 +295,14 @@ __global__ __launch_bounds__(kTakeNt) void k_pages_take(PageArgs a) {
         need_[k] = pages_of(r.want, T) - s_first[i];
       }
     }
+    // (a need of more than a pool is as good as any that no pool meets: 1,024 of them fit 31 bits)
     int total;
+    need_[k] = min(need_[k], kPagesMax + 1);
     const int at = scan_before(need_[k], &total);
-    if (i < R) s_start[i] = asked + at;
-    asked += total;
+    if (i < R) s_start[i] = static_cast<int>(min(wanted + at, kNever));
+    wanted += total;
   }
+  const int asked = static_cast<int>(min(wanted, kNever));
   // how many pages are free, and before each thread's words
   const int words = (P + 63) / 64, mine = (words + kTakeNt - 1) / kTakeNt;
   int count = 0;
@@ -302,7 +321,7 @@ __global__ __launch_bounds__(kTakeNt) void k_pages_take(PageArgs a) {
     RowPlan r{};
     if (i < R) {
       r = row_plan(a, i);
-      const bool given = need_[k] == 0 || s_start[i] + need_[k] <= n_free;
+      const bool given = need_[k] == 0 || (s_start[i] <= n_free && need_[k] <= n_free - s_start[i]);
       a.to.lens[i] = given ? r.want : r.len;
       if (a.ok) a.ok[i] = r.fits && given;
       copied = given && away_[k];
@@ -328,39 +347,59 @@ __global__ __launch_bounds__(kTakeNt) void k_pages_take(PageArgs a) {
   give_pages<kTakeNt>(a, words, asked, n_free, s_start, s_first, s_before, [&](int w) { return agent_load(&a.s.bits[w]); });
 }
 
-// A step of at most kTakeNt rows over a pool of at most kSmallPages pages in one launch: the tables' entries and the pool
-// in equal shares for all workgroups, the rest in the last one, a thread for each row and each word of free pages. ref
-// is taken over as it is, and the pages whose holders change are listed; the last workgroup makes them good.
-constexpr int kSmallPages = 64 * kTakeNt, kSmallEntries = 1 << 17;
+// A step of at most kTakeNt rows over a pool of at most kSmallPages pages: workgroups that take over ref and gather the free
+// pages as bits, and a last one that does the rest, a thread for each row and each word of bits. With WHOLE the tables are
+// among the workgroups' work (the first a.table_wgs of them), in one launch: ref is taken over as it is, the pages whose holders
+// change are listed, and the last workgroup makes them good. Without it k_pages_fork has been there, and delta is whole.
+// What one workgroup writes after another has is written through to memory by both: they may not share an L2.
+constexpr int kSmallPages = 64 * kTakeNt, kSmallEntries = 1 << 13;
+template <bool WHOLE>
 __global__ __launch_bounds__(kTakeNt) void k_pages_small(PageArgs a) {
   __shared__ unsigned long long s_bits[kTakeNt];
   __shared__ int s_before[kTakeNt], s_start[kTakeNt], s_first[kTakeNt];
   __shared__ int s_last, s_copies;
   const int tid = threadIdx.x, lane = tid & 63, P = a.to.n_pages, T = a.to.page_tokens, R = a.to.rows, words = (P + 63) / 64;
   const bool alone = gridDim.x == 1;  // nothing to hand over
-  // the pages of this workgroup
-  for (int p0 = (blockIdx.x * kTakeNt + tid) & ~63; p0 < P; p0 += gridDim.x * kTakeNt) {
-    const int ref = p0 + lane < P ? a.from.ref[p0 + lane] : 1;
+  // this thread's row in the last workgroup, and the begun page that it grows in: loaded beside the rest
+  RowPlan r{-1, 0, 0, true};
+  int begun = -1;
+  if (tid < R) {
+    r = row_plan(a, tid);
+    if (r.want > r.len && r.len % T) begun = a.from.table[r.src * a.from.ldt + r.len / T];
+    if (!is_page(begun, P)) begun = -1;
+  }
+  // the pages of this workgroup: all of them if it is alone
+  const int wg = static_cast<int>(blockIdx.x) - a.table_wgs;
+  for (int p0 = alone ? tid & ~63 : wg >= 0 ? (wg * kTakeNt + tid) & ~63 : P; p0 < P; p0 += alone ? kTakeNt : (gridDim.x - a.table_wgs) * kTakeNt) {
+    int ref = 1;
+    if (p0 + lane < P) {
+      ref = a.from.ref[p0 + lane];
+      if (!WHOLE) {
+        const int d = a.s.delta[p0 + lane];
+        ref += d;
+        if (d) a.s.delta[p0 + lane] = 0;
+      }
+      agent_store(&a.to.ref[p0 + lane], ref);
+    }
     const unsigned long long is_free = __ballot(ref <= 0);
-    if (p0 + lane < P) agent_store(&a.to.ref[p0 + lane], ref);
     if (lane == 0) {
       if (alone) s_bits[p0 >> 6] = is_free;
       else agent_store(&a.s.bits[p0 >> 6], is_free);
     }
   }
-  // the table entries: those of `to`, and the rows beyond it that `from` has
+  // its table entries: those of `to`, and the rows beyond it that `from` has
   const uint32_t cap = static_cast<uint32_t>(a.to.row_pages);
-  const uint32_t entries = static_cast<uint32_t>(max(a.from.rows, R)) * cap, step = gridDim.x * kTakeNt;
-  for (uint32_t e0 = (blockIdx.x * kTakeNt + tid) & ~63u; e0 < entries; e0 += step) {
+  const uint32_t entries = WHOLE ? static_cast<uint32_t>(max(a.from.rows, R)) * cap : 0u, step = (alone ? 1 : a.table_wgs) * kTakeNt;
+  for (uint32_t e0 = wg < 0 || alone ? (blockIdx.x * kTakeNt + tid) & ~63u : entries; e0 < entries; e0 += step) {
     const uint32_t e = min(e0 + lane, entries - 1);
     const int i = static_cast<int>(divide(e, cap, a.m_cap)), j = static_cast<int>(e - static_cast<uint32_t>(i) * cap);
     const bool mine = e0 + lane < entries;
-    RowPlan r{-1, 0, 0, true};
-    if (i < R) r = row_plan(a, i);
-    const int keep = pages_of(min(r.len, r.want), T), had = i < a.from.rows ? pages_of(held(a.from, i), T) : 0;
+    RowPlan o{-1, 0, 0, true};
+    if (i < R) o = row_plan(a, i);
+    const int keep = pages_of(min(o.len, o.want), T), had = i < a.from.rows ? pages_of(held(a.from, i), T) : 0;
     const int was = mine && j < had ? a.from.table[i * a.from.ldt + j] : -1;
-    const int now = mine && j < keep ? a.from.table[r.src * a.from.ldt + j] : -1;
-    if (mine && i < R) a.to.table[i * a.to.ldt + j] = now;
+    const int now = mine && j < keep ? a.from.table[o.src * a.from.ldt + j] : -1;
+    if (mine && i < R) agent_store(&a.to.table[i * a.to.ldt + j], now);
     auto change = [&](int page, bool there, int by) {
       const unsigned long long at = __ballot(there);
       if (!at) return;
@@ -374,9 +413,9 @@ __global__ __launch_bounds__(kTakeNt) void k_pages_small(PageArgs a) {
     };
     change(was, was != now && is_page(was, P), -1);
     change(now, was != now && is_page(now, P), 1);
-    if (mine && j == r.len / T && r.want > r.len && r.len % T && is_page(now, P)) {
+    if (mine && j == o.len / T && o.want > o.len && o.len % T && is_page(now, P)) {
       agent_add(&a.s.writers[now], 1);
-      __hip_atomic_fetch_max(&a.s.order[now], static_cast<unsigned long long>(r.len) << 32 | static_cast<uint32_t>(~i), __ATOMIC_RELAXED,
+      __hip_atomic_fetch_max(&a.s.order[now], static_cast<unsigned long long>(o.len) << 32 | static_cast<uint32_t>(~i), __ATOMIC_RELAXED,
                              __HIP_MEMORY_SCOPE_AGENT);
     }
   }
@@ -390,41 +429,45 @@ __global__ __launch_bounds__(kTakeNt) void k_pages_small(PageArgs a) {
     if (tid == 0) agent_store(a.s.tick, 0u);
   }
 
-  // this thread's row, and the begun page that it grows in
-  RowPlan r{-1, 0, 0, true};
-  int begun = -1;
-  if (tid < R) {
-    r = row_plan(a, tid);
-    if (r.want > r.len && r.len % T) begun = a.from.table[r.src * a.from.ldt + r.len / T];
-    if (!is_page(begun, P)) begun = -1;
-  }
   int writers = 0;
   unsigned long long order = 0;
   if (begun >= 0) {
     writers = agent_load(&a.s.writers[begun]);
     order = agent_load(&a.s.order[begun]);
   }
-  const int changes = agent_load(a.s.n_moves);
+  const int changes = WHOLE ? agent_load(a.s.n_moves) : 0;
   if (!alone && tid < words) s_bits[tid] = agent_load(&a.s.bits[tid]);
   if (tid == 0) s_copies = 0;
   __syncthreads();
-  if (tid == 0) agent_store(a.s.n_moves, 0);
-  for (int t = tid; t < changes; t += kTakeNt) {
-    const int p = agent_load(&a.s.moves[t]);
-    const int d = __hip_atomic_exchange(&a.s.delta[p], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (!d) continue;  // a page listed before, or one that as many give up as take
-    const int was = a.from.ref[p], ref = was + d;
-    agent_store(&a.to.ref[p], ref);
-    if ((was <= 0) != (ref <= 0)) atomicXor(&s_bits[p >> 6], 1ull << (p & 63));
+  if (WHOLE && tid == 0) agent_store(a.s.n_moves, 0);
+  for (int t0 = 0; t0 < changes; t0 += 4 * kTakeNt) {
+    int p[4], d[4], was[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) p[k] = t0 + k * kTakeNt + tid < changes ? agent_load(&a.s.moves[t0 + k * kTakeNt + tid]) : -1;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      d[k] = p[k] >= 0 ? agent_load(&a.s.delta[p[k]]) : 0;
+      was[k] = a.from.ref[max(p[k], 0)];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (!d[k]) continue;  // a page listed before, or one that as many give up as take
+      // (where a page is listed again, another thread may do the same beside this one)
+      const int ref = was[k] + d[k];
+      agent_store(&a.s.delta[p[k]], 0);
+      agent_store(&a.to.ref[p[k]], ref);
+      if (was[k] > 0 && ref <= 0) atomicOr(&s_bits[p[k] >> 6], 1ull << (p[k] & 63));
+      if (was[k] <= 0 && ref > 0) atomicAnd(&s_bits[p[k] >> 6], ~(1ull << (p[k] & 63)));
+    }
   }
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   __syncthreads();
   const bool away = begun >= 0 && (agent_load(&a.to.ref[begun]) != writers ||
                                    order != (static_cast<unsigned long long>(r.len) << 32 | static_cast<uint32_t>(~tid)));
   const int first = pages_of(r.len, T) - away, need = r.want > r.len ? pages_of(r.want, T) - first : 0;
-  int asked, n_free;
-  const int start = scan_before(need, &asked);
-  const int before = scan_before(tid < words ? __popcll(s_bits[tid]) : 0, &n_free);
+  int sum[2] = {need, tid < words ? static_cast<int>(__popcll(s_bits[tid])) : 0}, all[2];
+  scan_before<2>(sum, all);
+  const int asked = all[0], n_free = all[1], start = sum[0], before = sum[1];
   if (tid < words) s_before[tid] = before;
   if (tid < R) {
     s_start[tid] = start;
@@ -609,13 +652,19 @@ void launch_reorder(ReorderArgs a, int groups, int cus, hipStream_t st) {
 void launch_pages_step(PageArgs a, int cus, hipStream_t st) {
   const int rows = std::max(a.from.rows, a.to.rows);
   const long long entries = static_cast<long long>(rows) * a.to.row_pages;
-  if (rows <= kTakeNt && a.to.n_pages <= kSmallPages && entries <= kSmallEntries) {
-    const long long work = std::max(entries, static_cast<long long>(a.to.n_pages));
+  const bool small = rows <= kTakeNt && a.to.n_pages <= kSmallPages;
+  const int wgs = (a.to.n_pages + kTakeNt - 1) / kTakeNt;  // 64 at most of a small pool
+  if (small && entries <= kSmallEntries) {
     a.m_cap = 0xFFFFFFFFu / static_cast<uint32_t>(a.to.row_pages);
-    hipLaunchKernelGGL(k_pages_small, dim3(static_cast<unsigned>(std::min<long long>((work + kTakeNt - 1) / kTakeNt, 64))), dim3(kTakeNt), 0, st, a);
+    a.table_wgs = static_cast<int>((entries + kTakeNt - 1) / kTakeNt);
+    const bool alone = a.table_wgs == 1 && wgs == 1;
+    hipLaunchKernelGGL(k_pages_small<true>, dim3(static_cast<unsigned>(alone ? 1 : a.table_wgs + wgs)), dim3(kTakeNt), 0, st, a);
   } else {
     hipLaunchKernelGGL(k_pages_fork, dim3(static_cast<unsigned>(rows)), dim3(kNt), 0, st, a);
-    hipLaunchKernelGGL(k_pages_take, dim3(static_cast<unsigned>((a.to.n_pages + kTakePages - 1) / kTakePages)), dim3(kTakeNt), 0, st, a);
+    if (small)
+      hipLaunchKernelGGL(k_pages_small<false>, dim3(static_cast<unsigned>(wgs)), dim3(kTakeNt), 0, st, a);
+    else
+      hipLaunchKernelGGL(k_pages_take, dim3(static_cast<unsigned>((a.to.n_pages + kTakePages - 1) / kTakePages)), dim3(kTakeNt), 0, st, a);
   }
   if (a.cache.n_planes && (a.add || a.add_all > 0))
     hipLaunchKernelGGL(k_page_copy, dim3(static_cast<unsigned>(8 * cus)), dim3(kNt), 0, st, a);
