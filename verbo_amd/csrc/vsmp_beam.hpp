@@ -107,6 +107,7 @@ struct PageArgs {
   PlaneArgs cache;              // n_planes 0: none
   uint32_t m_cap;               // (2^32 - 1) / to.row_pages, and workgroups for the tables (launch_pages_step)
   int table_wgs;
+  uint32_t m_chunks, m_planes;  // (2^32 - 1) / a page's chunks, and cache.n_planes (copy_planes)
   PageScratch s;
 };
 

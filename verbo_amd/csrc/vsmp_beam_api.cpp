@@ -78,8 +78,6 @@ int check_step(const vsmp_pages* from, const vsmp_pages* to, const vsmp_planes* 
     if (check_planes(*cache) != 0) return -1;
     if (cache->rows != to->n_pages || cache->tokens != to->page_tokens)
       return set_error("vsmp: the cache's planes must have n_pages rows of page_tokens tokens");
-    const long long chunks = ((static_cast<long long>(cache->tokens) * cache->token_bytes + 15) / 16 * cache->pieces + 1023) / 1024;
-    if (chunks * cache->n_planes > INT32_MAX) return set_error("vsmp: a page's tokens must hold fewer than 2^45 bytes over all planes");
   }
   return 0;
 }

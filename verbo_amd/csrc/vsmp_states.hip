@@ -489,78 +489,125 @@ __global__ __launch_bounds__(kTakeNt) void k_pages_small(PageArgs a) {
   give_pages<kTakeNt>(a, words, asked, n_free, s_start, s_first, s_before, [&](int w) { return s_bits[w]; });
 }
 
-// Tokens of a page into another page of a plane: one chunk, four 16-byte columns a thread.
-__device__ __forceinline__ void copy_tokens(const PlaneArgs& c, int plane, int src, int dst, int tokens, uint32_t chunk) {
+// Tokens of a page into another page of a plane: a wave's chunk, four 16-byte columns a lane. The columns of all pieces
+// follow one another.
+constexpr int kChunk = 64 * 4;
+__device__ __forceinline__ uint32_t chunks_of(const PlaneArgs& c, int tokens) {
+  const uint32_t cols = (static_cast<uint32_t>(tokens) * static_cast<uint32_t>(c.token_bytes) + 15) / 16;
+  return (cols * static_cast<uint32_t>(c.pieces) + kChunk - 1) / kChunk;
+}
+__device__ __forceinline__ void copy_tokens(const PlaneArgs& c, uint32_t plane, int src, int dst, int tokens, uint32_t chunk) {
   typedef Column<16> vec;
   const uint32_t run = static_cast<uint32_t>(tokens) * static_cast<uint32_t>(c.token_bytes);
-  const uint32_t cols = (run + 15) / 16, m = 0xFFFFFFFFu / cols;
-  const uint32_t total = cols * static_cast<uint32_t>(c.pieces);
-  Bytes* base = plane_at(c, static_cast<uint32_t>(plane));
-  const Bytes* from = base + src * c.row_stride;
-  Bytes* to = base + dst * c.row_stride;
+  const uint32_t cols = (run + 15) / 16, m = 0xFFFFFFFFu / cols, total = cols * static_cast<uint32_t>(c.pieces);
+  const long long there = dst * c.row_stride - src * c.row_stride;
+  const Bytes* base = plane_at(c, plane) + src * c.row_stride;
   vec v[4];
-  long long off[4];
+  const Bytes* from[4];
   int n[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const uint32_t idx = chunk * (kNt * 4) + k * kNt + threadIdx.x;
+    const uint32_t idx = chunk * kChunk + k * 64 + (threadIdx.x & 63);
     n[k] = 0;
     if (idx < total) {
-      const uint32_t piece = divide(idx, cols, m), at = (idx - piece * cols) * 16;
-      off[k] = piece * c.piece_stride + at;
-      n[k] = static_cast<int>(min(run - at, 16u));
-      if (n[k] == 16) v[k] = get<vec>(from + off[k]);
+      const uint32_t piece = c.pieces == 1 ? 0u : divide(idx, cols, m), byte = (idx - piece * cols) * 16;
+      from[k] = base + piece * c.piece_stride + byte;
+      n[k] = static_cast<int>(min(run - byte, 16u));
+      if (n[k] == 16) v[k] = get<vec>(from[k]);
     }
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k)
-    if (n[k] == 16) set<vec>(to + off[k], v[k]);
+    if (n[k] == 16) set<vec>((Bytes*)from[k] + there, v[k]);
   // the runs' ends
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     if (n[k] == 0 || n[k] == 16) continue;
+    Bytes* to = (Bytes*)from[k] + there;
     int b = 0;
-    for (; b + 4 <= n[k]; b += 4) set<Loose<uint32_t>>(to + off[k] + b, get<Loose<uint32_t>>(from + off[k] + b));
-    for (; b < n[k]; ++b) set(to + off[k] + b, get<uint8_t>(from + off[k] + b));
+    for (; b + 4 <= n[k]; b += 4) set<Loose<uint32_t>>(to + b, get<Loose<uint32_t>>(from[k] + b));
+    for (; b < n[k]; ++b) set(to + b, get<uint8_t>(from[k] + b));
   }
 }
-__device__ __forceinline__ uint32_t chunks_of(const PlaneArgs& c, int tokens) {
-  const uint32_t cols = (static_cast<uint32_t>(tokens) * static_cast<uint32_t>(c.token_bytes) + 15) / 16;
-  return (cols * static_cast<uint32_t>(c.pieces) + kNt * 4 - 1) / (kNt * 4);
+
+// What wave `unit` of a copy does: unit = (page * planes + plane) * chunks + chunk.
+struct CopyUnit {
+  uint32_t page, plane, chunk;
+};
+__device__ __forceinline__ CopyUnit copy_unit(const PageArgs& a, uint32_t unit, uint32_t chunks) {
+  const uint32_t at = divide(unit, chunks, a.m_chunks), planes = static_cast<uint32_t>(a.cache.n_planes), page = divide(at, planes, a.m_planes);
+  return {page, at - page * planes, unit - at * chunks};
 }
+__device__ __forceinline__ uint32_t wave_of_grid() { return __builtin_amdgcn_readfirstlane(blockIdx.x * (kNt / 64) + (threadIdx.x >> 6)); }
 
 __global__ __launch_bounds__(kNt) void k_page_copy(PageArgs a) {
-  const uint32_t chunks = chunks_of(a.cache, a.cache.tokens), per = chunks * static_cast<uint32_t>(a.cache.n_planes);
-  const unsigned long long total = static_cast<unsigned long long>(*a.s.n_copies) * per;
-  for (unsigned long long u = blockIdx.x; u < total; u += gridDim.x) {
-    const PageCopy c = a.s.copies[u / per];
-    const uint32_t rest = static_cast<uint32_t>(u % per), plane = rest / chunks, chunk = rest % chunks;
-    if (chunk >= chunks_of(a.cache, c.tokens)) continue;
-    const long long row = c.row;
-    copy_tokens(a.cache, static_cast<int>(plane), c.src, a.to.table[row * a.to.ldt + c.at], c.tokens, chunk);
+  const uint32_t chunks = chunks_of(a.cache, a.cache.tokens);
+  const uint32_t total = static_cast<uint32_t>(*a.s.n_copies) * static_cast<uint32_t>(a.cache.n_planes) * chunks;
+  for (uint32_t u = wave_of_grid(); u < total; u += gridDim.x * (kNt / 64)) {
+    const CopyUnit w = copy_unit(a, u, chunks);
+    const PageCopy c = a.s.copies[w.page];
+    if (w.chunk < chunks_of(a.cache, c.tokens)) copy_tokens(a.cache, w.plane, c.src, a.to.table[c.row * a.to.ldt + c.at], c.tokens, w.chunk);
   }
 }
 
 // ---- compaction ------------------------------------------------------------------------------------------
 
-// The pages in use as bits; in the last workgroup, how many are in use before each word.
+// The pages in use as bits; in the last workgroup, how many are in use before each word; of a small pool also the lists of
+// k_pages_pair.
 __global__ __launch_bounds__(kTakeNt) void k_pages_scan(PageArgs a) {
+  __shared__ unsigned long long s_bits[kTakeNt];
+  __shared__ int s_before[kTakeNt + 1];
   __shared__ int s_last;
   const int tid = threadIdx.x, lane = tid & 63, P = a.to.n_pages;
+  const bool alone = gridDim.x == 1, small = P <= kSmallPages;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int p = blockIdx.x * kTakePages + k * kTakeNt + tid;
     const unsigned long long used = __ballot(p < P && a.from.ref[min(p, P - 1)] > 0);
-    if (lane == 0 && p < P) agent_store(&a.s.bits[p >> 6], used);
+    if (lane == 0 && p < P) {
+      agent_store(&a.s.bits[p >> 6], used);
+      if (alone) s_bits[p >> 6] = used;
+    }
   }
-  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-  __syncthreads();
-  if (tid == 0) s_last = agent_add(a.s.tick, 1u) == gridDim.x - 1;
-  __syncthreads();
-  if (!s_last) return;
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-  if (tid == 0) agent_store(a.s.tick, 0u);
-  const int words = (P + 63) / 64, mine = (words + kTakeNt - 1) / kTakeNt;
+  if (!alone) {
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    __syncthreads();
+    if (tid == 0) s_last = agent_add(a.s.tick, 1u) == gridDim.x - 1;
+    __syncthreads();
+    if (!s_last) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    if (tid == 0) agent_store(a.s.tick, 0u);
+  } else {
+    __syncthreads();
+  }
+  const int words = (P + 63) / 64;
+  if (small) {
+    unsigned long long b = 0;
+    if (tid < words) b = alone ? s_bits[tid] : agent_load(&a.s.bits[tid]);
+    int n;
+    const int at = scan_before(__popcll(b), &n);
+    if (tid < words) {
+      s_bits[tid] = b;
+      s_before[tid] = at;
+      a.s.before[tid] = at;
+    }
+    if (tid == 0) {
+      a.s.before[words] = n;
+      if (a.live) *a.live = n;
+    }
+    __syncthreads();
+    // a wave takes a word, a lane a page
+    const int kept = n < P ? s_before[n >> 6] + __popcll(s_bits[n >> 6] & ((1ull << (n & 63)) - 1ull)) : n;
+    for (int w = tid >> 6; w < words; w += kTakeNt / 64) {
+      const unsigned long long bits = s_bits[w];
+      const int p = w * 64 + lane, below = s_before[w] + __popcll(bits & ((1ull << lane) - 1ull));
+      const bool used = bits >> lane & 1ull;
+      if (p < n && !used) a.s.room[p - below] = p;
+      if (p >= n && used) a.s.moves[below - kept] = p;
+    }
+    return;
+  }
+  const int mine = (words + kTakeNt - 1) / kTakeNt;
   int count = 0;
   for (int w = tid * mine; w < min(words, (tid + 1) * mine); ++w) count += __popcll(agent_load(&a.s.bits[w]));
   int total;
@@ -599,7 +646,6 @@ __global__ __launch_bounds__(kNt) void k_pages_move(PageArgs a) {
   const int P = a.to.n_pages, T = a.to.page_tokens, n = a.s.before[(P + 63) / 64];
   const int kept = n < P ? used_before(a, n) : n;  // pages in use below n
   const int moves = n - kept;
-  const uint32_t chunks = chunks_of(a.cache, a.cache.tokens), per = chunks * static_cast<uint32_t>(a.cache.n_planes);
   // small work first: tables by rows, then the pool
   for (int i = blockIdx.x; i < a.to.rows; i += gridDim.x) {
     const int len = held(a.from, i), used = pages_of(len, T);
@@ -621,11 +667,11 @@ __global__ __launch_bounds__(kNt) void k_pages_move(PageArgs a) {
     if (p >= n) a.to.ref[p] = 0;
   }
   if (!a.cache.n_planes) return;
-  const unsigned long long total = static_cast<unsigned long long>(moves) * per;
-  for (unsigned long long u = blockIdx.x; u < total; u += gridDim.x) {
-    const int k = static_cast<int>(u / per);
-    const uint32_t rest = static_cast<uint32_t>(u % per);
-    copy_tokens(a.cache, static_cast<int>(rest / chunks), a.s.moves[k], a.s.room[k], a.cache.tokens, rest % chunks);
+  const uint32_t chunks = chunks_of(a.cache, a.cache.tokens);
+  const uint32_t total = static_cast<uint32_t>(moves) * static_cast<uint32_t>(a.cache.n_planes) * chunks;
+  for (uint32_t u = wave_of_grid(); u < total; u += gridDim.x * (kNt / 64)) {
+    const CopyUnit w = copy_unit(a, u, chunks);
+    copy_tokens(a.cache, w.plane, a.s.moves[w.page], a.s.room[w.page], a.cache.tokens, w.chunk);
   }
 }
 
@@ -649,6 +695,23 @@ void launch_reorder(ReorderArgs a, int groups, int cus, hipStream_t st) {
   else go_reorder<64, 8>(a, groups, blocks, st);
 }
 
+// Copies of up to n pages, by `launch` with at most `most` workgroups, in as many planes at a time as 31 bits count the
+// waves' chunks of (all of them, but for pools that hardly fit a card).
+template <class F>
+static void copy_planes(PageArgs a, int n, int most, F launch) {
+  const PlaneArgs c = a.cache;
+  const long long cols = (static_cast<long long>(c.tokens) * c.token_bytes + 15) / 16 * c.pieces, chunks = (cols + kChunk - 1) / kChunk;
+  const int planes = static_cast<int>(std::max<long long>(1, std::min<long long>(c.n_planes, INT32_MAX / (chunks * n))));
+  a.m_chunks = 0xFFFFFFFFu / static_cast<uint32_t>(chunks);
+  for (int p = 0; p < c.n_planes; p += a.cache.n_planes) {
+    a.cache.planes = c.planes + p;
+    a.cache.n_planes = std::min(planes, c.n_planes - p);
+    a.m_planes = 0xFFFFFFFFu / static_cast<uint32_t>(a.cache.n_planes);
+    const long long waves = chunks * n * a.cache.n_planes;
+    launch(a, static_cast<unsigned>(std::min<long long>(most, (waves + kNt / 64 - 1) / (kNt / 64))));
+  }
+}
+
 void launch_pages_step(PageArgs a, int cus, hipStream_t st) {
   const int rows = std::max(a.from.rows, a.to.rows);
   const long long entries = static_cast<long long>(rows) * a.to.row_pages;
@@ -667,13 +730,19 @@ void launch_pages_step(PageArgs a, int cus, hipStream_t st) {
       hipLaunchKernelGGL(k_pages_take, dim3(static_cast<unsigned>((a.to.n_pages + kTakePages - 1) / kTakePages)), dim3(kTakeNt), 0, st, a);
   }
   if (a.cache.n_planes && (a.add || a.add_all > 0))
-    hipLaunchKernelGGL(k_page_copy, dim3(static_cast<unsigned>(8 * cus)), dim3(kNt), 0, st, a);
+    copy_planes(a, a.to.rows, 16 * cus, [&](const PageArgs& c, unsigned wgs) { hipLaunchKernelGGL(k_page_copy, dim3(wgs), dim3(kNt), 0, st, c); });
 }
 
 void launch_pages_compact(const PageArgs& a, int cus, hipStream_t st) {
-  hipLaunchKernelGGL(k_pages_scan, dim3(static_cast<unsigned>((a.to.n_pages + kTakePages - 1) / kTakePages)), dim3(kTakeNt), 0, st, a);
-  hipLaunchKernelGGL(k_pages_pair, dim3(static_cast<unsigned>((a.to.n_pages + kNt - 1) / kNt)), dim3(kNt), 0, st, a);
-  hipLaunchKernelGGL(k_pages_move, dim3(static_cast<unsigned>(16 * cus)), dim3(kNt), 0, st, a);
+  const int P = a.to.n_pages;
+  hipLaunchKernelGGL(k_pages_scan, dim3(static_cast<unsigned>((P + kTakePages - 1) / kTakePages)), dim3(kTakeNt), 0, st, a);
+  if (P > kSmallPages) hipLaunchKernelGGL(k_pages_pair, dim3(static_cast<unsigned>((P + kNt - 1) / kNt)), dim3(kNt), 0, st, a);
+  // (tables and pool with each launch: there is hardly ever more than one)
+  const unsigned rest = std::min(static_cast<unsigned>(std::max(a.to.rows, (P + kNt - 1) / kNt)), 4u * cus);
+  if (a.cache.n_planes)
+    copy_planes(a, P / 2 + 1, 16 * cus, [&](const PageArgs& c, unsigned wgs) { hipLaunchKernelGGL(k_pages_move, dim3(std::max(rest, wgs)), dim3(kNt), 0, st, c); });
+  else
+    hipLaunchKernelGGL(k_pages_move, dim3(rest), dim3(kNt), 0, st, a);
 }
 
 }  // namespace vsmp
