@@ -19,6 +19,11 @@ free them as they finish (continuous batching); each step samples only the live 
     res = dec.serve([Request(prompt, Opts(max_tokens=32, seed=7), arrival=3), ...], logits_fn, stop_ids={2})
     # logits_fn(reqs, steps, last) -> cuda [len(reqs), V]: each live request's next position
 
+Beam search keeps `width` beams of every prompt, and lets the states behind them follow (include/vsmp_beam.h):
+
+    res = BeamDecoder(4, vocab=V).search(prompts, logits_fn, max_tokens=64, stop_ids={2}, pages=pages, cache=planes)
+    # logits_fn(step, tokens, pages) -> cuda [rows, V]; res[j]: the prompt's sequences as (ids, score), the best first
+
 `Opts` mirrors the reference's option block (`_Opts`, python/verbo/__init__.py:16-25, the C ABI's
 verbo_gen_opts): the fields verbo_generate lets a caller set. Like verbo_generate, which keeps the
 model's repeat_last (src/capi.cpp:131-151), BatchDecoder takes repeat_last (default 64) apart.
@@ -27,9 +32,9 @@ import ctypes
 
 import numpy as np
 
-from . import Params, Penalty, VsmpError, _adjust_args, _err, _penalty_rows, load_library, to_device_penalties
+from . import Context, Params, Penalty, VsmpError, _adjust_args, _err, _penalty_rows, load_library, to_device_penalties
 
-__all__ = ["Opts", "Request", "BatchDecoder", "params_of"]
+__all__ = ["Opts", "Request", "BatchDecoder", "BeamDecoder", "params_of"]
 
 
 class Opts(ctypes.Structure):
@@ -298,3 +303,100 @@ class BatchDecoder:
         if self.lib.vsmp_bsampler_full(self._h, ctypes.c_void_p(stream.cuda_stream)) != 0:
             raise VsmpError("a sequence's history outgrew its slot's region (cap)")
         return list(zip(toks, stopped))
+
+
+class BeamDecoder:
+    """Beam search on one device: `width` beams of each prompt, selected by Context.beam_select, with caches in pages
+    (Context.pages_step) or states held row by row (Context.reorder_rows) that follow them. The reference has no
+    such search; a greedy one (width 1) picks the tokens that its sampler picks at temp 0 (src/sampler.cpp:66-70)."""
+
+    def __init__(self, width, vocab, device=0):
+        self.width, self.vocab, self.device = int(width), int(vocab), int(device)
+        if not 1 <= self.width <= 64 or self.vocab < 1:
+            raise VsmpError("need 1 <= width <= 64 and a vocabulary")
+        self.ctx = Context(self.device)
+
+    def search(self, prompts, logits_fn, max_tokens, stop_ids=(), length_penalty=1.0, pages=None, cache=None, states=None):
+        """For each prompt the best `width` sequences, the best first, as (ids, score): the generated ids (a stop id ends a
+        sequence and is not among them) and their log-probabilities' sum divided by length ** length_penalty, the
+        length counting the stop id. A search ends when it has `width` ended sequences of which none is behind what its
+        best beam would score if it ended now, when no beam is left, or at max_tokens, where the beams count as they are.
+
+        logits_fn(step, tokens, pages) returns device logits [rows, V]. Step 0: a row for each prompt (tokens None); then a
+        row for each beam, width of a prompt one after the other, tokens (device int32 [rows]) their last ids, -1 for
+        a beam that is not live (its logits are not read). pages: None, or a Pages with a row for each prompt, which
+        holds the prompt's tokens; logits_fn gets the state in which each beam has room for its last id. cache: the
+        Planes whose rows are the pages, as Context.pages_step takes them. states: None, or a Planes of len(prompts) *
+        width rows in which row j * width holds prompt j's state when the search begins (its tokens, where the planes
+        have a token_dim); the rows follow their beams after every step. self.pages: the state that the search
+        ended with, all its rows given up."""
+        import torch
+
+        dev = torch.device("cuda", self.device)
+        G, W, ctx = len(prompts), self.width, self.ctx
+        stops = sorted(set(int(t) for t in stop_ids))
+        self.pages = pages
+        if G == 0 or max_tokens <= 0:
+            return [[] for _ in prompts]
+        if pages is not None and pages.lens.numel() != G:
+            raise VsmpError("pages must have a row for each prompt")
+        if states is not None and states.rows != G * W:
+            raise VsmpError("states must have width rows for each prompt")
+        held = None
+        if states is not None and states.token_dim is not None:
+            held = torch.tensor([len(p) for p in prompts], dtype=torch.int32, device=dev).repeat_interleave(W)
+        scores = torch.zeros(G, 1, device=dev)
+        tokens = None
+        back = []                         # per step: each beam's token and its row of the step before
+        ended = [[] for _ in prompts]     # (score, ids)
+        done = [False] * G
+        over = torch.zeros(G, 1, dtype=torch.bool, device=dev)
+
+        def ids_to(step, row):
+            out = []
+            while step >= 0:
+                out.append(int(back[step][0][row]))
+                row = int(back[step][1][row])
+                step -= 1
+            return out[::-1]
+
+        for t in range(int(max_tokens)):
+            lg = logits_fn(t, tokens, pages)
+            if tuple(lg.shape) != (G * (1 if t == 0 else W), self.vocab):
+                raise VsmpError("logits_fn must return [rows, V] logits")
+            sel = ctx.beam_select(lg, scores, W, stop_ids=stops)
+            token, parent, score, end_token, end_parent, end_score, n_end = (x.cpu().numpy() for x in sel)
+            back.append((token.reshape(-1), parent.reshape(-1)))
+            length = float(t + 1) ** length_penalty
+            for g in range(G):
+                if done[g]:
+                    continue
+                for i in range(int(n_end[g])):
+                    ended[g].append((float(end_score[g, i]) / length, ids_to(t - 1, int(end_parent[g, i]))))
+                ended[g].sort(key=lambda e: -e[0])
+                del ended[g][W:]
+                live = token[g, 0] >= 0
+                done[g] = not live or (len(ended[g]) == W and ended[g][-1][0] >= float(score[g, 0]) / length)
+                if not done[g] and t + 1 == max_tokens:
+                    last = [(float(score[g, i]) / length, ids_to(t, g * W + i)) for i in range(W) if token[g, i] >= 0]
+                    ended[g] = sorted(ended[g] + last, key=lambda e: -e[0])[:W]
+                    done[g] = True
+            if all(done):
+                break
+            over = torch.tensor(done, device=dev).view(G, 1)
+            scores = torch.where(over, -float("inf"), sel.score)
+            tokens = torch.where(over, -1, sel.token).view(-1)
+            rows = sel.parent.view(-1)
+            if states is not None:
+                ctx.reorder_rows(states, rows * W if t == 0 else rows, W, lens=held)
+                if held is not None:
+                    held = held + 1
+            if pages is not None:  # a beam that is not live, and all of a search that is over, give up their pages
+                go = tokens >= 0
+                pages, ok = ctx.pages_step(pages, torch.where(go, rows, -1), go.to(torch.int32), cache=cache)
+                if not bool(ok.all()):
+                    raise VsmpError("the pool has no page left for a beam")
+        if pages is not None:
+            n = pages.lens.numel()
+            self.pages, _ = ctx.pages_step(pages, torch.full((n,), -1, dtype=torch.int32, device=dev))
+        return [[(ids, sc) for sc, ids in e] for e in ended]
