@@ -28,7 +28,7 @@ extern "C" {
  * row of -inf alone is not live, nor is one with a NaN or a +inf). The continuations of a group are its live
  * rows' tokens with a logit x above -inf, each with
  *   s = score + (x - lse)
- * in 64 bits (the exponentials are added up in 32 bits a thread, in 64 beyond), in the order of s descending, beam
+ * in 64 bits (the exponentials are added up in 32 bits within a wave, in 64 beyond), in the order of s descending, beam
  * ascending, x descending, token ascending.
  *   logits, dtype, ld: device logits (vsmp_dtype), row r at element r * ld (ld >= V), aligned to their elements.
  *       V <= 1048576 (2^20).
@@ -47,8 +47,8 @@ VSMP_API int vsmp_beam_select(vsmp_ctx* ctx, const void* logits, int dtype, long
                               float* score, int* end_token, int* end_parent, float* end_score, int* n_end, void* stream);
 
 /* Tensors ("planes": the keys of a layer, its values, ...) of the same shape whose rows hold tokens: token t of
- * piece k of row r lies at planes[p] + r * row_stride + k * piece_stride + t * token_bytes, all in bytes. Rows and
- * pieces do not overlap: pieces lie within their rows, or rows within pieces. */
+ * piece k of row r lies at planes[p] + r * row_stride + k * piece_stride + t * token_bytes, all in bytes. Planes do not
+ * overlap, nor do rows and pieces: pieces lie within their rows, or rows within pieces. */
 typedef struct {
   void* const* planes;    /* DEVICE array of n_planes addresses */
   int n_planes;
@@ -110,7 +110,8 @@ VSMP_API int vsmp_pages_step(vsmp_ctx* ctx, const vsmp_pages* from, const vsmp_p
 
 /* A cache in pages moved together: of its n pages in use (ref > 0) those at n and beyond, in ascending order, move to the
  * free ones below n, in ascending order, in every plane of `cache`; tables and ref follow.
- *   from, to: as vsmp_pages_step's, to->rows = from->rows. `from` stays as it is, and so do its pages' tokens.
+ *   from, to: as vsmp_pages_step's, to->rows = from->rows. `from` stays as it is, and so do its pages' tokens. A table
+ *       entry whose page is not in use becomes -1.
  *   moved: device int[n_pages], or NULL: each page's new number, -1 for a page that was free (for pages that the
  *       caller holds).
  *   live: device int[1], or NULL: n.

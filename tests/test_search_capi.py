@@ -75,6 +75,9 @@ SELECT = dict(ctx=CTX, x=X, dtype=0, ld=100, G=2, W=3, V=100, scores=A, N=3, sto
     (dict(end_token=E), "go together"),
     (dict(end_token=E, end_parent=E, end_score=E), "go together"),
     (dict(n_end=E), "go together"),
+    (dict(token=B + 2), "outputs must be aligned"),
+    (dict(score=D + 1), "outputs must be aligned"),
+    (dict(end_token=E, end_parent=E, end_score=E, n_end=E + 2), "outputs must be aligned"),
 ])
 def test_select_refuses(change, words):
     assert words in refused("vsmp_beam_select", *dict(SELECT, **change).values())

@@ -625,9 +625,7 @@ def test_pages_rows_that_ask_for_more_than_there_is(ctx, rows, row_pages):
     table = torch.full((1, row_pages), -1, dtype=torch.int32, device="cuda")
     pages = V.Pages(table.expand(1, row_pages), i32([0]), i32(np.zeros(P)), 1 if row_pages > 40 else 1 << 24)
     T = pages.page_tokens
-    out = torch.full((1, row_pages), 7, dtype=torch.int32, device="cuda").expand(1, row_pages)
-    # a table of 8,192 rows of 2^20 entries would take 32 GB: the rows beyond the first few ask through add alone
-    n = 64 if row_pages > 40 else rows
+    n = 64 if row_pages > 40 else rows  # (8,192 rows of 2^20 entries would take 32 GB)
     to = V.Pages(torch.empty(n, row_pages, dtype=torch.int32, device="cuda"), i32(np.zeros(n)), i32(np.zeros(P)), T)
     want = np.full(n, row_pages * T if row_pages > 40 else 40 * T)
     want[:2] = 5 * T, 7 * T
@@ -737,6 +735,68 @@ def test_a_step_in_a_graph_beside_eager_work(ctx):
         for a, b in zip(got, seen()):
             assert torch.equal(a, b)
         scores.copy_(-torch.rand(G, W, device="cuda").sort(1).values * 3)
+
+
+def test_a_first_call_in_a_capture_is_refused():
+    """A context without the operators' scratch would have to allocate it: refused with a message, and the capture goes on."""
+    import torch
+
+    fresh = V.Context(0)
+    x, scores = torch.zeros(2, 100, device="cuda"), torch.zeros(1, 2, device="cuda")
+    pages, to = V.Pages.empty(2, 4, 10, 4), V.Pages.empty(2, 4, 10, 4)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = x + 1
+        for call in (lambda: fresh.beam_select(x, scores), lambda: fresh.pages_step(pages, add=1, out=to),
+                     lambda: fresh.pages_compact(pages, out=to)):
+            with pytest.raises(V.VsmpError, match="before capturing"):
+                call()
+    g.replay()
+    torch.cuda.synchronize()
+    assert y[0, 0].item() == 1.0
+
+
+def test_python_refuses_what_is_not_a_cache(ctx):
+    """Planes and pages of other shapes, strides, types and sizes than the operators take."""
+    import torch
+
+    x = torch.zeros(4, 3, 8, 5, device="cuda")
+    i = torch.zeros(4, dtype=torch.int32, device="cuda")
+    for make, words in (
+        (lambda: V.Planes([x, x]), "of their own"),
+        (lambda: V.Planes([x, torch.zeros(4, 3, 8, 4, device="cuda")]), "one shape"),
+        (lambda: V.Planes([x, x.clone().half()]), "one shape"),
+        (lambda: V.Planes([x], token_dim=4), "token_dim"),
+        (lambda: V.Planes([x], token_dim=0), "token_dim"),
+        (lambda: V.Planes([x.transpose(2, 3)], token_dim=2), "side by side"),
+        (lambda: V.Planes([x[:, :, :, ::2]], token_dim=2), "side by side"),
+        (lambda: V.Planes([torch.zeros(4, 3, 2, 16, 5, device="cuda")[:, :, :, ::2]], token_dim=3), "side by side"),
+        (lambda: V.Planes([torch.zeros(4, 3, 4, 8, 5, device="cuda")[:, :, :3]], token_dim=3), "one stride"),
+        (lambda: V.Planes([x[:0]]), "at least one"),
+        (lambda: V.Pages(i, i, i, 4), "2-D int32"),
+        (lambda: V.Pages(torch.zeros(4, 2, device="cuda"), i, i, 4), "2-D int32"),
+        (lambda: V.Pages(torch.zeros(2, 4, dtype=torch.int32, device="cuda").t(), i, i, 4), "contiguous rows"),
+        (lambda: V.Pages(torch.zeros(3, 4, dtype=torch.int32, device="cuda"), i, i, 4), "an entry for each row"),
+        (lambda: V.Pages(torch.zeros(4, 4, dtype=torch.int32, device="cuda"), i.float(), i, 4), "lens"),
+        (lambda: V.Pages(torch.zeros(4, 4, dtype=torch.int32, device="cuda"), i.view(2, 2), i, 4), "one-dimensional"),
+        (lambda: ctx.beam_select(torch.zeros(4, 10, device="cuda"), torch.zeros(4, device="cuda")), "scores"),
+        (lambda: ctx.beam_select(torch.zeros(4, 10, device="cuda"), torch.zeros(1, 3, device="cuda")), "scores"),
+        (lambda: ctx.beam_select(torch.zeros(4, 10, device="cuda"), torch.zeros(1, 4, device="cuda").double()), "scores"),
+        (lambda: ctx.beam_select(torch.zeros(4, 10, device="cuda").double(), torch.zeros(1, 4, device="cuda")), "float32, bfloat16"),
+        (lambda: ctx.beam_select(torch.zeros(4, 10, device="cuda"), torch.zeros(1, 4, device="cuda"), 0), "n >= 1"),
+        (lambda: ctx.beam_select(torch.zeros(4, 10, device="cuda"), torch.zeros(1, 4, device="cuda"), 4, range(17)), "n_stop"),
+        (lambda: ctx.reorder_rows(V.Planes([x]), i.long(), 4), "parent"),
+        (lambda: ctx.reorder_rows(V.Planes([x]), i[:3], 4), "parent"),
+        (lambda: ctx.reorder_rows(V.Planes([x]), i, 3), "width"),
+        (lambda: ctx.pages_step(V.Pages.empty(4, 2, 4, 4), add=i.float()), "add"),
+        (lambda: ctx.pages_step(V.Pages.empty(4, 2, 4, 4), cache=V.Planes([x], token_dim=2)), "page_tokens tokens"),
+    ):
+        with pytest.raises(V.VsmpError, match=words):
+            make()
+    p = V.Pages.empty(4, 2, 4, 4)
+    with pytest.raises(V.VsmpError, match="must not overlap"):
+        ctx.pages_step(p, add=1, out=p)
 
 
 def test_on_another_stream(ctx):

@@ -495,6 +495,8 @@ class Planes:
         for u in self.tensors:
             if u.shape != t.shape or u.stride() != t.stride() or u.dtype != t.dtype or u.device != t.device:
                 raise VsmpError("planes must have one shape, one type, the same strides and one device")
+        if len(set(u.data_ptr() for u in self.tensors)) != len(self.tensors):
+            raise VsmpError("planes must be tensors of their own")
         size, n = t.element_size(), t.dim()
         dim = None if token_dim is None else int(token_dim) + (n if token_dim < 0 else 0)
         if dim is not None and not 1 <= dim < n:
@@ -806,10 +808,8 @@ class Context:
             out = pages.like(None if parent is None else parent.numel(), stream)
         rows = out.lens.numel()
         every = 0
-        if isinstance(add, int):
-            add, every = None, add
-        if parent is None and add is None and rows != pages.lens.numel():
-            raise VsmpError("without parents the next state has the rows of this one")
+        if not hasattr(add, "data_ptr"):
+            add, every = None, int(add)
         ok = T.output((rows,), T.int32, dev, stream)
         if out.device != dev:
             raise VsmpError("out must be on the pages' device")

@@ -151,7 +151,7 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
     struct {
       Cand cand[kCands];
       Cand end[kBeamMax * kBeamStops];
-      unsigned short lists[kBeamMax * kBeamMax];
+      unsigned char lists[kNt];
     } group;
     Cand merge[kW][kBeamMax];
   };
@@ -301,7 +301,7 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
   }
   __syncthreads();
   const int slot = row * a.P + part;
-  const int lists = a.W * a.P, entries = lists * a.N;
+  const int lists = a.W * a.P, entries = lists * a.N;  // at most kNt lists (beam_parts)
   const unsigned long long* keys = a.s.key + static_cast<long long>(first) * a.P * a.N;
   const int n_ends = a.end_token ? a.W * a.n_stop : 0;
   // pieces of both ways to go on from here
@@ -539,8 +539,6 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
   // the N-th of the first entries that a wave's threads have, their scores as fp32 below them: the largest of the
   // waves' is a bound for all entries
   uint32_t top = tid < heads ? below_score(entry(head, beam_of(tid >> a.log_j))) : 0u;
-#pragma unroll 1
-  for (int i = tid + kNt; i < heads; i += kNt) top = max(top, below_score(entry(head_of(i), beam_of(i >> a.log_j))));
   if (wv * 64 < heads) sort64(top, lane, false);
   if (lane == a.N - 1) s_bound[wv] = top;
   __syncthreads();
@@ -555,9 +553,8 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
   // the entries that reach it: of all lists, or of those whose first one does
   int some = lists;
   if (!few) {
-#pragma unroll 1
-    for (int l = tid; l < lists; l += kNt)
-      if (entry(agent_load(&keys[l * a.N]), beam_of(l)).s >= bound) sh.group.lists[atomicAdd(&s_lists, 1)] = static_cast<unsigned short>(l);
+    if (tid < lists && entry(agent_load(&keys[tid * a.N]), beam_of(tid)).s >= bound)
+      sh.group.lists[atomicAdd(&s_lists, 1)] = static_cast<unsigned char>(tid);
     __syncthreads();
     some = s_lists;
   }
@@ -624,6 +621,10 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
 
 }  // namespace
 
+// Workgroups of four a CU or fewer, each of whole steps. Measured for one, two, four and eight a CU, us: 64 x 8 x 128,256
+// fp32 52.8, 52.7, 50.0, 55.7; 16 x 16 x 128,256 bf16 44.9, 31.6, 29.5, 34.8; 24 x 5 x 50,257 f16 23.3, 18.4, 15.4, 15.4; 200 x
+// 5 x 50,257 fp32 41.6, 41.6, 41.5, 49.0 (1,000 rows: one part each; two, more than four a CU, 49.5). No more lists than
+// threads in the group's last part: 1 x 8 x 151,936 in 32 parts a row 13.6, in 38 16.0.
 void beam_parts(int B, int W, int V, int dtype, int cus, int* P, int* L) {
   const int step = kNt * 4 * (dtype == VSMP_F32 ? 4 : 8);
   const int steps = (V + step - 1) / step;

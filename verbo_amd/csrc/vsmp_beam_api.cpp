@@ -110,6 +110,10 @@ int vsmp_beam_select(vsmp_ctx* ctx, const void* logits, int dtype, long long ld,
   if ((end_token == nullptr) != (end_parent == nullptr) || (end_token == nullptr) != (end_score == nullptr) ||
       (end_token == nullptr) != (n_end == nullptr))
     return set_error("vsmp: end_token, end_parent, end_score and n_end go together");
+  for (const void* p : {static_cast<const void*>(token), static_cast<const void*>(parent), static_cast<const void*>(score),
+                        static_cast<const void*>(end_token), static_cast<const void*>(end_parent), static_cast<const void*>(end_score),
+                        static_cast<const void*>(n_end)})
+    if (!aligned(p, 4)) return set_error("vsmp: outputs must be aligned to 4 bytes");
   vsmp::DeviceScope scope(vsmp::ctx_device(ctx));
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (!scope.ok() || !vsmp::stream_on_device(ctx, st)) return -1;

@@ -22,6 +22,13 @@ __device__ __forceinline__ T agent_add(T* p, T v) {
   return __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// What this thread has stored and added so far is in memory.
+__device__ __forceinline__ void drain() {
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+
 // ---- k_reorder -------------------------------------------------------------------------------------------
 
 template <int B>
@@ -264,7 +271,7 @@ __global__ __launch_bounds__(kTakeNt) void k_pages_take(PageArgs a) {
     const unsigned long long is_free = __ballot(ref <= 0);
     if (lane == 0 && p < P) agent_store(&a.s.bits[p >> 6], is_free);
   }
-  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  drain();
   __syncthreads();
   if (tid == 0) s_last = agent_add(a.s.tick, 1u) == gridDim.x - 1;
   __syncthreads();
@@ -419,7 +426,7 @@ __global__ __launch_bounds__(kTakeNt) void k_pages_small(PageArgs a) {
                              __HIP_MEMORY_SCOPE_AGENT);
     }
   }
-  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  drain();
   __syncthreads();
   if (!alone) {
     if (tid == 0) s_last = agent_add(a.s.tick, 1u) == gridDim.x - 1;
@@ -460,7 +467,7 @@ __global__ __launch_bounds__(kTakeNt) void k_pages_small(PageArgs a) {
       if (was[k] <= 0 && ref > 0) atomicAnd(&s_bits[p[k] >> 6], ~(1ull << (p[k] & 63)));
     }
   }
-  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  drain();
   __syncthreads();
   const bool away = begun >= 0 && (agent_load(&a.to.ref[begun]) != writers ||
                                    order != (static_cast<unsigned long long>(r.len) << 32 | static_cast<uint32_t>(~tid)));
@@ -570,7 +577,7 @@ __global__ __launch_bounds__(kTakeNt) void k_pages_scan(PageArgs a) {
     }
   }
   if (!alone) {
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    drain();
     __syncthreads();
     if (tid == 0) s_last = agent_add(a.s.tick, 1u) == gridDim.x - 1;
     __syncthreads();
