@@ -347,6 +347,20 @@ def test_reorder_far_rows(ctx):
     assert [int(x[i].min()) for i in range(4)] == [3, 1, 3, 2] == [int(x[i].max()) for i in range(4)]
 
 
+def test_reorder_more_than_the_caches_hold(ctx):
+    """700 MB, whose stores are streamed."""
+    import torch
+
+    n = 175 << 20
+    x = torch.empty(4, n, dtype=torch.uint8, device="cuda")
+    for i in range(4):
+        x[i].random_(50 * i, 50 * i + 50, generator=torch.Generator(device="cuda").manual_seed(i))
+    sums = [int(x[i].to(torch.int64).sum()) for i in range(4)]
+    log("reorder 700 MB")
+    ctx.reorder_rows(V.Planes([x]), i32([3, 0, 0, 2]), 4)
+    assert [int(x[i].to(torch.int64).sum()) for i in range(4)] == [sums[k] for k in (3, 0, 0, 2)] and torch.equal(x[1], x[2])
+
+
 # ---- a cache in pages ------------------------------------------------------------------------------------
 
 

@@ -73,6 +73,7 @@ struct ReorderArgs {
   const int* parent;         // of the whole batch
   const int* len;            // null: all tokens
   int width;
+  bool streams;              // the planes hold more than the caches do (launch_reorder)
   int unit;                  // 0: tokens are whole columns; else bytes that divide a token (launch_reorder)
 };
 

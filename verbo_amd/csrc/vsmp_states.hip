@@ -45,6 +45,10 @@ template <class T>
 __device__ __forceinline__ void set(Bytes* p, T v) {
   *(__attribute__((address_space(1))) T*)p = v;
 }
+template <class T>
+__device__ __forceinline__ void stream(Bytes* p, T v) {  // of more than the caches hold
+  __builtin_nontemporal_store(v, (__attribute__((address_space(1))) T*)p);
+}
 
 template <class T>
 using Loose __attribute__((aligned(1))) = T;
@@ -118,9 +122,15 @@ __global__ __launch_bounds__(kNt, MAXW == 8 ? 4 : 1) void k_reorder(ReorderArgs 
 #pragma unroll
       for (int i = 0; i < MAXW; ++i)
         if (i < n) v[i] = get<vec>(base + s_from[i]);
+      if (a.streams) {
 #pragma unroll
-      for (int i = 0; i < MAXW; ++i)
-        if (i < n) set<vec>(base + s_to[i], v[i]);
+        for (int i = 0; i < MAXW; ++i)
+          if (i < n) stream<vec>(base + s_to[i], v[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < MAXW; ++i)
+          if (i < n) set<vec>(base + s_to[i], v[i]);
+      }
     } else if (a.unit) {  // beyond some row's tokens
       if (a.unit == 4) ends<MAXW, B, uint32_t>(base, at, n, s_from, s_to, s_bytes);
       else if (a.unit == 2) ends<MAXW, B, uint16_t>(base, at, n, s_from, s_to, s_bytes);
@@ -367,33 +377,12 @@ __global__ __launch_bounds__(kTakeNt) void k_pages_small(PageArgs a) {
   __shared__ int s_last, s_copies;
   const int tid = threadIdx.x, lane = tid & 63, P = a.to.n_pages, T = a.to.page_tokens, R = a.to.rows, words = (P + 63) / 64;
   const bool alone = gridDim.x == 1;  // nothing to hand over
-  // this thread's row in the last workgroup, and the begun page that it grows in: loaded beside the rest
-  RowPlan r{-1, 0, 0, true};
-  int begun = -1;
-  if (tid < R) {
-    r = row_plan(a, tid);
-    if (r.want > r.len && r.len % T) begun = a.from.table[r.src * a.from.ldt + r.len / T];
-    if (!is_page(begun, P)) begun = -1;
-  }
-  // the pages of this workgroup: all of them if it is alone
-  const int wg = static_cast<int>(blockIdx.x) - a.table_wgs;
-  for (int p0 = alone ? tid & ~63 : wg >= 0 ? (wg * kTakeNt + tid) & ~63 : P; p0 < P; p0 += alone ? kTakeNt : (gridDim.x - a.table_wgs) * kTakeNt) {
-    int ref = 1;
-    if (p0 + lane < P) {
-      ref = a.from.ref[p0 + lane];
-      if (!WHOLE) {
-        const int d = a.s.delta[p0 + lane];
-        ref += d;
-        if (d) a.s.delta[p0 + lane] = 0;
-      }
-      agent_store(&a.to.ref[p0 + lane], ref);
-    }
-    const unsigned long long is_free = __ballot(ref <= 0);
-    if (lane == 0) {
-      if (alone) s_bits[p0 >> 6] = is_free;
-      else agent_store(&a.s.bits[p0 >> 6], is_free);
-    }
-  }
+  // The pages of this workgroup, all of them if it is alone: what does not wait for other loads is loaded first.
+  const int wg = static_cast<int>(blockIdx.x) - a.table_wgs, pages = (alone ? 1 : gridDim.x - a.table_wgs) * kTakeNt;
+  int p0 = alone ? tid & ~63 : wg >= 0 ? (wg * kTakeNt + tid) & ~63 : P;
+  auto load_ref = [&](int p) { return p < P ? a.from.ref[p] : 1; };
+  auto load_delta = [&](int p) { return !WHOLE && p < P ? a.s.delta[p] : 0; };
+  int ref = load_ref(p0 + lane), gain = load_delta(p0 + lane);
   // its table entries: those of `to`, and the rows beyond it that `from` has
   const uint32_t cap = static_cast<uint32_t>(a.to.row_pages);
   const uint32_t entries = WHOLE ? static_cast<uint32_t>(max(a.from.rows, R)) * cap : 0u, step = (alone ? 1 : a.table_wgs) * kTakeNt;
@@ -425,6 +414,26 @@ __global__ __launch_bounds__(kTakeNt) void k_pages_small(PageArgs a) {
       __hip_atomic_fetch_max(&a.s.order[now], static_cast<unsigned long long>(o.len) << 32 | static_cast<uint32_t>(~i), __ATOMIC_RELAXED,
                              __HIP_MEMORY_SCOPE_AGENT);
     }
+  }
+  // this thread's row in the last workgroup, and the begun page that it grows in
+  RowPlan r{-1, 0, 0, true};
+  int begun = -1;
+  if (tid < R) {
+    r = row_plan(a, tid);
+    if (r.want > r.len && r.len % T) begun = a.from.table[r.src * a.from.ldt + r.len / T];
+    if (!is_page(begun, P)) begun = -1;
+  }
+  for (; p0 < P; p0 += pages) {
+    ref += gain;
+    const unsigned long long is_free = __ballot(ref <= 0);
+    if (p0 + lane < P) agent_store(&a.to.ref[p0 + lane], ref);
+    if (gain) a.s.delta[p0 + lane] = 0;
+    if (lane == 0) {
+      if (alone) s_bits[p0 >> 6] = is_free;
+      else agent_store(&a.s.bits[p0 >> 6], is_free);
+    }
+    ref = load_ref(p0 + pages + lane);
+    gain = load_delta(p0 + pages + lane);
   }
   drain();
   __syncthreads();
@@ -503,6 +512,7 @@ __device__ __forceinline__ uint32_t chunks_of(const PlaneArgs& c, int tokens) {
   const uint32_t cols = (static_cast<uint32_t>(tokens) * static_cast<uint32_t>(c.token_bytes) + 15) / 16;
   return (cols * static_cast<uint32_t>(c.pieces) + kChunk - 1) / kChunk;
 }
+template <bool STREAM>
 __device__ __forceinline__ void copy_tokens(const PlaneArgs& c, uint32_t plane, int src, int dst, int tokens, uint32_t chunk) {
   typedef Column<16> vec;
   const uint32_t run = static_cast<uint32_t>(tokens) * static_cast<uint32_t>(c.token_bytes);
@@ -525,7 +535,7 @@ __device__ __forceinline__ void copy_tokens(const PlaneArgs& c, uint32_t plane, 
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k)
-    if (n[k] == 16) set<vec>((Bytes*)from[k] + there, v[k]);
+    if (n[k] == 16) STREAM ? stream<vec>((Bytes*)from[k] + there, v[k]) : set<vec>((Bytes*)from[k] + there, v[k]);
   // the runs' ends
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -553,7 +563,7 @@ __global__ __launch_bounds__(kNt) void k_page_copy(PageArgs a) {
   for (uint32_t u = wave_of_grid(); u < total; u += gridDim.x * (kNt / 64)) {
     const CopyUnit w = copy_unit(a, u, chunks);
     const PageCopy c = a.s.copies[w.page];
-    if (w.chunk < chunks_of(a.cache, c.tokens)) copy_tokens(a.cache, w.plane, c.src, a.to.table[c.row * a.to.ldt + c.at], c.tokens, w.chunk);
+    if (w.chunk < chunks_of(a.cache, c.tokens)) copy_tokens<false>(a.cache, w.plane, c.src, a.to.table[c.row * a.to.ldt + c.at], c.tokens, w.chunk);
   }
 }
 
@@ -678,7 +688,7 @@ __global__ __launch_bounds__(kNt) void k_pages_move(PageArgs a) {
   const uint32_t total = static_cast<uint32_t>(moves) * static_cast<uint32_t>(a.cache.n_planes) * chunks;
   for (uint32_t u = wave_of_grid(); u < total; u += gridDim.x * (kNt / 64)) {
     const CopyUnit w = copy_unit(a, u, chunks);
-    copy_tokens(a.cache, w.plane, a.s.moves[w.page], a.s.room[w.page], a.cache.tokens, w.chunk);
+    copy_tokens<true>(a.cache, w.plane, a.s.moves[w.page], a.s.room[w.page], a.cache.tokens, w.chunk);
   }
 }
 
@@ -694,6 +704,7 @@ void launch_reorder(ReorderArgs a, int groups, int cus, hipStream_t st) {
   a.unit = a.p.token_bytes % bytes == 0 ? 0 : a.p.token_bytes % 4 == 0 ? 4 : a.p.token_bytes % 2 == 0 ? 2 : 1;
   const long long cols = (static_cast<long long>(a.p.tokens) * a.p.token_bytes + bytes - 1) / bytes * a.p.n_planes * a.p.pieces;
   const long long most = (cols + kNt - 1) / kNt;
+  a.streams = cols * bytes * a.width * groups > 512ll << 20;
   const int blocks = static_cast<int>(std::max<long long>(1, std::min<long long>(most, (64ll * cus + groups - 1) / groups)));
   if (a.width <= 4) go_reorder<4, 16>(a, groups, blocks, st);
   else if (a.width <= 8) go_reorder<8, 16>(a, groups, blocks, st);
