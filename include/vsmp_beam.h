@@ -103,7 +103,7 @@ typedef struct {
  *       the caller copies by itself or has nothing to copy.
  *   ok: device int[to->rows], or NULL.
  * Rows that no row of `to` has for its parent give up their pages; so do all those of `from` beyond to->rows. The
- * context holds about 18 MB of scratch from the first call of vsmp_pages_step or vsmp_pages_compact on; a call that is
+ * context holds about 26 MB of scratch from the first call of vsmp_pages_step or vsmp_pages_compact on; a call that is
  * captured into a graph needs one before it. Returns 0 or -1. */
 VSMP_API int vsmp_pages_step(vsmp_ctx* ctx, const vsmp_pages* from, const vsmp_pages* to, const int* parent,
                              const int* add, int add_all, const vsmp_planes* cache, int* ok, void* stream);

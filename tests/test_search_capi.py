@@ -34,6 +34,24 @@ def test_header_compiles_as_c_and_the_structs_have_their_layout(tmp_path):
                     str(tmp_path / "h.o")], check=True)
 
 
+@pytest.mark.skipif(shutil.which("g++") is None, reason="g++ absent")
+def test_the_documented_step_compiles(tmp_path):
+    """The C++ block that INTEGRATION.md shows for these calls, with the variables that it names."""
+    block = [b for b in re.findall(r"```cpp\n(.*?)```", (ROOT / "INTEGRATION.md").read_text(), re.S) if "vsmp_beam.h" in b]
+    assert len(block) == 1
+    body = "\n".join(line for line in block[0].splitlines() if not line.startswith("#include"))
+    src = tmp_path / "step.cpp"
+    src.write_text("""#include "vsmp_beam.h"
+void step(vsmp_ctx* ctx, const void* d_logits, long long ld, int G, int W, int V, const float* d_scores, const int* stops, int n_stop,
+          int* d_token, int* d_parent, float* d_score, int* d_end_token, int* d_end_parent, float* d_end_score, int* d_n_end,
+          void* const* d_planes, int n_planes, long long row_stride, int heads, long long piece_stride, int room, int token_bytes,
+          int* d_lens, void* const* d_pools, int n_pages, int page_tokens, int row_pages, int* d_table, int* d_ref,
+          int* d_next_table, int* d_next_lens, int* d_next_ref, int* d_ok, void* stream) {
+""" + body + "\n}\n")
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-Wextra", "-Werror", "-I", str(ROOT / "include"), "-c", str(src), "-o",
+                    str(tmp_path / "step.o")], check=True)
+
+
 # Addresses that only the argument checks see: a call that they refuse reads nothing behind them.
 CTX, X, A, B, C, D, E, F = (1 << 20, *(k << 34 for k in range(1, 8)))
 
