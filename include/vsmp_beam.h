@@ -100,7 +100,8 @@ typedef struct {
  *       parent is row i.
  *   add: device int[to->rows], or NULL for add_all everywhere.
  *   cache: HOST pointer to the planes whose rows are the pages (rows = n_pages, tokens = page_tokens), or NULL where
- *       the caller copies by itself or has nothing to copy.
+ *       the caller copies by itself or has nothing to copy. Half of the pool's pages, and a page of each row, hold fewer
+ *       than 2^31 pieces of 4 KB (or less) in all planes.
  *   ok: device int[to->rows], or NULL.
  * Rows that no row of `to` has for its parent give up their pages; so do all those of `from` beyond to->rows. The
  * context holds about 26 MB of scratch from the first call of vsmp_pages_step or vsmp_pages_compact on; a call that is

@@ -193,6 +193,10 @@ def test_steps_refuse():
         args = [CTX, ax, ay, ap, None, None, None]
         args[k] = E + 2
         assert "aligned" in refused("vsmp_pages_compact", *args)
+    q = planes(n_planes=1 << 16, rows=1 << 18, tokens=16)
+    big = [pages(at << 4, n_pages=1 << 18, lens=(at << 4) + (1 << 24), ref=(at << 4) + (1 << 25)) for at in (C, D)]
+    for fn, rest in (("vsmp_pages_step", (None, None, 1, ctypes.addressof(q), None, None)), ("vsmp_pages_compact", (ctypes.addressof(q), None, None, None))):
+        assert "too many planes" in refused(fn, CTX, ctypes.addressof(big[0]), ctypes.addressof(big[1]), *rest)
     z = pages(D, rows=5)
     assert "same rows" in refused("vsmp_pages_compact", CTX, ax, ctypes.addressof(z), None, None, None, None)
     for change, words in PLANES_REFUSED + [(dict(rows=11), "n_pages rows"), (dict(tokens=15), "n_pages rows"), (dict(rows=13), "n_pages rows")]:

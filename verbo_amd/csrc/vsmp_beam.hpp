@@ -17,6 +17,7 @@ constexpr int kBeamPad = 32;          // 32-bit words between two groups' ticket
 constexpr int kPagesMax = 1 << 20;    // pages of a pool
 constexpr int kPageRows = 8192;       // rows of a paged cache
 constexpr int kPageRoom = 1 << 30;    // tokens of a row
+constexpr int kPageChunk = 256;       // 16-byte columns of a plane that a wave copies at a time
 
 // Device scratch of vsmp_beam_select: allocated by a context's first call, never replaced. The tickets are zero
 // between calls, which the last part of a group sees to.
@@ -108,7 +109,7 @@ struct PageArgs {
   PlaneArgs cache;              // n_planes 0: none
   uint32_t m_cap;               // (2^32 - 1) / to.row_pages, and workgroups for the tables (launch_pages_step)
   int table_wgs;
-  uint32_t m_chunks, m_planes;  // (2^32 - 1) / a page's chunks, and cache.n_planes (copy_planes)
+  uint32_t m_chunks, m_planes;  // (2^32 - 1) / a page's chunks, and cache.n_planes (copy_wgs)
   PageScratch s;
 };
 
@@ -117,6 +118,6 @@ void beam_parts(int B, int W, int V, int dtype, int cus, int* P, int* L);
 void launch_beam(BeamArgs a, int dtype, hipStream_t st);
 void launch_reorder(ReorderArgs a, int groups, int cus, hipStream_t st);
 void launch_pages_step(PageArgs a, int cus, hipStream_t st);
-void launch_pages_compact(const PageArgs& a, int cus, hipStream_t st);
+void launch_pages_compact(PageArgs a, int cus, hipStream_t st);
 
 }  // namespace vsmp

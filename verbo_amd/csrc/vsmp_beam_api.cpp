@@ -78,6 +78,11 @@ int check_step(const vsmp_pages* from, const vsmp_pages* to, const vsmp_planes* 
     if (check_planes(*cache) != 0) return -1;
     if (cache->rows != to->n_pages || cache->tokens != to->page_tokens)
       return set_error("vsmp: the cache's planes must have n_pages rows of page_tokens tokens");
+    // copies are counted with 31 bits, a plane's 4 KB of a page each
+    const long long cols = (static_cast<long long>(cache->tokens) * cache->token_bytes + 15) / 16 * cache->pieces;
+    const long long chunks = (cols + kPageChunk - 1) / kPageChunk, pages = std::max(to->n_pages / 2 + 1, to->rows);
+    if (chunks * cache->n_planes > INT32_MAX / pages)
+      return set_error("vsmp: too many planes for so many pages: fewer than 2^31 pieces of 4 KB in half of the pool, or in a page of each row");
   }
   return 0;
 }

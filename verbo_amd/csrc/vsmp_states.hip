@@ -517,7 +517,7 @@ __global__ __launch_bounds__(kTakeNt) void k_pages_small(PageArgs a) {
 // Tokens of a page into another page of a plane: a wave's chunk, four 16-byte columns a lane. The columns of all pieces
 // follow one another. Bound by reads and writes together: of 10,007 pages of 8 KB in 56 planes some 2,480 move, 2.26 GB, 477
 // us (4.7 TB/s); by workgroups of one plane's 16 KB 474, of several planes' (each lane loads its plane's address first) 512.
-constexpr int kChunk = 64 * 4;
+constexpr int kChunk = kPageChunk;
 __device__ __forceinline__ uint32_t chunks_of(const PlaneArgs& c, int tokens) {
   const uint32_t cols = (static_cast<uint32_t>(tokens) * static_cast<uint32_t>(c.token_bytes) + 15) / 16;
   return (cols * static_cast<uint32_t>(c.pieces) + kChunk - 1) / kChunk;
@@ -723,21 +723,13 @@ void launch_reorder(ReorderArgs a, int groups, int cus, hipStream_t st) {
   else go_reorder<64, 8>(a, groups, blocks, st);
 }
 
-// Copies of up to n pages, by `launch` with at most `most` workgroups, in as many planes at a time as 31 bits count the
-// waves' chunks of (all of them, but for pools that hardly fit a card).
-template <class F>
-static void copy_planes(PageArgs a, int n, int most, F launch) {
-  const PlaneArgs c = a.cache;
-  const long long cols = (static_cast<long long>(c.tokens) * c.token_bytes + 15) / 16 * c.pieces, chunks = (cols + kChunk - 1) / kChunk;
-  const int planes = static_cast<int>(std::max<long long>(1, std::min<long long>(c.n_planes, INT32_MAX / (chunks * n))));
+// Workgroups for the copies of up to n pages, at most `most`, and what the waves divide by.
+static unsigned copy_wgs(PageArgs& a, int n, int most) {
+  const long long cols = (static_cast<long long>(a.cache.tokens) * a.cache.token_bytes + 15) / 16 * a.cache.pieces;
+  const long long chunks = (cols + kChunk - 1) / kChunk;
   a.m_chunks = 0xFFFFFFFFu / static_cast<uint32_t>(chunks);
-  for (int p = 0; p < c.n_planes; p += a.cache.n_planes) {
-    a.cache.planes = c.planes + p;
-    a.cache.n_planes = std::min(planes, c.n_planes - p);
-    a.m_planes = 0xFFFFFFFFu / static_cast<uint32_t>(a.cache.n_planes);
-    const long long waves = chunks * n * a.cache.n_planes;
-    launch(a, static_cast<unsigned>(std::min<long long>(most, (waves + kNt / 64 - 1) / (kNt / 64))));
-  }
+  a.m_planes = 0xFFFFFFFFu / static_cast<uint32_t>(a.cache.n_planes);
+  return static_cast<unsigned>(std::min<long long>(most, (chunks * a.cache.n_planes * n + kNt / 64 - 1) / (kNt / 64)));
 }
 
 void launch_pages_step(PageArgs a, int cus, hipStream_t st) {
@@ -757,20 +749,19 @@ void launch_pages_step(PageArgs a, int cus, hipStream_t st) {
     else
       hipLaunchKernelGGL(k_pages_take, dim3(static_cast<unsigned>((a.to.n_pages + kTakePages - 1) / kTakePages)), dim3(kTakeNt), 0, st, a);
   }
-  if (a.cache.n_planes && (a.add || a.add_all > 0))
-    copy_planes(a, a.to.rows, 16 * cus, [&](const PageArgs& c, unsigned wgs) { hipLaunchKernelGGL(k_page_copy, dim3(wgs), dim3(kNt), 0, st, c); });
+  if (a.cache.n_planes && (a.add || a.add_all > 0)) {
+    const unsigned wgs = copy_wgs(a, a.to.rows, 16 * cus);
+    hipLaunchKernelGGL(k_page_copy, dim3(wgs), dim3(kNt), 0, st, a);
+  }
 }
 
-void launch_pages_compact(const PageArgs& a, int cus, hipStream_t st) {
+void launch_pages_compact(PageArgs a, int cus, hipStream_t st) {
   const int P = a.to.n_pages;
   hipLaunchKernelGGL(k_pages_scan, dim3(static_cast<unsigned>((P + kTakePages - 1) / kTakePages)), dim3(kTakeNt), 0, st, a);
   if (P > kSmallPages) hipLaunchKernelGGL(k_pages_pair, dim3(static_cast<unsigned>((P + kNt - 1) / kNt)), dim3(kNt), 0, st, a);
-  // (tables and pool with each launch: there is hardly ever more than one)
-  const unsigned rest = std::min(static_cast<unsigned>(std::max(a.to.rows, (P + kNt - 1) / kNt)), 4u * cus);
-  if (a.cache.n_planes)
-    copy_planes(a, P / 2 + 1, 16 * cus, [&](const PageArgs& c, unsigned wgs) { hipLaunchKernelGGL(k_pages_move, dim3(std::max(rest, wgs)), dim3(kNt), 0, st, c); });
-  else
-    hipLaunchKernelGGL(k_pages_move, dim3(rest), dim3(kNt), 0, st, a);
+  unsigned wgs = std::min(static_cast<unsigned>(std::max(a.to.rows, (P + kNt - 1) / kNt)), 4u * cus);  // tables and pool
+  if (a.cache.n_planes) wgs = std::max(wgs, copy_wgs(a, P / 2 + 1, 16 * cus));
+  hipLaunchKernelGGL(k_pages_move, dim3(wgs), dim3(kNt), 0, st, a);
 }
 
 }  // namespace vsmp
