@@ -375,17 +375,22 @@ __global__ __launch_bounds__(kTakeNt) void k_pages_take(PageArgs a) {
 // What one workgroup writes after another has is written through to memory by both: they may not share an L2.
 //
 // Bound by loads that follow one another (parent, length, table entry; ticket; bits and lists; ref; the pages' stores): 4 rows
-// over 256 pages 8.2 us in one workgroup, 64 rows over 2,048 pages 11.8 us, the copies a launch more. Pages that many rows
+// over 256 pages 7.9 us in one workgroup, 64 rows over 2,048 pages 10.8 us, the copies a launch more. Pages that many rows
 // change at once cost the last workgroup scattered loads and stores (256 rows of which 16 end, 1,300 pages: 19 us); there,
-// from kSmallEntries table entries on, the tables have a launch of their own (3.2 us and 11.4).
+// from kSmallEntries table entries on, the tables have a launch of their own (3.2 us and 10.4).
 constexpr int kSmallPages = 64 * kTakeNt, kSmallEntries = 1 << 13;
 template <bool WHOLE>
 __global__ __launch_bounds__(kTakeNt) void k_pages_small(PageArgs a) {
   __shared__ unsigned long long s_bits[kTakeNt];
   __shared__ int s_before[kTakeNt], s_start[kTakeNt], s_first[kTakeNt];
-  __shared__ int s_last, s_copies;
+  __shared__ int s_list[WHOLE ? 2 * kTakeNt : 1];  // alone: the pages whose holders change, at most two an entry
+  __shared__ int s_last, s_copies, s_changes;
   const int tid = threadIdx.x, lane = tid & 63, P = a.to.n_pages, T = a.to.page_tokens, R = a.to.rows, words = (P + 63) / 64;
-  const bool alone = gridDim.x == 1;  // nothing to hand over
+  const bool alone = WHOLE && gridDim.x == 1;  // nothing to hand over
+  if (alone) {
+    if (tid == 0) s_changes = 0;
+    __syncthreads();
+  }
   // The pages of this workgroup, all of them if it is alone: what does not wait for other loads is loaded first.
   const int wg = static_cast<int>(blockIdx.x) - a.table_wgs, pages = (alone ? 1 : gridDim.x - a.table_wgs) * kTakeNt;
   int p0 = alone ? tid & ~63 : wg >= 0 ? (wg * kTakeNt + tid) & ~63 : P;
@@ -405,19 +410,21 @@ __global__ __launch_bounds__(kTakeNt) void k_pages_small(PageArgs a) {
     const int was = mine && j < had ? a.from.table[i * a.from.ldt + j] : -1;
     const int now = mine && j < keep ? a.from.table[o.src * a.from.ldt + j] : -1;
     if (mine && i < R) agent_store(&a.to.table[i * a.to.ldt + j], now);
-    auto change = [&](int page, bool there, int by) {
-      const unsigned long long at = __ballot(there);
-      if (!at) return;
-      int first = 0;
-      if (lane == 0) first = agent_add(a.s.n_moves, static_cast<int>(__popcll(at)));
-      first = __shfl(first, 0);
-      if (there) {
+    const bool gone = was != now && is_page(was, P), come = was != now && is_page(now, P);
+    const unsigned long long at_gone = __ballot(gone), at_come = __ballot(come), lower = (1ull << lane) - 1ull;
+    const int n_gone = __popcll(at_gone), n_both = n_gone + __popcll(at_come);
+    if (n_both) {
+      int to = 0;
+      if (lane == 0) to = alone ? atomicAdd(&s_changes, n_both) : agent_add(a.s.n_moves, n_both);
+      to = __builtin_amdgcn_readfirstlane(to);
+      auto change = [&](int page, int at, int by) {
         agent_add(&a.s.delta[page], by);
-        agent_store(&a.s.moves[first + __popcll(at & ((1ull << lane) - 1ull))], page);
-      }
-    };
-    change(was, was != now && is_page(was, P), -1);
-    change(now, was != now && is_page(now, P), 1);
+        if (alone) s_list[at] = page;
+        else agent_store(&a.s.moves[at], page);
+      };
+      if (gone) change(was, to + __popcll(at_gone & lower), -1);
+      if (come) change(now, to + n_gone + __popcll(at_come & lower), 1);
+    }
     if (mine && j == o.len / T && o.want > o.len && o.len % T && is_page(now, P)) {
       agent_add(&a.s.writers[now], 1);
       __hip_atomic_fetch_max(&a.s.order[now], static_cast<unsigned long long>(o.len) << 32 | static_cast<uint32_t>(~i), __ATOMIC_RELAXED,
@@ -460,15 +467,18 @@ __global__ __launch_bounds__(kTakeNt) void k_pages_small(PageArgs a) {
     writers = agent_load(&a.s.writers[begun]);
     order = agent_load(&a.s.order[begun]);
   }
-  const int changes = WHOLE ? agent_load(a.s.n_moves) : 0;
+  const int changes = alone ? s_changes : WHOLE ? agent_load(a.s.n_moves) : 0;
   if (!alone && tid < words) s_bits[tid] = agent_load(&a.s.bits[tid]);
   if (tid == 0) s_copies = 0;
   __syncthreads();
-  if (WHOLE && tid == 0) agent_store(a.s.n_moves, 0);
+  if (WHOLE && !alone && tid == 0) agent_store(a.s.n_moves, 0);
   for (int t0 = 0; t0 < changes; t0 += 4 * kTakeNt) {
     int p[4], d[4], was[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) p[k] = t0 + k * kTakeNt + tid < changes ? agent_load(&a.s.moves[t0 + k * kTakeNt + tid]) : -1;
+    for (int k = 0; k < 4; ++k) {
+      const int t = t0 + k * kTakeNt + tid;
+      p[k] = t >= changes ? -1 : alone ? s_list[min(t, 2 * kTakeNt - 1)] : agent_load(&a.s.moves[t]);
+    }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       d[k] = p[k] >= 0 ? agent_load(&a.s.delta[p[k]]) : 0;
