@@ -129,14 +129,15 @@ constexpr int kWait = 144;     // logits that a wave has collected: 64 that wait
 
 // One part of a row: a step of four 16-byte groups a thread at a time, the next in flight; what a row has beyond whole
 // groups, a lane each, in the end. Each wave collects in LDS the logits that reach its bound, below which none can be
-// among the part's N largest that are no stop tokens. The bound is at first the N-th largest of the
-// lanes' maxima over the first step, stop tokens left out of account: few more logits reach it. Where 64 have collected, the wave sorts them into a list over its lanes, whose N-th is the bound from then
-// on. In the end the waves' logits that reach the largest of their bounds are ranked by comparing each with each, a
-// thread each: mostly they are few more than N.
+// among the part's N largest that are no stop tokens. The bound is at first the N-th largest of the lanes' maxima over the
+// first step, stop tokens left out of account: few more logits reach it. It is sharpened to the N-th of what waits as more
+// comes. Where 64 wait, the wave sorts them into a list over its lanes, whose N-th is the bound from then on. In the end
+// the waves' logits that reach the largest of their bounds are ranked by comparing each with each, a thread each: mostly
+// they are few more than N.
 //
 // The last part of a group ranks its rows' lists by score in the same way: the N-th largest first entry of the lists (of
-// those of a wave's threads; several of each list where there are few) is a bound for all entries. Where more entries than kCands reach it (many equal
-// ones) each wave merges lists in order instead, and the first wave the waves'.
+// those of a wave's threads; several of each list where there are few) is a bound for all entries. Where more entries than
+// kCands reach it (many equal ones) each wave merges lists in order instead, and the first wave the waves'.
 //
 // Many rows are bound by the logits' read, in bf16 and f16 by the exponentials too: 64 groups of 8 rows of 128,256 fp32 50.3
 // us (5.2 TB/s), 64 of 16 of 151,936 bf16 80 us (3.9 TB/s). A few rows are bound by latencies that follow one another: one
