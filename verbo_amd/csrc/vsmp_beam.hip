@@ -131,17 +131,18 @@ constexpr int kWait = 144;     // logits that a wave has collected: 64 that wait
 // groups, a lane each, in the end. Each wave collects in LDS the logits that reach its bound, below which none can be
 // among the part's N largest that are no stop tokens. The bound is at first the N-th largest of the lanes' maxima over the
 // first step, stop tokens left out of account: few more logits reach it. It is sharpened to the N-th of what waits as more
-// comes. Where 64 wait, the wave sorts them into a list over its lanes, whose N-th is the bound from then on. In the end
-// the waves' logits that reach the largest of their bounds are ranked by comparing each with each, a thread each: mostly
-// they are few more than N.
+// comes, and to the least of the keys that a quarter of N of each wave's logits reach, which the waves tell each other.
+// Where 64 wait, the wave sorts them into a list over its lanes, whose N-th is the bound from then on. In the end the
+// waves' logits that reach the largest of their bounds are ranked by comparing each with each, a thread each: mostly they
+// are few more than N.
 //
 // The last part of a group ranks its rows' lists by score in the same way: the N-th largest first entry of the lists (of
 // those of a wave's threads; several of each list where there are few) is a bound for all entries. Where more entries than
 // kCands reach it (many equal ones) each wave merges lists in order instead, and the first wave the waves'.
 //
-// Many rows are bound by the logits' read, in bf16 and f16 by the exponentials too: 64 groups of 8 rows of 128,256 fp32 50.3
-// us (5.2 TB/s), 64 of 16 of 151,936 bf16 80 us (3.9 TB/s). A few rows are bound by latencies that follow one another: one
-// group of 4 rows of 49,152 fp32 10.2 us, of which the logits' load and sums take about 3, a part's ranks and their way to
+// Many rows are bound by the logits' read, in bf16 and f16 by the exponentials too: 64 groups of 8 rows of 128,256 fp32 49.4
+// us (5.3 TB/s), 64 of 16 of 151,936 bf16 73 us (4.3 TB/s; 80 with each wave's own bound). A few rows are bound by latencies that follow one another: one
+// group of 4 rows of 49,152 fp32 10.4 us, of which the logits' load and sums take about 3, a part's ranks and their way to
 // memory 2, the ticket 1, the last part's loads 1, and its sums, bound and ranks 3. Every workgroup runs most of the code
 // once; loops stay rolled where they hardly turn, and nothing is divided by what is not a constant. Sorting networks and
 // merges by shuffles through LDS, in the place of bounds and ranks, took 24.6 and 80 us.
@@ -166,7 +167,7 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
   __shared__ Shared sh;
   __shared__ float s_m[kW], s_s[kW];
   __shared__ double s_lse[kBeamMax], s_score[kBeamMax];
-  __shared__ uint32_t s_bound[kW];
+  __shared__ uint32_t s_bound[kW], s_share[kW];
   __shared__ int s_wait[kW], s_n, s_lists, s_end, s_ended, s_last;
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int part = static_cast<int>(blockIdx.x), group = static_cast<int>(blockIdx.z);
@@ -174,7 +175,11 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
   const int lo = part * a.L, hi = min(a.V, lo + a.L), whole = hi & ~(N - 1);
   const char* x = static_cast<const char*>(a.x) + row * a.ld * E::kSize;
   const int stop = lane < a.n_stop ? a.stops[lane] : -1;  // a lane each
+  // A key that a wave's share of N, a quarter, of its logits reach: the least of the waves' is one that N of the part's reach.
+  const int share = (a.N + kW - 1) / kW;
+  if (tid < kW) s_share[tid] = 0u;
   if (tid == 0) s_n = 0;
+  __syncthreads();
 
   Lse z{-INFINITY, 0.0f};
   int waiting = 0;               // logits that the wave has collected
@@ -210,13 +215,25 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
       waiting += __popcll(at);
     };
     int known = 64;              // of those that wait, how many the bound takes into account
+    uint32_t mine = 0;           // what the wave has published
+    auto publish = [&](uint32_t key) {
+      mine = max(mine, key);
+      if (lane == 0) __hip_atomic_store(&s_share[wv], mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    };
+    auto shared = [&]() {        // (what it has of the others may be old: a smaller key, which is as true)
+      uint32_t k[kW];
+#pragma unroll
+      for (int w = 0; w < kW; ++w) k[w] = __hip_atomic_load(&s_share[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      return min(min(k[0], k[1]), min(k[2], k[3]));
+    };
     auto sharpen = [&]() {       // the N-th of the first 64 that wait
       __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
       uint32_t top = lane < waiting ? static_cast<uint32_t>(sh.part.wait[wv][lane] >> 32) : 0u;
       sort64(top, lane, false);
-      top = __builtin_amdgcn_readlane(top, a.N - 1);
-      sure = max(sure, top);
+      const uint32_t nth = __builtin_amdgcn_readlane(top, a.N - 1);
+      sure = max(sure, nth);
       known = waiting;
+      publish(__builtin_amdgcn_readlane(top, share - 1));
     };
     for (int e0 = lo; e0 < whole; e0 += kStep) {
       float v[G * N], gm[G];
@@ -246,13 +263,17 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
       if (e0 == lo && a.N + skip <= 64) {
         uint32_t top = ord_key(mx == mx ? mx : -INFINITY);
         sort64(top, lane, false);
+        const uint32_t few = __builtin_amdgcn_readlane(top, share + skip - 1);
         top = __builtin_amdgcn_readlane(top, a.N + skip - 1);
         known = a.N;
+        if (key_val(few) > -INFINITY) publish(few);
         if (key_val(top) > -INFINITY) {
           bound = key_val(top);
           sure = top;
         }
       }
+      // (equal logits of other waves may come after this wave's, so that those stay)
+      if (const uint32_t k = shared()) bound = fmaxf(bound, key_val(k));
       if (!__ballot(mx >= bound)) continue;
       uint32_t hits = 0;  // the lane's logits that reach the bound, a bit each
 #pragma unroll
@@ -284,11 +305,13 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
           bound = fmaxf(bound, key_val(nth));
           known = 0;
         }
+        publish(__builtin_amdgcn_readlane(static_cast<uint32_t>(best >> 32), share - 1));
       }
       if (waiting > known + max(4, a.N / 2)) sharpen();
       // what comes in later steps has higher tokens: among equal logits it is behind those that N have reached
       if (sure) bound = fmaxf(bound, next_up(key_val(sure)));
     }
+    sure = max(sure, shared());
     if (whole < hi && wv == 0) {
       const float m = fmaxf(z.m, rest), rel = m == -INFINITY ? 0.0f : m;
       z = {m, z.s * exp_rel(z.m, rel) + exp_rel(rest, rel)};
