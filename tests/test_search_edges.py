@@ -1,0 +1,126 @@
+"""Selection where masks are finite numbers and logits are large, and steps of a cache whose rows ask for more pages
+than 32 bits count, on the GPU.
+
+Tolerances count roundings: u = 2^-24 is the most that rounding to fp32 takes, relative to the value."""
+import numpy as np
+import pytest
+
+import verbo_amd as V
+from helpers import log, mode_ctx
+from test_search_ops import INF, U, continuations, i32, torch_type
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    import torch
+
+    assert torch.cuda.is_available(), "the gpu tests need a ROCm device"
+    return mode_ctx()
+
+
+# ---- selection: finite masks, large logits ---------------------------------------------------------------
+
+
+def lse_tolerance(vocab, dtype):
+    """How far a row's log of a sum may be off. Terms at most 40 below the largest (others count for less than e^-40 each)
+    have arguments that are rounded twice on the way from the term to the row's maximum, each time by 40 u at most,
+    and log2 e is off by a quarter of a rounding (10 u): 90 u whatever the number of maxima on the way. An exponential is
+    off by 2 u, what makes good the argument's rounding by 3 u. A thread adds a step of 16 logits (32 of 2 bytes)
+    one by one, then the steps, each with a factor for the new maximum (an exponential and a product, 3 u); the same factor
+    comes in three joins; a wave adds in 6 turns, what is beyond is in 64 bits. A row's end is one step more."""
+    per = 16 if dtype == "f32" else 32
+    steps = -(-vocab // (256 * per)) + 1
+    return (90 + 5 + per + 4 * steps + 9 + 6) * U
+
+
+def check(ctx, x, scores, n, dtype, stops=()):
+    """The step on device rows x against the definition in 64 bits, in which logits of size M leave lse and x - lse with
+    2^-53 M each, here and there. Where two neighbours in the order lie closer than the tolerance either may come first."""
+    import torch
+
+    G, W = scores.shape
+    r = V.BeamStep(*[t.cpu().numpy() for t in ctx.beam_select(x, torch.from_numpy(scores).cuda(), n, stop_ids=stops)])
+    host = x.double().cpu().numpy()
+    vocab = host.shape[1]
+    for g, (s, row, v, tok) in enumerate(continuations(host, scores, W)):
+        rows = host[g * W:(g + 1) * W]
+        tops = np.where(np.isnan(rows), -INF, rows).max(1)
+        big = np.abs(tops[np.isfinite(tops)]).max(initial=0.0)
+        tol = lse_tolerance(vocab, dtype) + 4 * 2.0 ** -53 * big
+        end = np.isin(tok, list(stops))
+        place = {(int(a), int(t)): k for k, (a, t) in enumerate(zip(row, tok))}
+        go = np.flatnonzero(~end)[:n]
+        assert (r.token[g] >= 0).sum() == go.size, (g, r.token[g], go.size)
+        for i in range(go.size):
+            k = place[(int(r.parent[g, i]), int(r.token[g, i]))]
+            # (a score that lies far below has the roundings of its own size)
+            near = tol + 4 * 2.0 ** -53 * abs(s[k])
+            assert not end[k] and abs(float(r.score[g, i]) - s[k]) <= near + U * abs(s[k]), (g, i, r.score[g, i], s[k])
+            if k != go[i]:
+                assert abs(s[k] - s[go[i]]) <= 2 * near and row[k] != row[go[i]], (g, i, s[k], s[go[i]])
+    return r
+
+
+SHAPES = [  # G, W, n, vocab: a wave's end; four waves'; several parts; many parts
+    (2, 3, 4, 5003),
+    (2, 9, 20, 9001),
+    (1, 2, 5, 70001),
+]
+
+
+@pytest.mark.parametrize("mask,dtype", [(m, d) for d in ("f32", "bf16") for m in (-1e4, -1e6, -1e8, -1e9, -1e10, -1e15, -1e20, -1e30, -1e38)] +
+                         [(-1e4, "f16"), (-6e4, "f16")])
+@pytest.mark.parametrize("left", ["half", "a part", "few", "one", "one behind the last whole group", "none"])
+def test_select_finite_masks(ctx, mask, dtype, left):
+    """Rows masked with a finite number: whole lanes and whole parts of it, all but some tokens, and all."""
+    import torch
+
+    log("finite mask", mask, dtype, left)
+    for G, W, n, vocab in SHAPES:
+        rng = np.random.default_rng(vocab + W)
+        x = rng.normal(0, 3, (G * W, vocab)).astype(np.float32)
+        keep = np.zeros(x.shape, bool)
+        if left == "half":
+            keep[:, vocab // 2:] = True
+        elif left == "a part":
+            keep[:, 4096:4200] = True
+        elif left == "few":
+            keep[np.arange(G * W)[:, None], rng.integers(0, vocab, (G * W, 7))] = True
+        elif left == "one":
+            keep[np.arange(G * W), rng.integers(0, vocab, G * W)] = True
+        elif left != "none":
+            keep[:, -1] = True
+        x = torch.from_numpy(np.where(keep, x, np.float32(mask))).cuda().to(torch_type(dtype))
+        scores = -rng.uniform(1, 5, (G, W)).astype(np.float32)
+        check(ctx, x, scores, n, dtype, [vocab - 2, 4100])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shift", [1e4, 11356.0, 11357.0, 1.2e4, 1e5, 1e6, 1e8, 1e15, 1e20, 1e30, 3e38])
+def test_select_large_logits(ctx, shift, dtype):
+    """Rows that are large throughout, in either sign, on both sides of what the kernel's shorter exponential serves."""
+    import torch
+
+    log("large logits", shift, dtype)
+    for G, W, n, vocab in SHAPES:
+        rng = np.random.default_rng(vocab)
+        x = rng.normal(0, 3, (G * W, vocab)).astype(np.float32)
+        with np.errstate(over="ignore"):
+            x += np.where(np.arange(G * W)[:, None] % 2 == 0, shift, -shift).astype(np.float32)
+        x = torch.from_numpy(x).cuda().to(torch_type(dtype))
+        check(ctx, x, -rng.uniform(1, 5, (G, W)).astype(np.float32), n, dtype, [3])
+
+
+def test_select_mixed_masks_in_many_rows(ctx):
+    """A part a row (more rows than workgroups of four a CU): every row with a mask of its own."""
+    import torch
+
+    log("mixed masks")
+    G, W, n, vocab = 150, 8, 8, 4999
+    rng = np.random.default_rng(2)
+    masks = np.array([-1e4, -1e9, -1e10, -1e30, -1e38, -3e38, -INF, 0.0], np.float32)[rng.integers(0, 8, G * W)]
+    x = rng.normal(0, 3, (G * W, vocab)).astype(np.float32)
+    x = np.where(rng.random(x.shape) < 0.01, x, masks[:, None])
+    check(ctx, torch.from_numpy(x).cuda(), -rng.uniform(1, 5, (G, W)).astype(np.float32), n, "f32", [7])

@@ -248,14 +248,15 @@ __global__ __launch_bounds__(kNt, 4) void k_beam(BeamArgs a) {
       }
       const float mx = fmaxf(fmaxf(gm[0], gm[1]), fmaxf(gm[2], gm[3]));
       const float m = fmaxf(z.m, mx), rel = m == -INFINITY ? 0.0f : m;  // of -inf alone: exp(-inf - 0) = 0, and NaN stays
-      // exp(x - rel) as 2^(x log2e - r), one operation less a logit; r is rel log2e rounded, which the sum makes good
+      // exp(x - rel) as 2^(x log2e - r), one operation less a logit. r is rel log2e rounded, off by d, and the sum's 2^d is
+      // made good by its first two terms: below 2^14 d is at most 2^-11, and the third one 2^-24
       const float r2 = rel * kLog2e;
       float s = 0.0f;
-      if (!__ballot(!(fabsf(r2) < 3e38f))) {
+      if (!__ballot(!(fabsf(r2) < 16384.0f))) {
 #pragma unroll
         for (int k = 0; k < G * N; ++k) s += __builtin_amdgcn_exp2f(fmaf(v[k], kLog2e, -r2));
         s = fmaf(s, -0.693147181f * fmaf(rel, kLog2e, -r2), s);
-      } else {  // infinite or next to it
+      } else {  // large, as where all of a lane's logits are masked by a finite number, or infinite
 #pragma unroll
         for (int k = 0; k < G * N; ++k) s += exp_rel(v[k], rel);
       }
