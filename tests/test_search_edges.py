@@ -124,3 +124,26 @@ def test_select_mixed_masks_in_many_rows(ctx):
     x = rng.normal(0, 3, (G * W, vocab)).astype(np.float32)
     x = np.where(rng.random(x.shape) < 0.01, x, masks[:, None])
     check(ctx, torch.from_numpy(x).cuda(), -rng.uniform(1, 5, (G, W)).astype(np.float32), n, "f32", [7])
+
+
+# ---- a cache in pages ------------------------------------------------------------------------------------
+
+
+def test_pages_rows_that_together_ask_for_more_than_32_bits_count(ctx):
+    """1,024 rows that ask for 2^21 pages each and more: rows that fit get their pages, all others none."""
+    import torch
+
+    P, R, cap = 1000, 1024, (1 << 21) + 8192
+    start = V.Pages.empty(1, 1, P, 1)
+    to = V.Pages(torch.empty(R, cap, dtype=torch.int32, device="cuda"), i32(np.zeros(R)), i32(np.zeros(P)), 1)
+    want = np.full(R, cap)
+    want[:2] = 5, 7
+    assert int(want.sum()) >= 1 << 31
+    log("more than 32 bits count")
+    got, ok = ctx.pages_step(start, i32(np.full(R, -1)), i32(want), out=to)
+    fits = np.cumsum(want) <= P
+    assert ok.cpu().numpy().tolist() == fits.astype(int).tolist()
+    assert got.lens.cpu().numpy().tolist() == np.where(fits, want, 0).tolist()
+    assert got.ref.cpu().numpy().tolist() == [1] * 12 + [0] * (P - 12)
+    assert got.table[0, :5].tolist() == [0, 1, 2, 3, 4] and got.table[1, :7].tolist() == [5, 6, 7, 8, 9, 10, 11]
+    assert int((got.table >= 0).sum()) == 12

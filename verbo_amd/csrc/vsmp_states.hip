@@ -499,7 +499,8 @@ __global__ __launch_bounds__(kTakeNt) void k_pages_small(PageArgs a) {
   __syncthreads();
   const bool away = begun >= 0 && (agent_load(&a.to.ref[begun]) != writers ||
                                    order != (static_cast<unsigned long long>(r.len) << 32 | static_cast<uint32_t>(~tid)));
-  const int first = pages_of(r.len, T) - away, need = r.want > r.len ? pages_of(r.want, T) - first : 0;
+  // (a need of more than the pool has is as good as any that it does not meet: 1,024 of them fit 31 bits)
+  const int first = pages_of(r.len, T) - away, need = r.want > r.len ? min(pages_of(r.want, T) - first, kSmallPages + 1) : 0;
   int sum[2] = {need, tid < words ? static_cast<int>(__popcll(s_bits[tid])) : 0}, all[2];
   scan_before<2>(sum, all);
   const int asked = all[0], n_free = all[1], start = sum[0], before = sum[1];
