@@ -184,3 +184,64 @@ def test_search_of_width_one_is_greedy():
     got = decode.BeamDecoder(1, 64).search(prompts, own, 7)
     want = decode.BatchDecoder([decode.Opts(max_tokens=7, temp=0.0)] * 2, 64).generate(prompts, batch)
     assert [r[0][0] for r in got] == [t for t, _ in want]
+
+
+def holders(pages):
+    """How many rows hold each page, from the tables."""
+    table, lens = pages.table.cpu().numpy(), pages.lens.cpu().numpy()
+    out = np.zeros(pages.ref.numel(), int)
+    for row, n in zip(table, lens):
+        np.add.at(out, row[:-(-int(n) // pages.page_tokens)], 1)
+    return out
+
+
+@pytest.mark.gpu
+def test_the_state_of_a_search_that_raised_owns_its_pages():
+    """One search ends at once and its pages go to the other's beams, then the pool is short: what self.pages holds is
+    the state whose rows own the pages, and giving those rows up empties the pool."""
+    import torch
+
+    prompts = [[1, 2, 3], [4, 5, 6]]
+
+    def logits(ids):
+        x = model(30, 2)(ids)
+        if len(ids) == 3 and ids[0] == 1:
+            x[[7, 8]] = 50.0  # both beams of the first prompt end here
+        return x
+
+    m = Recall(logits, prompts, 2, 6, True, page=1)
+    m.vocab = 30
+    P = 10  # three tokens of each prompt, and four more
+    ctx = V.Context(0)
+    m.pool = torch.full((P, 1, 1), -5, dtype=torch.int32, device="cuda")
+    m.cache = V.Planes([m.pool], token_dim=1)
+    m.start, ok = ctx.pages_step(V.Pages.empty(2, 10, P, 1), add=3)
+    assert bool(ok.all()) and m.start.table[0, :3].tolist() == [0, 1, 2]
+    m.pool[:6, 0, 0] = torch.tensor(prompts[0] + prompts[1], dtype=torch.int32, device="cuda")
+    dec = decode.BeamDecoder(2, 30)
+    with pytest.raises(V.VsmpError, match="no page left"):
+        dec.search(prompts, m, 20, stop_ids=(7, 8), pages=m.start, cache=m.cache)
+    assert dec.pages.lens[:2].tolist() == [0, 0] and dec.pages.lens[2:].min() > 3
+    assert dec.pages.ref.tolist() == holders(dec.pages).tolist()
+    gone, _ = ctx.pages_step(dec.pages, torch.full((4,), -1, dtype=torch.int32, device="cuda"))
+    assert int(gone.ref.abs().sum()) == 0
+
+
+@pytest.mark.gpu
+def test_the_state_of_a_search_whose_model_raised():
+    """An exception of logits_fn leaves self.pages at the state that it was called with."""
+    m = Recall(model(30, 3), [[1, 2, 3, 4, 5]], 3, 8, True)
+    m.vocab = 30
+    seen = []
+
+    def failing(step, tokens, pages):
+        seen.append(pages)
+        if step == 3:
+            raise KeyError("model")
+        return m(step, tokens, pages)
+
+    dec = decode.BeamDecoder(3, 30)
+    with pytest.raises(KeyError):
+        dec.search([[1, 2, 3, 4, 5]], failing, 8, pages=m.start, cache=m.cache)
+    assert dec.pages is seen[-1] and dec.pages.lens.tolist() == [8, 8, 8]
+    assert dec.pages.ref.tolist() == holders(dec.pages).tolist()

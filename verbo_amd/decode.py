@@ -329,7 +329,9 @@ class BeamDecoder:
         Planes whose rows are the pages, as Context.pages_step takes them. states: None, or a Planes of len(prompts) *
         width rows in which row j * width holds prompt j's state when the search begins (its tokens, where the planes
         have a token_dim); the rows follow their beams after every step. self.pages: the state that the search
-        ended with, all its rows given up."""
+        ended with, all its rows given up. Where the search raises (no page left, or out of logits_fn), it is the state
+        that the last step left, whose rows hold their pages until the caller gives them up; `pages` is not to be
+        used again: pages of its prompts may have been given up and written by other beams."""
         import torch
 
         dev = torch.device("cuda", self.device)
@@ -394,6 +396,7 @@ class BeamDecoder:
             if pages is not None:  # a beam that is not live, and all of a search that is over, give up their pages
                 go = tokens >= 0
                 pages, ok = ctx.pages_step(pages, torch.where(go, rows, -1), go.to(torch.int32), cache=cache)
+                self.pages = pages
                 if not bool(ok.all()):
                     raise VsmpError("the pool has no page left for a beam")
         if pages is not None:
