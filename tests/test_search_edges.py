@@ -147,3 +147,28 @@ def test_pages_rows_that_together_ask_for_more_than_32_bits_count(ctx):
     assert got.ref.cpu().numpy().tolist() == [1] * 12 + [0] * (P - 12)
     assert got.table[0, :5].tolist() == [0, 1, 2, 3, 4] and got.table[1, :7].tolist() == [5, 6, 7, 8, 9, 10, 11]
     assert int((got.table >= 0).sum()) == 12
+
+
+# ---- streams ---------------------------------------------------------------------------------------------
+
+
+def test_outputs_of_calls_on_the_default_stream_are_its_memory(ctx):
+    """From within another stream: once freed, the default stream's next tensor of that size takes the memory, and the
+    other stream's does not."""
+    import torch
+
+    G, n = 200_003, 8
+    x, scores = torch.randn(G, 9, device="cuda"), torch.full((G, 1), -1.0, device="cuda")
+    want = ctx.beam_select(x, scores, n)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    log("default stream")
+    with torch.cuda.stream(torch.cuda.Stream()):
+        got = ctx.beam_select(x, scores, n, stream=torch.cuda.default_stream())
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        at = got.token.data_ptr()
+        del got
+        other = torch.empty(6, G, n, dtype=torch.int32, device="cuda")
+    again = torch.empty(6, G, n, dtype=torch.int32, device="cuda")
+    assert other.data_ptr() != at and again.data_ptr() == at

@@ -343,7 +343,7 @@ class _Torch:
         self.codes = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # vsmp_dtype
         self._raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         self._current = torch.cuda.current_stream
-        self._use, self._external = torch.cuda.stream, torch.cuda.ExternalStream
+        self._use, self._external, self._default = torch.cuda.stream, torch.cuda.ExternalStream, torch.cuda.default_stream
 
     def stream(self, stream, device):
         """The address of `stream`, or of torch's current one on `device`."""
@@ -351,14 +351,18 @@ class _Torch:
             return stream.cuda_stream
         return self._raw(device.index) if self._raw is not None else self._current(device).cuda_stream
 
+    def _at(self, address, device):
+        """The stream at an address: of a stream, the calls ask for no more than that. (Made from the default stream's,
+        0, an ExternalStream would be a new one.)"""
+        return self._external(address, device=device) if address else self._default(device)
+
     def output(self, shape, dtype, device, stream):
         """A new tensor that a call on `stream` (None: the current one) writes. On a stream of its own the call takes
         that stream's memory, since the current one may still be using what it has freed; once the tensor is freed,
         the memory waits for the work of both."""
         if stream is None or stream.cuda_stream == self.stream(None, device):
             return self.empty(shape, dtype=dtype, device=device)
-        # by its address: of a stream, the calls ask for no more than that
-        with self._use(self._external(stream.cuda_stream, device=device)):
+        with self._use(self._at(stream.cuda_stream, device)):
             t = self.empty(shape, dtype=dtype, device=device)
         t.record_stream(self._current(device))
         return t
