@@ -172,3 +172,50 @@ def test_outputs_of_calls_on_the_default_stream_are_its_memory(ctx):
         other = torch.empty(6, G, n, dtype=torch.int32, device="cuda")
     again = torch.empty(6, G, n, dtype=torch.int32, device="cuda")
     assert other.data_ptr() != at and again.data_ptr() == at
+
+
+@pytest.mark.parametrize("call", ["reorder", "step", "compact"])
+@pytest.mark.parametrize("how", ["argument", "current"])
+def test_planes_that_are_gone_before_their_call_has_run(ctx, call, how):
+    """Planes made on one stream and dropped after a call on another, which is busy: what is allocated then does not take
+    the addresses' memory, and the call finds them."""
+    import torch
+
+    st = torch.cuda.Stream()
+    a = torch.randn(4096, 4096, device="cuda")
+    x = torch.arange(4 * 6, dtype=torch.int32, device="cuda").view(4, 6, 1)
+    parent = i32([1, 1, 3, 2])
+    pages = V.Pages(i32([[3, -1], [3, 1]]), i32([3, 8]), i32([0, 1, 0, 2]), 6)
+    want = {"reorder": lambda: ctx.reorder_rows(V.Planes([x.clone()], token_dim=1), parent, 2),
+            "step": lambda: ctx.pages_step(pages, add=1, cache=V.Planes([x.clone()], token_dim=1))[0].table,
+            "compact": lambda: ctx.pages_compact(pages, cache=V.Planes([x.clone()], token_dim=1))[0].table}[call]()
+    planes = V.Planes([x], token_dim=1)
+    at = planes._ptrs.data_ptr()
+    log("gone", call, how)
+    b = a @ a
+    torch.cuda.synchronize()
+    with torch.cuda.stream(st):
+        for _ in range(100):
+            torch.mm(a, a, out=b)
+    if how == "current":
+        with torch.cuda.stream(st):
+            got = ctx.reorder_rows(planes, parent, 2) if call == "reorder" else \
+                (ctx.pages_step(pages, add=1, cache=planes) if call == "step" else ctx.pages_compact(pages, cache=planes))[0]
+    else:
+        got = ctx.reorder_rows(planes, parent, 2, stream=st) if call == "reorder" else \
+            (ctx.pages_step(pages, add=1, cache=planes, stream=st) if call == "step" else ctx.pages_compact(pages, cache=planes, stream=st))[0]
+    del planes
+    new = [torch.empty(1, dtype=torch.int64, device="cuda") for _ in range(100)]
+    busy = not st.query()
+    torch.cuda.synchronize()
+    assert busy and at not in [t.data_ptr() for t in new]
+    rows = x.view(4, 6).tolist()
+    was = np.arange(24).reshape(4, 6).tolist()
+    if call == "reorder":
+        assert rows == [was[k] for k in (1, 1, 3, 2)]
+    else:
+        assert torch.equal(got.table, want)
+        if call == "step":    # row 0 shares its begun page with a full one of row 1: it copies three tokens to page 0
+            assert rows == [was[3][:3] + was[0][3:]] + was[1:]
+        else:                 # pages 1 and 3 move to 1 and 0
+            assert rows == [was[3]] + was[1:]

@@ -483,7 +483,8 @@ row, both int32 [G, n]; score: float32 [G, n]) and those that a stop token ends 
 
 class Planes:
     """vsmp_planes: device tensors of one shape, strides and type whose rows (dimension 0) hold tokens, such as the keys
-    and values of every layer; kept by a program beside them. token_dim: the dimension that counts tokens, with a
+    and values of every layer. Making them uploads the tensors' addresses and waits for the current stream, so that a program
+    keeps them as long as the tensors, and as long as it replays graphs of calls with them. token_dim: the dimension that counts tokens, with a
     token's values side by side behind it and whole tokens one after the other; None: a row is one token, whole.
     Dimensions before it must have one stride in common (heads that lie apart)."""
 
@@ -538,9 +539,17 @@ class Planes:
         self._ptrs = torch.tensor([u.data_ptr() for u in self.tensors], dtype=torch.int64).to(t.device)
         # the addresses are there for every stream from here on
         torch.cuda.current_stream(t.device).synchronize()
+        self._stream = _t().stream(None, t.device)
         self._arg = _PlanesArg(self._ptrs.data_ptr(), len(self.tensors), shape[0], stride[0] * size if shape[0] > 1 else 0, outer[0],
                                outer[1] * size, tokens, token * size)
         self._addr = ctypes.addressof(self._arg)
+
+    def _on(self, address):
+        """The planes for a call on the stream at that address: where that is not the one they were made on, the addresses'
+        memory waits for it too when the planes are gone."""
+        if address != self._stream:
+            self._ptrs.record_stream(_t()._at(address, self.device))
+        return self._addr
 
 
 class Pages:
@@ -787,17 +796,18 @@ class Context:
         dev = planes.device
         if self.device >= 0 and dev.index != self.device:
             raise VsmpError(f"expected tensors on the context's device ({self.device})")
-        if _lib.vsmp_reorder_rows(self._h, planes._addr, _array_of(parent, T.int32, planes.rows, "parent", dev), int(width),
-                                  _array_of(lens, T.int32, planes.rows, "lens", dev), T.stream(stream, dev)) != 0:
+        st = T.stream(stream, dev)
+        if _lib.vsmp_reorder_rows(self._h, planes._on(st), _array_of(parent, T.int32, planes.rows, "parent", dev), int(width),
+                                  _array_of(lens, T.int32, planes.rows, "lens", dev), st) != 0:
             raise _err()
 
-    def _pages(self, pages, cache):
-        dev = pages.device
+    def _pages(self, pages, cache, stream):
+        dev, st = pages.device, _t().stream(stream, pages.device)
         if self.device >= 0 and dev.index != self.device:
             raise VsmpError(f"expected tensors on the context's device ({self.device})")
         if cache is not None and cache.device != dev:
             raise VsmpError("the cache must be on the pages' device")
-        return dev, cache._addr if cache is not None else None
+        return dev, st, cache._on(st) if cache is not None else None
 
     def pages_step(self, pages, parent=None, add=0, cache=None, out=None, stream=None):
         """vsmp_pages_step: the step of a cache in pages from the state `pages` (a Pages, left as it is). Row i takes the
@@ -807,7 +817,7 @@ class Context:
         next state (default: new, a row for each parent). Returns (the next state, ok int32 [rows]: 0 for a row that
         did not get its pages)."""
         T = _t()
-        dev, cp = self._pages(pages, cache)
+        dev, st, cp = self._pages(pages, cache, stream)
         if out is None:
             out = pages.like(None if parent is None else parent.numel(), stream)
         rows = out.lens.numel()
@@ -818,7 +828,7 @@ class Context:
         if out.device != dev:
             raise VsmpError("out must be on the pages' device")
         if _lib.vsmp_pages_step(self._h, pages._addr, out._addr, _array_of(parent, T.int32, rows, "parent", dev),
-                                _array_of(add, T.int32, rows, "add", dev), every, cp, ok.data_ptr(), T.stream(stream, dev)) != 0:
+                                _array_of(add, T.int32, rows, "add", dev), every, cp, ok.data_ptr(), st) != 0:
             raise _err()
         return out, ok
 
@@ -827,14 +837,14 @@ class Context:
         is), in every plane of `cache`. Returns (the next state: `out`, or a new Pages; moved int32 [n_pages]: each
         page's new number, -1 for a free one; live int32 [1]: how many are in use)."""
         T = _t()
-        dev, cp = self._pages(pages, cache)
+        dev, st, cp = self._pages(pages, cache, stream)
         if out is None:
             out = pages.like(stream=stream)
         if out.device != dev:
             raise VsmpError("out must be on the pages' device")
         n = pages.ref.numel()
         moved, live = T.output((n,), T.int32, dev, stream), T.output((1,), T.int32, dev, stream)
-        if _lib.vsmp_pages_compact(self._h, pages._addr, out._addr, cp, moved.data_ptr(), live.data_ptr(), T.stream(stream, dev)) != 0:
+        if _lib.vsmp_pages_compact(self._h, pages._addr, out._addr, cp, moved.data_ptr(), live.data_ptr(), st) != 0:
             raise _err()
         return out, moved, live
 
