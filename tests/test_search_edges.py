@@ -219,3 +219,29 @@ def test_planes_that_are_gone_before_their_call_has_run(ctx, call, how):
             assert rows == [was[3][:3] + was[0][3:]] + was[1:]
         else:                 # pages 1 and 3 move to 1 and 0
             assert rows == [was[3]] + was[1:]
+
+
+# ---- numbers that a C int does not hold ------------------------------------------------------------------
+
+
+def test_numbers_beyond_32_bits(ctx):
+    """Refused, or, as stop tokens, outside the vocabulary: cut to 32 bits each of these would be a number that serves."""
+    import torch
+
+    x, scores = torch.zeros(4, 10, device="cuda"), torch.zeros(2, 2, device="cuda")
+    x[:, 3] = 5.0
+    log("numbers beyond 32 bits")
+    assert ctx.beam_select(x, scores, stop_ids=[(1 << 32) + 3, -(1 << 32) + 3, 1 << 40]).n_end.tolist() == [0, 0]
+    state = torch.zeros(4, 6, dtype=torch.int32, device="cuda")
+    parent, pages = i32([1, 0, 2, 3]), V.Pages.empty(4, 4, 16, 4)
+    wide = torch.empty(2, (1 << 30) + 16, device="cuda")  # rows of 2^32 + 64 bytes
+    for make in (lambda: ctx.beam_select(x, scores, (1 << 32) + 2), lambda: ctx.reorder_rows(V.Planes([state]), parent, (1 << 32) + 2),
+                 lambda: V.Planes([wide]), lambda: V.Planes([wide.view(torch.uint8)]),
+                 lambda: V.Pages(pages.table, pages.lens, pages.ref, (1 << 32) + 4), lambda: ctx.pages_step(pages, add=1 << 31),
+                 lambda: ctx.pages_step(pages, add=(1 << 32) + 1), lambda: ctx.pages_step(pages, add=-(1 << 31) - 1)):
+        with pytest.raises(V.VsmpError, match="32 bits"):
+            make()
+    with pytest.raises(V.VsmpError):
+        V.Planes([wide.view(torch.uint8).view(2, -1, 1)], token_dim=1)
+    to, ok = ctx.pages_step(pages, add=(1 << 31) - 1)
+    assert ok.tolist() == [0] * 4 and to.lens.tolist() == [0] * 4

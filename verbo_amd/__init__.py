@@ -407,6 +407,14 @@ def _array_of(t, dtype, n, name, device):
     return t.data_ptr()
 
 
+def _int32(v, name):
+    """v as an int that a C int holds (ctypes would cut it)."""
+    v = int(v)
+    if not -1 << 31 <= v < 1 << 31:
+        raise VsmpError(f"{name} must fit 32 bits")
+    return v
+
+
 def _penalty_rows(rows):
     """A PENALTY_DTYPE array of such an array or of a list of Penalty, each of them what a shared one has to be."""
     if not isinstance(rows, np.ndarray):
@@ -535,6 +543,8 @@ class Planes:
             raise VsmpError("a token's values must lie side by side, and tokens one after the other")
         if outer is None:
             raise VsmpError("the dimensions before the tokens must have one stride in common")
+        for v, name in ((shape[0], "rows"), (outer[0], "pieces"), (tokens, "tokens"), (token * size, "a token's bytes")):
+            _int32(v, name)
         self.device, self.rows, self.tokens, self.token_dim = t.device, shape[0], tokens, dim
         self._ptrs = torch.tensor([u.data_ptr() for u in self.tensors], dtype=torch.int64).to(t.device)
         # the addresses are there for every stream from here on
@@ -569,9 +579,9 @@ class Pages:
             _array_of(t, T.int32, rows if name == "lens" else 1, name, dev)
         if lens.numel() != rows:
             raise VsmpError("lens must hold an entry for each row of the table")
-        self.table, self.lens, self.ref, self.page_tokens, self.device = table, lens, ref, int(page_tokens), dev
-        self._arg = _PagesArg(rows, cap, ref.numel(), self.page_tokens, table.data_ptr(), table.stride(0) if rows > 1 else cap,
-                              lens.data_ptr(), ref.data_ptr())
+        self.table, self.lens, self.ref, self.page_tokens, self.device = table, lens, ref, _int32(page_tokens, "page_tokens"), dev
+        self._arg = _PagesArg(_int32(rows, "rows"), _int32(cap, "row_pages"), _int32(ref.numel(), "n_pages"), self.page_tokens,
+                              table.data_ptr(), table.stride(0) if rows > 1 else cap, lens.data_ptr(), ref.data_ptr())
         self._addr = ctypes.addressof(self._arg)
 
     @classmethod
@@ -774,10 +784,12 @@ class Context:
         if scores.dim() != 2 or scores.numel() != B:
             raise VsmpError("scores must be a float32 tensor [G, W] with an entry for each row of logits")
         G, W = scores.shape
-        n = W if n is None else int(n)
+        n = W if n is None else _int32(n, "n")
         if n < 1:
             raise VsmpError("need n >= 1 beams of the next step")
-        stops = (ctypes.c_int * len(stop_ids))(*stop_ids) if len(stop_ids) else None
+        _int32(max(B, V), "logits' sizes")
+        # (those outside the vocabulary end nothing, also where a C int would not hold them)
+        stops = (ctypes.c_int * len(stop_ids))(*[t if 0 <= t < V else -1 for t in stop_ids]) if len(stop_ids) else None
         sp = _array_of(scores, T.float32, B, "scores", dev)
         token, parent, end_token, end_parent, score, end_score = T.output((6, G, n), T.int32, dev, stream).unbind(0)
         n_end = T.output((G,), T.int32, dev, stream)
@@ -797,7 +809,7 @@ class Context:
         if self.device >= 0 and dev.index != self.device:
             raise VsmpError(f"expected tensors on the context's device ({self.device})")
         st = T.stream(stream, dev)
-        if _lib.vsmp_reorder_rows(self._h, planes._on(st), _array_of(parent, T.int32, planes.rows, "parent", dev), int(width),
+        if _lib.vsmp_reorder_rows(self._h, planes._on(st), _array_of(parent, T.int32, planes.rows, "parent", dev), _int32(width, "width"),
                                   _array_of(lens, T.int32, planes.rows, "lens", dev), st) != 0:
             raise _err()
 
@@ -823,7 +835,7 @@ class Context:
         rows = out.lens.numel()
         every = 0
         if not hasattr(add, "data_ptr"):
-            add, every = None, int(add)
+            add, every = None, _int32(add, "add")
         ok = T.output((rows,), T.int32, dev, stream)
         if out.device != dev:
             raise VsmpError("out must be on the pages' device")
