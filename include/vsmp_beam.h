@@ -91,8 +91,11 @@ typedef struct {
  *       if all that hold it are rows that grow in it in this step, the one with the most tokens (the lowest row among
  *       those) keeps it; every other row, and all of them if anyone else holds it, gets a page of its own, into
  *       which the begun page's tokens are copied in every plane of `cache`.
- * A row for which there are not enough free pages left after the rows before it, or not enough room in the table,
- * holds its parent's L tokens and shares its pages (ok 0).
+ * A row for which there are not enough free pages left after what the rows before it ask for, or not enough room in the
+ * table, holds its parent's L tokens and shares its pages (ok 0). What a row asks for in vain counts for the rows behind
+ * it: from the first one on that the pool has too few pages for, all that need a page get none in this step (rows that
+ * need none go on; a row without room in the table asks for none). So a prompt that may not fit goes into the last
+ * rows, or into a step of its own.
  *   from, to: HOST pointers; the same n_pages and page_tokens, to->row_pages >= from->row_pages, no array of one
  *       overlapping the other's. to->table is written whole (-1 behind a row's pages), as are to->lens and to->ref.
  *       A page that only rows given up in this step held is free in it, and may be given out and written again.

@@ -149,6 +149,23 @@ def test_pages_rows_that_together_ask_for_more_than_32_bits_count(ctx):
     assert int((got.table >= 0).sum()) == 12
 
 
+@pytest.mark.parametrize("rows,n_pages", [(6, 40), (64, 100), (200, 300), (6, 65537), (1025, 300)])
+def test_pages_that_a_row_asked_for_in_vain_count(ctx, rows, n_pages):
+    """Behind a row that the pool has too few pages for, rows that need a page get none, and rows that need none, or are cut,
+    go on; a row that the table has too little room for asks for none."""
+    cap, T = n_pages + 8, 2
+    table = np.full((rows, cap), -1, np.int32)
+    table[:, 0] = np.arange(rows) % n_pages  # where there are more rows than pages they share them
+    start = V.Pages(i32(table), i32(np.full(rows, 1)), i32(np.bincount(table[:, 0], minlength=n_pages)), T)
+    add = np.zeros(rows, int)
+    add[:6] = 2 * cap, n_pages * T if rows < n_pages else 0, 2, 1, 0, -1
+    log("asked for in vain", rows, n_pages)
+    to, ok = ctx.pages_step(start, add=i32(add))
+    m = [0, 0, 0, 1, 1, 1] if rows < n_pages else [0, 1, 0, 0, 1, 1]
+    assert ok.cpu().numpy()[:6].tolist() == m and bool(ok[6:].all())
+    assert to.lens.cpu().numpy()[:6].tolist() == [1 + int(a) * o for a, o in zip(add, m)]
+
+
 # ---- streams ---------------------------------------------------------------------------------------------
 
 

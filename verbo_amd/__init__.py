@@ -827,7 +827,7 @@ class Context:
         grows by add[i] tokens, or is cut by -add[i] (an int32 tensor, or an int for every row). cache: a Planes whose
         rows are the pages, so that begun pages which rows share are copied; None: tables alone. out: a Pages for the
         next state (default: new, a row for each parent). Returns (the next state, ok int32 [rows]: 0 for a row that
-        did not get its pages)."""
+        did not get its pages; from the first row on that the pool has too few for, no row gets any in that step)."""
         T = _t()
         dev, st, cp = self._pages(pages, cache, stream)
         if out is None:
