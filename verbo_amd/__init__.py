@@ -484,6 +484,7 @@ def _adjust_args(logits, penalty, hist, hist_off, prompt_len, bias_ids, bias, bi
     return (logits.data_ptr(), code, ld), (B, V), (pp, per_row), (h, ho), rest, out
 
 
+_Stops = ctypes.c_int * 16  # the most stop tokens of a selection
 BeamStep = namedtuple("BeamStep", "token parent score end_token end_parent end_score n_end")
 BeamStep.__doc__ = """What Context.beam_select returns: for each group the n best continuations that go on (token, parent: the
 row, both int32 [G, n]; score: float32 [G, n]) and those that a stop token ends (the same, n_end of them: int32 [G])."""
@@ -549,7 +550,7 @@ class Planes:
         self._ptrs = torch.tensor([u.data_ptr() for u in self.tensors], dtype=torch.int64).to(t.device)
         # the addresses are there for every stream from here on
         torch.cuda.current_stream(t.device).synchronize()
-        self._stream = _t().stream(None, t.device)
+        self._streams = {_t().stream(None, t.device)}
         self._arg = _PlanesArg(self._ptrs.data_ptr(), len(self.tensors), shape[0], stride[0] * size if shape[0] > 1 else 0, outer[0],
                                outer[1] * size, tokens, token * size)
         self._addr = ctypes.addressof(self._arg)
@@ -557,8 +558,9 @@ class Planes:
     def _on(self, address):
         """The planes for a call on the stream at that address: where that is not the one they were made on, the addresses'
         memory waits for it too when the planes are gone."""
-        if address != self._stream:
+        if address not in self._streams:
             self._ptrs.record_stream(_t()._at(address, self.device))
+            self._streams.add(address)
         return self._addr
 
 
@@ -784,17 +786,19 @@ class Context:
         if scores.dim() != 2 or scores.numel() != B:
             raise VsmpError("scores must be a float32 tensor [G, W] with an entry for each row of logits")
         G, W = scores.shape
-        n = W if n is None else _int32(n, "n")
+        n = W if n is None else int(n)
         if n < 1:
             raise VsmpError("need n >= 1 beams of the next step")
-        _int32(max(B, V), "logits' sizes")
+        if (B | V | n) >> 31:
+            raise VsmpError("logits' sizes and n must fit 32 bits")
+        ns = len(stop_ids)
         # (those outside the vocabulary end nothing, also where a C int would not hold them)
-        stops = (ctypes.c_int * len(stop_ids))(*[t if 0 <= t < V else -1 for t in stop_ids]) if len(stop_ids) else None
+        stops = (_Stops if ns <= 16 else ctypes.c_int * ns)(*[t if 0 <= t < V else -1 for t in stop_ids]) if ns else None
         sp = _array_of(scores, T.float32, B, "scores", dev)
         token, parent, end_token, end_parent, score, end_score = T.output((6, G, n), T.int32, dev, stream).unbind(0)
         n_end = T.output((G,), T.int32, dev, stream)
         p, k = token.data_ptr(), 4 * G * n  # the six lie one after the other
-        if _lib.vsmp_beam_select(self._h, logits.data_ptr(), code, ld, G, W, V, sp, n, stops, len(stop_ids), p, p + k, p + 4 * k, p + 2 * k,
+        if _lib.vsmp_beam_select(self._h, logits.data_ptr(), code, ld, G, W, V, sp, n, stops, ns, p, p + k, p + 4 * k, p + 2 * k,
                                  p + 3 * k, p + 5 * k, n_end.data_ptr(), T.stream(stream, dev)) != 0:
             raise _err()
         score, end_score = score.view(T.float32), end_score.view(T.float32)
