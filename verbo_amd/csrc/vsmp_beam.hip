@@ -140,8 +140,10 @@ constexpr int kWait = 144;     // logits that a wave has collected: 64 that wait
 // those of a wave's threads; several of each list where there are few) is a bound for all entries. Where more entries than
 // kCands reach it (many equal ones) each wave merges lists in order instead, and the first wave the waves'.
 //
-// Many rows are bound by the logits' read, in bf16 and f16 by the exponentials too: 64 groups of 8 rows of 128,256 fp32 49.4
-// us (5.3 TB/s), 64 of 16 of 151,936 bf16 73 us (4.3 TB/s; 80 with each wave's own bound). A few rows are bound by latencies that follow one another: one
+// Many fp32 rows are bound by the logits' read: 64 groups of 8 rows of 128,256 49.4 us (5.3 TB/s; 8 vector instructions a
+// logit, the waves wait for memory half of their time). bf16 by vector instructions: 64 of 16 of 151,936 73 us (4.3 TB/s; 13 a
+// logit at N = 16, active in a third of each wave's time, with four waves a SIMD; 80 us with each wave's own bound). f16
+// of the same size takes 94 us with as many instructions: the waves wait for loads two thirds of their time. A few rows are bound by latencies that follow one another: one
 // group of 4 rows of 49,152 fp32 10.4 us, of which the logits' load and sums take about 3, a part's ranks and their way to
 // memory 2, the ticket 1, the last part's loads 1, and its sums, bound and ranks 3. Every workgroup runs most of the code
 // once; loops stay rolled where they hardly turn, and nothing is divided by what is not a constant. Sorting networks and

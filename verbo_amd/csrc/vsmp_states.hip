@@ -377,7 +377,9 @@ __global__ __launch_bounds__(kTakeNt) void k_pages_take(PageArgs a) {
 // Bound by loads that follow one another (parent, length, table entry; ticket; bits and lists; ref; the pages' stores): 4 rows
 // over 256 pages 7.9 us in one workgroup, 64 rows over 2,048 pages 10.8 us, the copies a launch more. Pages that many rows
 // change at once cost the last workgroup scattered loads and stores (256 rows of which 16 end, 1,300 pages: 19 us); there,
-// from kSmallEntries table entries on, the tables have a launch of their own (3.2 us and 10.4).
+// beyond kSmallEntries table entries, the tables have a launch of their own (3.2 us and 10.4). Tables alone, calls through Python,
+// which take 9.7 us at the least, in one launch and in two: 1,024 entries 9.7 and 9.7, 4,096 10.5 and 9.9, 8,192 11.7 and 10.1,
+// 16,384 14.7 and 10.4, 65,536 28.6 and 11.1. So two are level or better from some 4,096 on; the limit is above that.
 constexpr int kSmallPages = 64 * kTakeNt, kSmallEntries = 1 << 13;
 template <bool WHOLE>
 __global__ __launch_bounds__(kTakeNt) void k_pages_small(PageArgs a) {
